@@ -36,6 +36,22 @@ class NormFusion(C.Structure):
                 ("scale", Tensor), ("rows_per_sequence", C.c_int32), ("source_rows", C.c_void_p)]
 
 
+class Cache(C.Structure):
+    _fields_ = [("keys", C.c_void_p), ("values", C.c_void_p), ("key_scales", C.c_void_p), ("value_scales", C.c_void_p),
+                ("pages", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32),
+                ("type", C.c_int32), ("device", C.c_int32)]
+
+
+class RotaryPlan(C.Structure):
+    _fields_ = [("turns", C.c_void_p), ("dims", C.c_int32), ("interleaved", C.c_int32), ("scale", C.c_float),
+                ("device", C.c_int32)]
+
+
+class Attention(C.Structure):
+    _fields_ = [("queries", Tensor), ("output", Tensor), ("pages", Tensor), ("lengths", Tensor), ("query_offsets", Tensor),
+                ("prefix_pages", Tensor), ("prefix_length", Tensor), ("scale", C.c_float)]
+
+
 class Path_(C.Structure):
     _fields_ = [("kind", C.c_int32), ("tokens", C.c_int32), ("channels", C.c_int32), ("splits", C.c_int32)]
 
@@ -43,6 +59,7 @@ class Path_(C.Structure):
 _ERR = (C.c_char_p, C.c_size_t)
 _PT, _PR, _PE, _PP = C.POINTER(Tensor), C.POINTER(RowScaled), C.POINTER(Epilogue), C.POINTER(Path_)
 _PF = C.POINTER(NormFusion)
+_PC, _PO = C.POINTER(Cache), C.POINTER(RotaryPlan)
 
 # name -> (restype, argtypes); the single source of truth the symbol-export test checks against.
 SIGNATURES = {
@@ -65,6 +82,14 @@ SIGNATURES = {
     "b200q_layer_norm_quantize": (C.c_int, (C.c_void_p, _PT, _PR, _PT, _PT, C.c_float, _PF, _PT, *_ERR)),
     "b200q_normalized_linear": (C.c_int, (C.c_void_p, _PT, _PR, _PT, _PT, _PT, _PT, _PT, C.c_float, _PF, _PE, _PR,
                                           C.POINTER(C.c_int32), *_ERR)),
+    "b200q_rotary_turns": (C.c_int, (C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_double,
+                                     C.POINTER(C.c_double), C.POINTER(C.c_float), *_ERR)),
+    "b200q_rotary": (C.c_int, (C.c_void_p, _PT, _PT, _PO, C.c_int32, _PT, *_ERR)),
+    "b200q_cache_write": (C.c_int, (C.c_void_p, _PC, _PT, _PT, _PT, _PT, _PO, _PT, _PT, _PT, _PT, C.c_float, *_ERR)),
+    "b200q_cache_read": (C.c_int, (C.c_void_p, _PC, _PT, _PT, _PT, *_ERR)),
+    "b200q_cached_attention": (C.c_int, (C.c_void_p, _PC, C.POINTER(Attention), *_ERR)),
+    "b200q_attention_workspace": (C.c_int, (C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                            C.POINTER(C.c_size_t), *_ERR)),
     "b200q_linear_layer_create": (C.c_int, (C.c_void_p, _PT, C.c_int32, _PT, C.POINTER(C.c_void_p), *_ERR)),
     "b200q_linear_layer_destroy": (None, (C.c_void_p,)),
     "b200q_linear_layer_prepare": (C.c_int, (C.c_void_p, C.c_void_p, C.c_int32, *_ERR)),

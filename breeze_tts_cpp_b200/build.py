@@ -39,6 +39,9 @@ SOURCES = [
     ("ops/sequence.cpp", []),
     ("kernels/sequence_pointwise.cu", ["--fmad=false"]),
     ("kernels/sequence_norm.cu", ["--fmad=false"]),
+    ("kernels/rotary_cache.cu", []),
+    ("kernels/cached_attention.cu", []),
+    ("ops/attention.cpp", []),
     ("layers/linear.cpp", []),
     ("c_api.cpp", []),
 ]

@@ -3,6 +3,7 @@
 #include "b200q.h"
 #include "c_api_convert.h"
 #include "kernels/quant_dispatch.h"
+#include "ops/attention.h"
 #include "ops/context.h"
 #include "ops/ops.h"
 #include "layers/linear.h"
@@ -43,8 +44,10 @@ CudaContext &context_of(b200q_context *c) {
     if (!c || !c->gpu) throw std::invalid_argument("null b200q context");
     return *c->gpu;
 }
+using capi::cache_of;
 using capi::epilogue_of;
 using capi::fusion_of;
+using capi::rotary_of;
 using capi::scaled_of;
 using capi::type_of;
 using capi::view_of;
@@ -312,6 +315,59 @@ int b200q_inject_wait_expiry(int32_t extra_bytes, int64_t limit_cycles, char *er
 int b200q_inject_refill_delay(int32_t nanoseconds, char *error, size_t capacity) {
     return guarded(error, capacity, [&] { quant_linear_inject_refill_delay(nanoseconds); });
 }
+int b200q_rotary_turns(int32_t dims, double base, int32_t scaling, double factor, int32_t original_length, double low, double high,
+                       double *turns, float *scale, char *error, size_t capacity) {
+    return guarded(error, capacity, [&] {
+        if (!scale) throw std::invalid_argument("null scale");
+        if (scaling < 0 || scaling > int(ops::RotaryScaling::Wavelength)) throw std::invalid_argument("invalid rotary scaling");
+        *scale = ops::rotary_turns({dims, base, factor, ops::RotaryScaling(scaling), original_length, low, high}, turns);
+    });
+}
+int b200q_rotary(b200q_context *c, const b200q_tensor *input, const b200q_tensor *positions, const b200q_rotary_plan *plan, int32_t head_dim,
+                 const b200q_tensor *output, char *error, size_t capacity) {
+    return guarded(error, capacity, [&] {
+        ops::validate_rotary(view_of(input), view_of(positions), rotary_of(plan), head_dim, view_of(output));
+        ExecutionScope scope(context_of(c));
+        ops::rotary(view_of(input), view_of(positions), rotary_of(plan), head_dim, view_of(output));
+    });
+}
+int b200q_cache_write(b200q_context *c, const b200q_cache *cache, const b200q_tensor *keys, const b200q_tensor *values, const b200q_tensor *slots,
+                      const b200q_tensor *positions, const b200q_rotary_plan *plan, const b200q_tensor *queries, const b200q_tensor *query_output,
+                      const b200q_tensor *query_norm, const b200q_tensor *key_norm, float epsilon, char *error, size_t capacity) {
+    return guarded(error, capacity, [&] {
+        ops::validate_cache_write(cache_of(cache), view_of(keys), view_of(values), view_of(slots), view_of(positions), rotary_of(plan),
+                                  view_of(queries), view_of(query_output), view_of(query_norm), view_of(key_norm), epsilon);
+        ExecutionScope scope(context_of(c));
+        ops::cache_write(cache_of(cache), view_of(keys), view_of(values), view_of(slots), view_of(positions), rotary_of(plan), view_of(queries),
+                         view_of(query_output), view_of(query_norm), view_of(key_norm), epsilon);
+    });
+}
+int b200q_cache_read(b200q_context *c, const b200q_cache *cache, const b200q_tensor *slots, const b200q_tensor *keys, const b200q_tensor *values,
+                     char *error, size_t capacity) {
+    return guarded(error, capacity, [&] {
+        ops::validate_cache_read(cache_of(cache), view_of(slots), view_of(keys), view_of(values));
+        ExecutionScope scope(context_of(c));
+        ops::cache_read(cache_of(cache), view_of(slots), view_of(keys), view_of(values));
+    });
+}
+int b200q_cached_attention(b200q_context *c, const b200q_cache *cache, const b200q_attention *a, char *error, size_t capacity) {
+    return guarded(error, capacity, [&] {
+        if (!a) throw std::invalid_argument("null attention arguments");
+        const ops::Attention arguments{view_of(&a->queries),       view_of(&a->output),       view_of(&a->pages),        view_of(&a->lengths),
+                                       view_of(&a->query_offsets), view_of(&a->prefix_pages), view_of(&a->prefix_length), a->scale};
+        ops::validate_cached_attention(cache_of(cache), arguments);
+        ExecutionScope scope(context_of(c));
+        ops::cached_attention(cache_of(cache), arguments);
+    });
+}
+int b200q_attention_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t prefix, int32_t multiprocessors,
+                              size_t *needed, char *error, size_t capacity) {
+    return guarded(error, capacity, [&] {
+        if (!needed) throw std::invalid_argument("null size");
+        *needed = ops::cached_attention_workspace(rows, heads, kv_heads, head_dim, prefix != 0, multiprocessors);
+    });
+}
+
 int b200q_status(b200q_context *c, int32_t *status, char *error, size_t capacity) {
     return guarded(error, capacity, [&] {
         auto &gpu = context_of(c);

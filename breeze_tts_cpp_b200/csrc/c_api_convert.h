@@ -1,6 +1,7 @@
 // POD structs of the C ABI -> the C++ value types of the library. Shared by every extern "C" source.
 #pragma once
 #include "b200q.h"
+#include "core/cache.h"
 #include "core/quantization.h"
 #include "ops/epilogue.h"
 #include "ops/sequence.h"
@@ -22,6 +23,14 @@ inline RowScaledView scaled_of(const b200q_row_scaled *r) {
     v.group_size = r->group_size;
     v.rotation_size = r->rotation_size;
     return v;
+}
+inline CacheView cache_of(const b200q_cache *c) {
+    if (!c) throw std::invalid_argument("null cache");
+    return {c->keys, c->values, c->key_scales, c->value_scales, c->pages, c->kv_heads, c->page_size, c->head_dim, type_of(c->type), c->device};
+}
+inline RotaryView rotary_of(const b200q_rotary_plan *r) {
+    if (!r) return {};
+    return {r->turns, r->dims, r->interleaved != 0, r->scale, r->device};
 }
 inline ops::Epilogue epilogue_of(const b200q_epilogue *e) {
     ops::Epilogue out;

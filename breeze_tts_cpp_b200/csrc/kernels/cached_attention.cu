@@ -1,0 +1,142 @@
+// Host side of the attention over the quantized cache: workspace, tensor maps, choice of the instance.
+#include "kernels/cached_attention.h"
+#include "kernels/cached_attention_sm100.cuh"
+#include "kernels/tensor_map.h"
+#include <algorithm>
+#include <climits>
+
+namespace tts {
+namespace {
+using namespace b200;
+
+int shift_of(int power) {
+    int s = 0;
+    while ((1 << s) < power) ++s;
+    return s;
+}
+CUtensorMap cache_map(const void *base, const CacheView &cache, int box_rows) {
+    CUtensorMap map;
+    cuuint64_t dims[2] = {cuuint64_t(cache.head_dim), cuuint64_t(cache.rows())};
+    cuuint64_t strides[1] = {cuuint64_t(cache.head_dim)};
+    cuuint32_t box[2] = {cuuint32_t(cache.head_dim), cuuint32_t(box_rows)};
+    cuuint32_t element_strides[2] = {1, 1};
+    CUresult status = encode_tiled()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides, box, element_strides,
+                                     CU_TENSOR_MAP_INTERLEAVE_NONE, cache.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (status != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled (cache) failed with code " + std::to_string(int(status)));
+    return map;
+}
+
+constexpr size_t kPiece = 256; // parts of the workspace start on multiples of this
+size_t padded(size_t bytes) { return (bytes + kPiece - 1) / kPiece * kPiece; }
+constexpr int kMostColumns = 16;
+
+// The workspace of one pass: the table, the parts, and for a shared prefix the rows that were done in one part.
+struct Carve {
+    size_t table, partials, complete, bytes;
+    Carve(int rows, int heads, int head_dim, bool prefix, int ctas) {
+        const size_t row = size_t(head_dim + kPartialExtra) * 4;
+        table = 0;
+        partials = padded(size_t(rows) * heads * sizeof(int4));
+        complete = partials + padded(size_t(ctas) * 2 * kMostColumns * row);
+        bytes = complete + (prefix ? padded(size_t(rows) * heads * row) : 0);
+    }
+};
+
+template <class T, Type F, int HeadDim, int Tiles>
+void launch_pass(const AttentionArgs &args, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
+    launch_pdl("cached attention", cached_attention<T, F, HeadDim, Tiles>, dim3(unsigned(ctas)), dim3(kAttentionThreads),
+               AttentionShape<HeadDim, Tiles>::smem, stream, keys, values, args);
+}
+template <class T, Type F, int HeadDim>
+void launch_pass(bool narrow, const AttentionArgs &args, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
+    if (narrow) launch_pass<T, F, HeadDim, 1>(args, keys, values, ctas, stream);
+    else launch_pass<T, F, HeadDim, 2>(args, keys, values, ctas, stream);
+}
+// Calls f(element, format, head width) with the run-time types as compile-time ones.
+template <class Call> void by_type(Type element, Type format, int head_dim, Call &&call) {
+    auto width = [&](auto t, auto f) {
+        if (head_dim == 64) call(t, f, std::integral_constant<int, 64>{});
+        else call(t, f, std::integral_constant<int, 128>{});
+    };
+    auto storage = [&](auto t) {
+        if (format == Type::I8) width(t, std::integral_constant<Type, Type::I8>{});
+        else width(t, std::integral_constant<Type, Type::FP8>{});
+    };
+    if (element == Type::F16) storage(__half{});
+    else storage(__nv_bfloat16{});
+}
+bool aligned16(const TensorView &v) {
+    return reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && (v.rows <= 1 || v.ld() % 8 == 0);
+}
+template <class T, Type F, int HeadDim> void raise_limit() {
+    for (auto [kernel, bytes] : {std::pair{cached_attention<T, F, HeadDim, 1>, AttentionShape<HeadDim, 1>::smem},
+                                 std::pair{cached_attention<T, F, HeadDim, 2>, AttentionShape<HeadDim, 2>::smem}}) {
+        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+        if (status != cudaSuccess) throw std::runtime_error(std::string("cudaFuncSetAttribute(attention): ") + cudaGetErrorString(status));
+    }
+}
+} // namespace
+
+void raise_attention_limits() {
+    for (Type element : {Type::F16, Type::BF16})
+        for (Type format : {Type::I8, Type::FP8})
+            for (int head_dim : {64, 128})
+                by_type(element, format, head_dim, [](auto t, auto f, auto width) { raise_limit<decltype(t), decltype(f)::value, decltype(width)::value>(); });
+}
+
+size_t attention_workspace_bytes(int rows, int heads, int, int head_dim, bool prefix, int multiprocessors) {
+    return Carve(rows, heads, head_dim, prefix, multiprocessors).bytes * (prefix ? 2 : 1);
+}
+
+void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t workspace_bytes, int *status, int multiprocessors,
+                             cudaStream_t stream) {
+    const int rows = p.queries.rows, head_dim = p.cache.head_dim, heads = p.queries.cols / head_dim, ctas = multiprocessors;
+    const bool prefix = p.prefix_pages != nullptr;
+    if (!rows) return;
+    const Carve carve(rows, heads, head_dim, prefix, ctas);
+    if (workspace_bytes < carve.bytes * (prefix ? 2 : 1)) throw std::invalid_argument("attention workspace is too small");
+
+    AttentionArgs args{};
+    args.queries = p.queries.data, args.output = p.output.data;
+    args.query_stride = p.queries.ld(), args.output_stride = p.output.ld();
+    args.rows = rows, args.heads = heads, args.kv_heads = p.cache.kv_heads, args.group = heads / p.cache.kv_heads;
+    args.aligned = aligned16(p.queries) && aligned16(p.output);
+    args.pages = p.pages, args.lengths = p.lengths, args.query_offsets = p.query_offsets;
+    args.sequences = p.sequences, args.page_columns = p.page_columns, args.page_stride = p.page_stride;
+    args.page_shift = shift_of(p.cache.page_size), args.total_pages = p.cache.pages, args.offset_count = p.sequences;
+    args.box_shift = std::min(args.page_shift, shift_of(kTileKeys));
+    args.key_scales = p.cache.key_scales, args.value_scales = p.cache.value_scales;
+    const float format = p.cache.type == Type::FP8 ? 256.f : 1.f; // e4m3 bytes enter the products times 2^-8
+    args.score_scale = p.scale * 1.4426950408889634f * format;
+    args.output_scale = format;
+    args.status = status;
+
+    CombineArgs combine{};
+    combine.sources = prefix ? 2 : 1, combine.rows = rows, combine.heads = heads, combine.output_stride = p.output.ld();
+    combine.row_count = p.query_offsets ? p.query_offsets + p.sequences : nullptr;
+    combine.output = p.output.data, combine.output_scale = format;
+    const CUtensorMap keys = cache_map(p.cache.keys, p.cache, 1 << args.box_shift), values = cache_map(p.cache.values, p.cache, 1 << args.box_shift);
+    by_type(p.queries.type, p.cache.type, head_dim, [&](auto element, auto format, auto width) {
+        using T = decltype(element);
+        for (int pass = 0; pass < combine.sources; ++pass) {
+            char *base = static_cast<char *>(workspace) + pass * carve.bytes;
+            args.table = reinterpret_cast<int4 *>(base + carve.table);
+            args.partials = reinterpret_cast<float *>(base + carve.partials);
+            args.complete = prefix ? reinterpret_cast<float *>(base + carve.complete) : nullptr;
+            // Eight query rows per segment, or sixteen where a sequence has more than eight: each cached byte is then widened for both halves.
+            bool narrow = args.group <= 8 && (!p.query_offsets || rows <= p.sequences);
+            if (pass) {
+                args.prefix = true;
+                args.pages = p.prefix_pages, args.lengths = p.prefix_length, args.sequences = 1;
+                args.page_columns = args.page_stride = p.prefix_columns;
+                narrow = (long long)rows * args.group <= 8;
+            }
+            launch_pass<T, decltype(format)::value, decltype(width)::value>(narrow, args, keys, values, ctas, stream);
+            combine.source[pass] = {args.partials, args.complete, args.table, ctas, narrow ? 8 : 16};
+        }
+        const long long warps = (long long)rows * heads;
+        launch_pdl("attention combine", combine_attention<T, decltype(width)::value>, dim3(unsigned((warps + 7) / 8)), dim3(256), 0, stream, combine);
+    });
+}
+} // namespace tts

@@ -2,15 +2,16 @@
 // launch. Drop-in for the reference launchers `launch_quant_linear` and `grouped_quant_gemm`
 // (src/ops/kernels/quant/quant_dispatch.cu:194-234, quant_grouped.cu:221-239).
 #include "kernels/quant_dispatch.h"
+#include "kernels/cached_attention.h"
 #include "kernels/launch.cuh"
 #include "kernels/quant_linear_dense.h"
 #include "kernels/quant_linear_sm100.cuh"
 #include "kernels/quant_prefill_pair_sm100.cuh"
 #include "kernels/quant_prefill_grouped_sm100.cuh"
+#include "kernels/tensor_map.h"
 #include "ops/epilogue.h"
 #include "ops/quantization_policy.h"
 #include <atomic>
-#include <cudaTypedefs.h>
 #include <map>
 #include <mutex>
 #include <stdexcept>
@@ -23,19 +24,6 @@ using namespace b200;
 void check(cudaError_t status, const char *what) {
     if (status != cudaSuccess)
         throw std::runtime_error(std::string(what) + ": " + cudaGetErrorString(status));
-}
-
-PFN_cuTensorMapEncodeTiled_v12000 encode_tiled() {
-    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-        void *entry = nullptr;
-        cudaDriverEntryPointQueryResult result{};
-        check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &entry, cudaEnableDefault, &result),
-              "cudaGetDriverEntryPoint(cuTensorMapEncodeTiled)");
-        if (!entry || result != cudaDriverEntryPointSuccess)
-            throw std::runtime_error("cuTensorMapEncodeTiled is unavailable in this driver");
-        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(entry);
-    }();
-    return fn;
 }
 
 // Tensor maps are returned by value (128 bytes, encoded on the host without a driver round trip):
@@ -260,6 +248,7 @@ void quant_linear_initialize(int device) {
     raise_limits<Type::I8>();
     raise_limits<Type::FP8>();
     raise_dense_limits();
+    raise_attention_limits();
     encode_tiled();
     check(cudaSetDevice(current), "cudaSetDevice");
     done[device] = true;

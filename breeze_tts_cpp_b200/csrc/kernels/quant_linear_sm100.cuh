@@ -31,6 +31,7 @@
 //                    shared memory, and are finished token-row-wise so that every global access
 //                    (fp32 residual, bias, bf16 store) is a coalesced 16-byte vector.
 #pragma once
+#include "kernels/quant_linear_workspace.h"
 #include "kernels/sm100_ptx.cuh"
 #include "kernels/quant_blocks.cuh"
 #include "kernels/quant_linear_geometry.h"
@@ -45,11 +46,7 @@ namespace tts::b200 {
 constexpr int kGemmThreads = 320;   // warp 0 TMA, warp 1 MMA + TMEM, warps 2-9 epilogue
 constexpr int kEpilogueThreads = 256;
 
-// Workspace carve-up (owner zeroes the first kWorkspaceHeader bytes once). The GEMM itself needs
-// no scratch; only the status word lives here.
-constexpr size_t kStatusOffset = 16384;    // int status[4]: nonzero after a bounded wait gave up
-constexpr size_t kSettleOffset = 16640;    // int: written by quant_linear_settle, read by nobody
-constexpr size_t kWorkspaceHeader = 32768;
+// The GEMM itself needs no scratch; of the workspace it uses the header's status word only.
 
 struct FusedEpilogue {
     const void *bias = nullptr;         // [N], output dtype

@@ -1,0 +1,374 @@
+// Rotary positions, and the quantized key/value cache: written from 16-bit rows, read back into them.
+//
+// Mathematics. Pair i of a head at position p turns by the angle 2 pi a, a = p * turns[i]: (x, y) -> (x c - y n, y c + x n) with
+// c = s cos 2 pi a, n = s sin 2 pi a. Positions reach 10^5 and more, where an fp32 product has lost every digit behind the point, so
+// p * turns[i] is taken in 64 bits and reduced to [-1/2, 1/2] there; sincospi works on the fp32 remainder. A stored row (one token,
+// one head) has one scale: amax / range, as for any row of this library (quant_codec.cuh). Everything between the load and the store
+// is fp32: a 16-bit rounding between the rotation and the quantizer would only add an error that nobody needs.
+//
+// All of it is bound by memory, or by latency where rows are few. A CTA takes one row of tokens: the angles of a row are the same
+// for all heads, so they are computed once, into shared memory, while the row's loads are in flight. A thread takes 16 columns of
+// a head, two blocks of eight that hold both partners of its pairs, so no pair crosses lanes; a head's scale and norm reduce over the 4
+// or 8 lanes that share it.
+#include "kernels/rotary_cache.h"
+#include "kernels/launch.cuh"
+#include "kernels/quant_codec.cuh"
+#include <algorithm>
+
+namespace tts {
+namespace {
+using namespace b200;
+
+constexpr int kMaxPairs = 256; // of a head of at most 512 columns
+
+__device__ __forceinline__ int load_index(const int *p) {
+    int v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+template <class T> __device__ __forceinline__ void store8(T *p, bool aligned, const float (&v)[8]) {
+    union {
+        uint4 word;
+        T e[8];
+    } out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.e[i] = T(v[i]);
+    if (aligned) {
+        *reinterpret_cast<uint4 *>(p) = out.word;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = out.e[i];
+    }
+}
+
+struct Turning {
+    const double *turns;
+    int half; // pairs; 0 = nothing turns
+    float scale;
+};
+// cos, sin of this CTA's position into shared memory; the caller synchronises.
+__device__ __forceinline__ void fill_angles(const Turning &t, int position, float2 *angles) {
+    for (int i = threadIdx.x; i < t.half; i += blockDim.x) {
+        const double a = double(position) * t.turns[i];
+        float s, c;
+        sincospif(2.f * float(a - rint(a)), &s, &c);
+        angles[i] = make_float2(t.scale * c, t.scale * s);
+    }
+}
+// The two blocks of eight columns that lane j of a head takes.
+template <bool Interleaved> __device__ __forceinline__ int2 blocks_of(int j, int half) {
+    if (!Interleaved && 8 * j < half) return make_int2(j, j + half / 8);
+    return make_int2(2 * j, 2 * j + 1); // half layout: what lies behind the turning columns
+}
+template <bool Interleaved>
+__device__ __forceinline__ void turn(float (&a)[8], float (&b)[8], int j, int2 block, int half, const float2 *angles) {
+    if (Interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (4 * block.x < half) {
+                const float2 w = angles[4 * block.x + i];
+                const float x = a[2 * i], y = a[2 * i + 1];
+                a[2 * i] = x * w.x - y * w.y;
+                a[2 * i + 1] = y * w.x + x * w.y;
+            }
+            if (4 * block.y < half) {
+                const float2 w = angles[4 * block.y + i];
+                const float x = b[2 * i], y = b[2 * i + 1];
+                b[2 * i] = x * w.x - y * w.y;
+                b[2 * i + 1] = y * w.x + x * w.y;
+            }
+        }
+    } else if (8 * j < half) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 w = angles[8 * j + i];
+            const float x = a[i], y = b[i];
+            a[i] = x * w.x - y * w.y;
+            b[i] = y * w.x + x * w.y;
+        }
+    }
+}
+
+template <class T> struct RotaryArgs {
+    const T *input;
+    T *output;
+    int input_stride, output_stride, lanes, tasks; // lanes per head, lanes per row
+    bool aligned;
+    const int *positions;
+    Turning turning;
+};
+
+template <class T, bool Interleaved> __global__ void __launch_bounds__(256) rotary_rows(const RotaryArgs<T> args) {
+    __shared__ float2 angles[kMaxPairs];
+    pdl_launch_dependents();
+    pdl_wait_upstream();
+    const int row = blockIdx.x;
+    const T *input = args.input + size_t(row) * args.input_stride;
+    T *output = args.output + size_t(row) * args.output_stride;
+    for (int task = threadIdx.x, first = 1; first || task < args.tasks; task += blockDim.x, first = 0) {
+        const int head = task / args.lanes, j = task - head * args.lanes;
+        const int2 block = blocks_of<Interleaved>(j, args.turning.half);
+        const int base = head * args.lanes * 16;
+        float a[8], b[8];
+        if (task < args.tasks) {
+            load8(input + base + 8 * block.x, 8, args.aligned, a);
+            load8(input + base + 8 * block.y, 8, args.aligned, b);
+        }
+        if (first) {
+            fill_angles(args.turning, load_index(args.positions + row), angles);
+            __syncthreads();
+        }
+        if (task >= args.tasks) break;
+        turn<Interleaved>(a, b, j, block, args.turning.half, angles);
+        store8(output + base + 8 * block.x, args.aligned, a);
+        store8(output + base + 8 * block.y, args.aligned, b);
+    }
+}
+
+template <class T> struct WriteArgs {
+    const T *queries, *keys, *values, *query_norm, *key_norm;
+    T *query_output;
+    int query_stride, key_stride, value_stride, output_stride;
+    bool aligned;
+    int query_heads, kv_heads, page_shift;
+    unsigned slots;
+    unsigned char *cached_keys, *cached_values;
+    float *key_scales, *value_scales;
+    const int *slot_of, *positions;
+    Turning turning;
+    float epsilon;
+};
+
+// Lanes of one warp hold whole heads (4 or 8 lanes each). Key, value and query heads are told apart by their number only.
+template <class T, Type F, int HeadDim, bool Interleaved> __global__ void __launch_bounds__(256) write_rows(const WriteArgs<T> args) {
+    constexpr int kLanes = HeadDim / 16;
+    __shared__ float2 angles[HeadDim / 2];
+    pdl_launch_dependents();
+    pdl_wait_upstream();
+    const int row = blockIdx.x, kv = args.kv_heads;
+    const int slot = load_index(args.slot_of + row);
+    const bool kept = unsigned(slot) < args.slots; // negative ones are past any cache, read as unsigned
+    const int tasks = (args.query_heads + 2 * kv) * kLanes, j = threadIdx.x % kLanes;
+    const int2 block = blocks_of<Interleaved>(j, args.turning.half);
+    for (int task = threadIdx.x, first = 1; first || task - int(threadIdx.x & 31u) < tasks; task += blockDim.x, first = 0) {
+        const bool live = task < tasks;
+        const int number = task / kLanes; // keys first, then values, then queries
+        const int head = number < 2 * kv ? (number < kv ? number : number - kv) : number - 2 * kv;
+        const bool is_query = number >= 2 * kv, is_value = !is_query && number >= kv;
+        const T *source = is_query ? args.queries + size_t(row) * args.query_stride
+                          : is_value ? args.values + size_t(row) * args.value_stride
+                                     : args.keys + size_t(row) * args.key_stride;
+        source += head * HeadDim;
+        float a[8] = {}, b[8] = {};
+        if (live) {
+            load8(source + 8 * block.x, 8, args.aligned, a);
+            load8(source + 8 * block.y, 8, args.aligned, b);
+        }
+        if (first) {
+            if (args.turning.half) fill_angles(args.turning, load_index(args.positions + row), angles);
+            __syncthreads();
+        }
+        const T *norm = is_value ? nullptr : is_query ? args.query_norm : args.key_norm;
+        float squares = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) squares += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+        if (norm && live) {
+            const float r = 1.f / sqrtf(squares * (1.f / HeadDim) + args.epsilon);
+            float w[8];
+            load8(norm + 8 * block.x, 8, args.aligned, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = a[i] * r * w[i];
+            load8(norm + 8 * block.y, 8, args.aligned, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) b[i] = b[i] * r * w[i];
+        }
+        if (!is_value) turn<Interleaved>(a, b, j, block, args.turning.half, angles);
+        // Magnitudes order like their bits, and infinities and NaN lie above every finite one.
+        unsigned most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            most = max(most, max(__float_as_uint(a[i]) & 0x7fffffffu, __float_as_uint(b[i]) & 0x7fffffffu));
+#pragma unroll
+        for (int d = 1; d < kLanes; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        if (!live) continue;
+        if (is_query) {
+            T *output = args.query_output + size_t(row) * args.output_stride + head * HeadDim;
+            store8(output + 8 * block.x, args.aligned, a);
+            store8(output + 8 * block.y, args.aligned, b);
+        } else if (kept) {
+            const bool finite = most < 0x7f800000u;
+            const float scale = finite ? quant_scale<F>(__uint_as_float(most)) : __int_as_float(0x7fffffff);
+            const float inverse = finite ? __fdiv_rn(1.f, scale) : 0.f;
+            const size_t at = ((size_t(slot >> args.page_shift) * kv + head) << args.page_shift) + (slot & ((1 << args.page_shift) - 1));
+            unsigned char *to = (is_value ? args.cached_values : args.cached_keys) + at * HeadDim;
+            if (!finite) { // the scale says NaN; the bytes stay numbers
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.f;
+            }
+            b200::store8<F>(to + 8 * block.x, 8, true, a, inverse);
+            b200::store8<F>(to + 8 * block.y, 8, true, b, inverse);
+            if (!j) (is_value ? args.value_scales : args.key_scales)[at] = scale;
+        }
+    }
+}
+
+template <class T> struct ReadArgs {
+    const unsigned char *cached_keys, *cached_values;
+    const float *key_scales, *value_scales;
+    T *keys, *values;
+    int key_stride, value_stride, rows, kv_heads, page_shift, per_row, rows_per_cta; // per_row: threads that share a row
+    bool aligned;
+    unsigned slots;
+    const int *slot_of;
+};
+
+template <Type F> __device__ __forceinline__ void decode16(uint4 raw, float scale, float (&a)[8], float (&b)[8]) {
+    const unsigned words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        float v[4];
+        if (F == Type::I8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = float(int(static_cast<signed char>(words[w] >> (8 * i))));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const __half2_raw pair = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(words[w] >> (16 * i)), __NV_E4M3);
+                const float2 f = __half22float2(__half2(pair));
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) (w < 2 ? a : b)[4 * (w & 1) + i] = v[i] * scale;
+    }
+}
+
+// A thread takes 16 columns of a head, of keys and values: both 16-byte loads are in flight together.
+template <class T, Type F, int HeadDim> __global__ void __launch_bounds__(256) read_rows(const ReadArgs<T> args) {
+    constexpr int kLanes = HeadDim / 16;
+    pdl_launch_dependents();
+    pdl_wait_upstream();
+    const int in_cta = int(threadIdx.x) / args.per_row, rest = int(threadIdx.x) - in_cta * args.per_row;
+    const long long row = (long long)blockIdx.x * args.rows_per_cta + in_cta;
+    if (in_cta >= args.rows_per_cta || row >= args.rows) return;
+    const int slot = load_index(args.slot_of + row);
+    const bool held = unsigned(slot) < args.slots;
+    for (int task = rest; task < args.kv_heads * kLanes; task += args.per_row) {
+        const int head = task / kLanes, j = task % kLanes;
+        const size_t at =
+            held ? ((size_t(slot >> args.page_shift) * args.kv_heads + head) << args.page_shift) + (slot & ((1 << args.page_shift) - 1)) : 0;
+        uint4 k{}, v{};
+        float ks = 0.f, vs = 0.f;
+        if (held && args.keys) {
+            k = load_upstream16(args.cached_keys + at * HeadDim + 16 * j);
+            ks = __int_as_float(load_index(reinterpret_cast<const int *>(args.key_scales + at)));
+        }
+        if (held && args.values) {
+            v = load_upstream16(args.cached_values + at * HeadDim + 16 * j);
+            vs = __int_as_float(load_index(reinterpret_cast<const int *>(args.value_scales + at)));
+        }
+        float a[8], b[8];
+        if (args.keys) {
+            decode16<F>(k, ks, a, b);
+            T *to = args.keys + size_t(row) * args.key_stride + head * HeadDim + 16 * j;
+            store8(to, args.aligned, a);
+            store8(to + 8, args.aligned, b);
+        }
+        if (args.values) {
+            decode16<F>(v, vs, a, b);
+            T *to = args.values + size_t(row) * args.value_stride + head * HeadDim + 16 * j;
+            store8(to, args.aligned, a);
+            store8(to + 8, args.aligned, b);
+        }
+    }
+}
+
+bool aligned16(const TensorView &v) {
+    return !v.data || (reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && (v.rows <= 1 || v.ld() % 8 == 0));
+}
+int shift_of(int power) {
+    int s = 0;
+    while ((1 << s) < power) ++s;
+    return s;
+}
+Turning turning_of(const RotaryView &r) { return {r.turns, r.turns ? r.dims / 2 : 0, r.scale}; }
+
+template <class T>
+void rotate(TensorView input, TensorView output, const int *positions, RotaryView rotary, int head_dim, cudaStream_t stream) {
+    RotaryArgs<T> args{input.ptr<T>(), output.ptr<T>(), input.ld(), output.ld(), head_dim / 16, input.cols / 16,
+                       aligned16(input) && aligned16(output), positions, turning_of(rotary)};
+    const int threads = std::min(256, (args.tasks + 31) / 32 * 32);
+    launch_pdl("rotary", rotary.interleaved ? rotary_rows<T, true> : rotary_rows<T, false>, dim3(unsigned(input.rows)), dim3(unsigned(threads)), 0,
+               stream, args);
+}
+template <class T, Type F, int HeadDim> void write(const WriteArgs<T> &args, bool interleaved, int rows, cudaStream_t stream) {
+    const int tasks = (args.query_heads + 2 * args.kv_heads) * (HeadDim / 16);
+    launch_pdl("cache write", interleaved ? write_rows<T, F, HeadDim, true> : write_rows<T, F, HeadDim, false>, dim3(unsigned(rows)),
+               dim3(unsigned(std::min(256, (tasks + 31) / 32 * 32))), 0, stream, args);
+}
+template <class T, Type F, int HeadDim> void read(const ReadArgs<T> &args, cudaStream_t stream) {
+    const unsigned ctas = unsigned((args.rows + args.rows_per_cta - 1) / args.rows_per_cta);
+    launch_pdl("cache read", read_rows<T, F, HeadDim>, dim3(ctas), dim3(256), 0, stream, args);
+}
+// Calls f(element, format, head width) with the run-time types as compile-time ones.
+template <class Call> void by_type(Type element, Type format, int head_dim, Call &&call) {
+    auto width = [&](auto t, auto f) {
+        if (head_dim == 64) call(t, f, std::integral_constant<int, 64>{});
+        else call(t, f, std::integral_constant<int, 128>{});
+    };
+    auto storage = [&](auto t) {
+        if (format == Type::I8) width(t, std::integral_constant<Type, Type::I8>{});
+        else width(t, std::integral_constant<Type, Type::FP8>{});
+    };
+    if (element == Type::F16) storage(__half{});
+    else storage(__nv_bfloat16{});
+}
+} // namespace
+
+void launch_rotary(TensorView input, TensorView output, const int *positions, RotaryView rotary, int head_dim, cudaStream_t stream) {
+    if (!input.rows || !input.cols) return;
+    if (input.type == Type::F16) rotate<__half>(input, output, positions, rotary, head_dim, stream);
+    else rotate<__nv_bfloat16>(input, output, positions, rotary, head_dim, stream);
+}
+
+void launch_cache_write(CacheView cache, TensorView keys, TensorView values, const int *slots, const int *positions, RotaryView rotary,
+                        TensorView queries, TensorView query_output, TensorView query_norm, TensorView key_norm, float epsilon,
+                        cudaStream_t stream) {
+    if (!keys.rows) return;
+    by_type(keys.type, cache.type, cache.head_dim, [&](auto element, auto format, auto width) {
+        using T = decltype(element);
+        WriteArgs<T> args{};
+        args.queries = queries.ptr<T>(), args.keys = keys.ptr<T>(), args.values = values.ptr<T>();
+        args.query_norm = query_norm.ptr<T>(), args.key_norm = key_norm.ptr<T>(), args.query_output = query_output.ptr<T>();
+        args.query_stride = queries.ld(), args.key_stride = keys.ld(), args.value_stride = values.ld();
+        args.output_stride = query_output.ld();
+        args.aligned = aligned16(queries) && aligned16(keys) && aligned16(values) && aligned16(query_norm) && aligned16(key_norm) &&
+                       aligned16(query_output);
+        args.query_heads = queries.data ? queries.cols / cache.head_dim : 0;
+        args.kv_heads = cache.kv_heads, args.page_shift = shift_of(cache.page_size), args.slots = unsigned(cache.slots());
+        args.cached_keys = static_cast<unsigned char *>(cache.keys), args.cached_values = static_cast<unsigned char *>(cache.values);
+        args.key_scales = cache.key_scales, args.value_scales = cache.value_scales;
+        args.slot_of = slots, args.positions = positions, args.turning = turning_of(rotary), args.epsilon = epsilon;
+        write<T, decltype(format)::value, decltype(width)::value>(args, rotary.interleaved, keys.rows, stream);
+    });
+}
+
+void launch_cache_read(CacheView cache, const int *slots, TensorView keys, TensorView values, cudaStream_t stream) {
+    const TensorView &any = keys.data ? keys : values;
+    if (!any.rows) return;
+    by_type(any.type, cache.type, cache.head_dim, [&](auto element, auto format, auto width) {
+        using T = decltype(element);
+        ReadArgs<T> args{};
+        args.cached_keys = static_cast<unsigned char *>(cache.keys), args.cached_values = static_cast<unsigned char *>(cache.values);
+        args.key_scales = cache.key_scales, args.value_scales = cache.value_scales;
+        args.keys = keys.ptr<T>(), args.values = values.ptr<T>(), args.key_stride = keys.ld(), args.value_stride = values.ld();
+        args.rows = any.rows, args.kv_heads = cache.kv_heads, args.page_shift = shift_of(cache.page_size);
+        args.per_row = std::min(256, cache.kv_heads * cache.head_dim / 16), args.rows_per_cta = 256 / args.per_row;
+        args.aligned = aligned16(keys) && aligned16(values), args.slots = unsigned(cache.slots()), args.slot_of = slots;
+        read<T, decltype(format)::value, decltype(width)::value>(args, stream);
+    });
+}
+} // namespace tts

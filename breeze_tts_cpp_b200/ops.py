@@ -16,7 +16,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import BF16, F16, F32, FP8, I8, I32, Epilogue, NormFusion, Path_, RowScaled, Tensor
+from ._lib import (BF16, F16, F32, FP8, I8, I32, Attention, Cache, Epilogue, NormFusion, Path_, RotaryPlan, RowScaled,
+                   Tensor)
 
 try:
     from . import _native
@@ -77,6 +78,70 @@ class RowScaledView:
             raise ValueError("row slices of K-group scales are not contiguous")
         return RowScaledView(self.values[first:first + count], self.scales[first:first + count], self.format, 0,
                              self.rotation_size)
+
+
+@dataclass
+class CacheView:
+    """Quantized key/value cache: one byte per value [pages, kv_heads, page_size, head_dim], one fp32 scale per token and head
+    [pages, kv_heads, page_size]. Slot s is token s % page_size of page s // page_size."""
+    keys: torch.Tensor          # uint8 (or int8 / float8_e4m3fn) storage
+    values: torch.Tensor
+    key_scales: torch.Tensor    # float32
+    value_scales: torch.Tensor
+    format: int                 # I8 or FP8
+
+    @staticmethod
+    def empty(pages: int, kv_heads: int, page_size: int, head_dim: int, fmt: int, device="cuda") -> "CacheView":
+        """Slots hold anything until they are written; no operator reads one that its arguments do not name."""
+        shape = (pages, kv_heads, page_size)
+        values = (torch.empty(*shape, head_dim, dtype=torch.uint8, device=device) for _ in range(2))
+        scales = (torch.empty(shape, dtype=torch.float32, device=device) for _ in range(2))
+        return CacheView(*values, *scales, fmt)
+
+    def c(self) -> Cache:
+        shape, device = self.keys.shape, self.keys.device
+        parts = (self.keys, self.values, self.key_scales, self.value_scales)
+        if (len(shape) != 4 or self.values.shape != shape or any(t.shape != shape[:3] for t in parts[2:])
+                or any(t.dtype != torch.float32 for t in parts[2:]) or any(t.element_size() != 1 for t in parts[:2])
+                or any(not t.is_cuda or t.device != device or not t.is_contiguous() for t in parts)):
+            raise ValueError("a cache is two contiguous one-byte tensors [pages, kv_heads, page_size, head_dim] and two float32 "
+                             "tensors [pages, kv_heads, page_size] on one CUDA device")
+        return Cache(*(t.data_ptr() for t in parts), *shape, self.format, device.index)
+
+
+@dataclass
+class Rotary:
+    """Rotary positions: pair i of a head turns by turns[i] revolutions per position. The first 2 * len(turns) columns of a head take part,
+    as pairs (i, i + len(turns)), or (2i, 2i + 1) when interleaved; cosine and sine are multiplied by `scale`."""
+    turns: torch.Tensor  # float64 on the device
+    interleaved: bool = False
+    scale: float = 1.0
+
+    SCALINGS = ("none", "linear", "base", "yarn", "wavelength")
+
+    @staticmethod
+    def plan(dims: int, base: float = 10000.0, interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+             original_length: int = 0, low: float = 1.0, high: float = 0.0, device="cuda") -> "Rotary":
+        """The usual turns base ** (-2 i / dims) / 2 pi, stretched by `factor` for longer contexts: "linear" all of them, "base" by a larger
+        base, "yarn" and "wavelength" those that make few turns within original_length (a ramp between `low` and `high` turns)."""
+        if scaling not in Rotary.SCALINGS:
+            raise ValueError(f"scaling must be one of {Rotary.SCALINGS}")
+        host, scale = torch.empty(max(dims // 2, 0), dtype=torch.float64), C.c_float(1.0)
+        _lib.call("b200q_rotary_turns", dims, base, Rotary.SCALINGS.index(scaling), factor, original_length, low, high,
+                  C.cast(host.data_ptr(), C.POINTER(C.c_double)), C.byref(scale))
+        return Rotary(host.to(device), interleaved, scale.value)
+
+    def c(self) -> RotaryPlan:
+        if self.turns.dtype != torch.float64 or self.turns.dim() != 1 or not self.turns.is_cuda or not self.turns.is_contiguous():
+            raise ValueError("rotary turns must be a contiguous float64 vector on a CUDA device")
+        return RotaryPlan(self.turns.data_ptr(), 2 * self.turns.numel(), int(self.interleaved), self.scale, self.turns.device.index)
+
+
+def attention_workspace(rows: int, heads: int, kv_heads: int, head_dim: int, prefix: bool = False, multiprocessors: int = 148) -> int:
+    """Bytes of context workspace that Context.cached_attention needs."""
+    needed = C.c_size_t()
+    _lib.call("b200q_attention_workspace", rows, heads, kv_heads, head_dim, int(prefix), multiprocessors, C.byref(needed))
+    return needed.value
 
 
 def _epilogue(bias=None, residual=None, residual_f32=None, activation=0, value_scale=1.0, output_scale=1.0,
@@ -224,6 +289,40 @@ class Context:
                   C.byref(_tensor(norm_bias)), epsilon, C.byref(_fusion(**(fusion or {}))), C.byref(_epilogue(**epilogue)),
                   qo, C.byref(taken))
         return bool(taken.value)
+
+    # ---- between the QKV and the O projection
+    def rotary(self, x: torch.Tensor, positions: torch.Tensor, rotary: Rotary, head_dim: int, out: torch.Tensor | None = None) -> torch.Tensor:
+        """Turns every head of x [rows, heads * head_dim] by positions [rows] (int32). out may be x."""
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _lib.call("b200q_rotary", self._handle, C.byref(_tensor(x)), C.byref(_tensor(positions)), C.byref(rotary.c()), head_dim,
+                  C.byref(_tensor(out)))
+        return out
+
+    def cache_write(self, cache: CacheView, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor | None = None,
+                    rotary: Rotary | None = None, q: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                    q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, epsilon: float = 1e-6) -> None:
+        """Quantizes row r of k and v [rows, kv_heads * head_dim] into slot slots[r] (int32, each at most once; negative or past the
+        cache: left out). k, and q into q_out (may be q), are normalised over each head and turned first, where the arguments say so."""
+        _lib.call("b200q_cache_write", self._handle, C.byref(cache.c()), C.byref(_tensor(k)), C.byref(_tensor(v)), C.byref(_tensor(slots)),
+                  C.byref(_tensor(positions)), C.byref(rotary.c()) if rotary is not None else None, C.byref(_tensor(q)),
+                  C.byref(_tensor(q_out)), C.byref(_tensor(q_norm)), C.byref(_tensor(k_norm)), epsilon)
+
+    def cache_read(self, cache: CacheView, slots: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None) -> None:
+        """Row r of k and v (either may be None) = what slot slots[r] holds; zeros for a slot outside of the cache."""
+        _lib.call("b200q_cache_read", self._handle, C.byref(cache.c()), C.byref(_tensor(slots)), C.byref(_tensor(k)), C.byref(_tensor(v)))
+
+    def cached_attention(self, q: torch.Tensor, cache: CacheView, pages: torch.Tensor, lengths: torch.Tensor, out: torch.Tensor,
+                         scale: float = 0.0, query_offsets: torch.Tensor | None = None, prefix_pages: torch.Tensor | None = None,
+                         prefix_length: torch.Tensor | None = None) -> torch.Tensor:
+        """Causal attention of q [rows, heads * head_dim] over the cache. pages [sequences, n] and lengths [sequences] (int32) name each
+        sequence's cached tokens, the query rows' own among them; query_offsets [sequences + 1] its rows (without it, one each). All
+        rows also see the prefix_length [1] tokens on prefix_pages [m], which are read once for the batch. Rows that see nothing are
+        zero, rows behind the last offset are left alone. scale 0: 1 / sqrt(head_dim)."""
+        arguments = Attention(_tensor(q), _tensor(out), _tensor(pages), _tensor(lengths), _tensor(query_offsets), _tensor(prefix_pages),
+                              _tensor(prefix_length), scale)
+        _lib.call("b200q_cached_attention", self._handle, C.byref(cache.c()), C.byref(arguments))
+        return out
 
     def status(self) -> int:
         value = C.c_int32(0)

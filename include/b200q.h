@@ -167,6 +167,72 @@ int b200q_normalized_linear(b200q_context *, const b200q_tensor *input, const b2
                             const b200q_norm_fusion *fusion, const b200q_epilogue *epilogue,
                             const b200q_row_scaled *quantized_output, int32_t *taken, char *error, size_t error_capacity);
 
+/* ---- Between the QKV and the O projection ---------------------------------------------------------
+ * No counterparts among the reference's quantized operators: its attention and its cache are 16-bit. Index tensors are int32 on the
+ * device, [1, n] unless said otherwise; their contents cannot be checked by the host, so what an index out of range does is said with each
+ * operator, and none reads or writes outside of what the caller passed. Strided 16-bit rows (slices of a packed QKV buffer) are taken
+ * as they are; 16-byte aligned ones are faster. Every call can be captured. */
+
+/* A quantized key/value cache: one byte per value, [pages, kv_heads, page_size, head_dim], type B200Q_I8 or B200Q_FP8 (e4m3), and one
+ * fp32 scale per token and head, [pages, kv_heads, page_size]; all four dense and 16-byte aligned. page_size is a power of two from 16 to 1024,
+ * head_dim 64 or 128. A slot is page * page_size + the token's place in its page. A scale that is NaN marks a row as not a number. */
+typedef struct b200q_cache {
+    void *keys, *values;
+    float *key_scales, *value_scales;
+    int32_t pages, kv_heads, page_size, head_dim, type, device;
+} b200q_cache;
+/* Rotary positions: pair i of a head turns by turns[i] revolutions per position (device fp64 [dims / 2]: far positions need them), and
+ * cosine and sine are multiplied by `scale`. dims is a multiple of 16 of at most the head; the pairs are (i, i + dims / 2), or
+ * (2i, 2i + 1) when interleaved; columns behind dims pass through. */
+typedef struct b200q_rotary_plan {
+    const double *turns;
+    int32_t dims, interleaved;
+    float scale;
+    int32_t device;
+} b200q_rotary_plan;
+
+/* Host only. Fills turns (host, [dims / 2]) and *scale for a base and a way to stretch it by `factor` >= 1: scaling 0 none, 1 linear
+ * (all positions divided by the factor), 2 a larger base, 3 a ramp over the pairs between those that make `high` (0: 32) and `low` (usually 1) turns
+ * within original_length, with the matching scale (yarn), 4 a ramp over the turns themselves between `low` and `high` (0: 4). */
+int b200q_rotary_turns(int32_t dims, double base, int32_t scaling, double factor, int32_t original_length, double low, double high,
+                       double *turns, float *scale, char *error, size_t error_capacity);
+/* output[r] = input[r] ([rows, heads * head_dim], BF16 or F16; head_dim a multiple of 16 up to 512) turned by positions[r] (any int32). Both
+ * may be the same view. Products and sums in fp32, angles reduced in fp64. */
+int b200q_rotary(b200q_context *, const b200q_tensor *input, const b200q_tensor *positions, const b200q_rotary_plan *plan, int32_t head_dim,
+                 const b200q_tensor *output, char *error, size_t error_capacity);
+/* Quantizes row r of keys and values ([rows, kv_heads * head_dim]) into slot slots[r], each head's 64 or 128 values by the rule of
+ * b200q_row_quantize with one scale; a head that holds an infinity or NaN gets a NaN scale. Keys are first normalised over the head (RMSNorm,
+ * key_norm 16-bit [1, head_dim], or NULL) and turned (plan and positions, or NULL both), in fp32 up to the bytes. queries and query_output (NULL
+ * both, or the same view) get the same treatment with query_norm and are written as 16-bit rows, so one launch takes a QKV row apart. A row whose
+ * slot is negative or past the cache is not written (its queries are). Slots must differ from one another: where two rows name the same slot,
+ * what that slot holds afterwards is unspecified. */
+int b200q_cache_write(b200q_context *, const b200q_cache *cache, const b200q_tensor *keys, const b200q_tensor *values,
+                      const b200q_tensor *slots, const b200q_tensor *positions, const b200q_rotary_plan *plan, const b200q_tensor *queries,
+                      const b200q_tensor *query_output, const b200q_tensor *query_norm, const b200q_tensor *key_norm, float epsilon, char *error,
+                      size_t error_capacity);
+/* keys[r], values[r] ([rows, kv_heads * head_dim], BF16 or F16; either may be NULL) = what slot slots[r] holds, times its scale;
+ * zeros for a slot outside of the cache. The same slot may be read by several rows. */
+int b200q_cache_read(b200q_context *, const b200q_cache *cache, const b200q_tensor *slots, const b200q_tensor *keys, const b200q_tensor *values,
+                     char *error, size_t error_capacity);
+
+/* Attention over the cache. queries and output are [rows, heads * head_dim], BF16 or F16; heads is a multiple of the cache's kv_heads,
+ * query head h reads cached head h / (heads / kv_heads). pages [sequences, columns] (rows may be strided) gives each sequence's pages, lengths its cached
+ * tokens, those of its query rows included (clamped to 0 .. columns * page_size). query_offsets ([1, sequences + 1], rising from 0) says which rows are a
+ * sequence's; without it there is one row per sequence. Row i of n sees positions 0 .. length - n + i; a row that sees nothing is zero; rows behind the
+ * last offset are left as they are. With prefix_pages ([1, columns]) and prefix_length ([1, 1]), all rows also see all of that prefix, which is read once for
+ * the whole batch; positions in lengths and pages then count from behind it. scale 0 means 1 / sqrt(head_dim). A position on a page that the cache does
+ * not have reads as NaN. The maximum, the sums and the output are kept in fp32; weights are rounded to fp16 for the second product.
+ * Uses the context's workspace behind its header (b200q_attention_workspace bytes in all), so graphs captured from one context must not run
+ * at the same time, like all work of a context. */
+typedef struct b200q_attention {
+    b200q_tensor queries, output, pages, lengths, query_offsets, prefix_pages, prefix_length;
+    float scale;
+} b200q_attention;
+int b200q_cached_attention(b200q_context *, const b200q_cache *cache, const b200q_attention *arguments, char *error, size_t error_capacity);
+/* Host only: bytes of context workspace that b200q_cached_attention needs. */
+int b200q_attention_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t prefix, int32_t multiprocessors,
+                              size_t *needed, char *error, size_t error_capacity);
+
 /* ---- Linear layer object --------------------------------------------------------------------
  * reference: tts::Linear (src/layers/linear.h:11-76) over a quantized weight, with the load-time
  * step of Weights::quantized (src/io/weights.cpp:80-87,133-154): `parts` are `part_count` 16-bit
