@@ -44,14 +44,20 @@ struct Carve {
 };
 
 template <class T, Type F, int HeadDim, int Tiles>
-void launch_pass(const AttentionArgs &args, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
+void launch_pass(AttentionArgs args, int most_columns, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
+    using Shape = AttentionShape<HeadDim, Tiles>;
+    // What the workers leave for the mergers, twice where that is small, and as many stages as the rest of the shared memory holds.
+    args.merge_columns = std::min(Shape::columns, most_columns);
+    args.merge_buffers = args.merge_columns <= 8 ? 2 : 1;
+    const size_t merge = size_t(args.merge_buffers) * Shape::merge(args.merge_columns);
+    args.stages = int(std::min<size_t>(kMaxRing, (kAttentionSmem - 1024 - merge) / Shape::stage));
     launch_pdl("cached attention", cached_attention<T, F, HeadDim, Tiles>, dim3(unsigned(ctas)), dim3(kAttentionThreads),
-               AttentionShape<HeadDim, Tiles>::smem, stream, keys, values, args);
+               1024 + args.stages * size_t(Shape::stage) + merge, stream, keys, values, args);
 }
 template <class T, Type F, int HeadDim>
-void launch_pass(bool narrow, const AttentionArgs &args, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
-    if (narrow) launch_pass<T, F, HeadDim, 1>(args, keys, values, ctas, stream);
-    else launch_pass<T, F, HeadDim, 2>(args, keys, values, ctas, stream);
+void launch_pass(bool narrow, int most_columns, const AttentionArgs &args, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
+    if (narrow) launch_pass<T, F, HeadDim, 1>(args, most_columns, keys, values, ctas, stream);
+    else launch_pass<T, F, HeadDim, 2>(args, most_columns, keys, values, ctas, stream);
 }
 // Calls f(element, format, head width) with the run-time types as compile-time ones.
 template <class Call> void by_type(Type element, Type format, int head_dim, Call &&call) {
@@ -70,9 +76,8 @@ bool aligned16(const TensorView &v) {
     return reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && (v.rows <= 1 || v.ld() % 8 == 0);
 }
 template <class T, Type F, int HeadDim> void raise_limit() {
-    for (auto [kernel, bytes] : {std::pair{cached_attention<T, F, HeadDim, 1>, AttentionShape<HeadDim, 1>::smem},
-                                 std::pair{cached_attention<T, F, HeadDim, 2>, AttentionShape<HeadDim, 2>::smem}}) {
-        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    for (auto *kernel : {cached_attention<T, F, HeadDim, 1>, cached_attention<T, F, HeadDim, 2>}) {
+        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kAttentionSmem));
         if (status != cudaSuccess) throw std::runtime_error(std::string("cudaFuncSetAttribute(attention): ") + cudaGetErrorString(status));
     }
 }
@@ -132,7 +137,9 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
                 args.page_columns = args.page_stride = p.prefix_columns;
                 narrow = (long long)rows * args.group <= 8;
             }
-            launch_pass<T, decltype(format)::value, decltype(width)::value>(narrow, args, keys, values, ctas, stream);
+            // Query rows of one segment at most: where each sequence has one row, those of a cached head.
+            const int most = !pass && !p.query_offsets ? args.group : INT_MAX;
+            launch_pass<T, decltype(format)::value, decltype(width)::value>(narrow, most, args, keys, values, ctas, stream);
             combine.source[pass] = {args.partials, args.complete, args.table, ctas, narrow ? 8 : 16};
         }
         const long long warps = (long long)rows * heads;

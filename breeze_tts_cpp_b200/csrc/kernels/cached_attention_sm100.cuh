@@ -13,11 +13,15 @@
 // transposed weights take one 8 x 8 transposition in registers to become the second product's operand; its rows are head_dim and a
 // thread owns 16 consecutive columns of the output.
 //
-// Bound. A cached byte takes part in 2 x query rows multiply-adds and costs about 1.3 instructions of conversion; at two to eight rows per head memory is
-// the floor. One CTA per multiprocessor streams 128-token tiles (box copies by the tensor map, 128-byte swizzle, so that no shared load has
-// a bank conflict) through a ring; eight warps take 16 keys of a tile each and keep their own softmax state and output, which meet once per
-// segment. Work is divided evenly over the CTAs in tiles, whatever the lengths are: a CTA's share is a run of consecutive tiles, a segment (sequence, cached
-// head, query tile) that runs over a share's end leaves partial sums that a second launch adds in a fixed order.
+// Bound. A cached byte takes part in 2 x query rows multiply-adds and costs about 1.4 instructions of conversion; at two to eight rows per
+// head memory is the floor. One CTA per multiprocessor streams 128-token tiles (box copies by the tensor map, 128-byte swizzle, so that no
+// shared load has a bank conflict; the segment's query rows come with its first tiles) through a ring. Two groups of four warps take alternate
+// tiles, 32 keys a warp, so that a warp has two independent chains and its scheduler another warp; each warp keeps its own softmax state and output.
+// At a segment's end the warps leave theirs in shared memory and go on; two further warps add them up and store.
+//
+// Division. A segment is a sequence, a cached head and a tile of query rows. All CTAs get an equal run of the same list of tiles, whatever
+// the lengths are, a segment's fixed cost counted as a part of a tile; a segment that runs over a share's end leaves partial sums, which a second launch adds in
+// a fixed order.
 #pragma once
 #include "kernels/launch.cuh"
 #include "kernels/sm100_ptx.cuh"
@@ -26,7 +30,9 @@
 #include <cuda_fp16.h>
 
 namespace tts::b200 {
-constexpr int kTileKeys = 128, kAttentionWarps = 8, kAttentionThreads = 32 * (kAttentionWarps + 1);
+constexpr int kTileKeys = 128, kWorkers = 8, kMergers = 2; // workers: two groups of four warps
+constexpr int kProducer = kWorkers, kAttentionThreads = 32 * (kWorkers + 1 + kMergers);
+constexpr int kMaxRing = 12;
 constexpr int kPartialExtra = 4; // maximum and sum behind a partial row, padded to 16 bytes
 constexpr size_t kAttentionSmem = 224 * 1024;
 
@@ -43,6 +49,7 @@ struct AttentionArgs {
     const float *key_scales, *value_scales;
     float score_scale; // softmax scale, log2 e and the key format's factor
     float output_scale;
+    int stages, merge_columns, merge_buffers;
     float *partials; // [ctas][2][columns][head_dim + kPartialExtra]
     int4 *table;     // [rows * heads]: first CTA, parts, slot of the first part, column; parts == 0: complete
     float *complete; // [rows * heads][head_dim + kPartialExtra], or null: complete segments go to the output
@@ -104,18 +111,16 @@ template <int HeadDim, int Tiles> struct AttentionShape {
     static constexpr int columns = 8 * Tiles; // query rows of a segment
     static constexpr int row = HeadDim + kPartialExtra;
     static constexpr uint32_t values = kTileKeys * HeadDim, scales = 2 * kTileKeys * HeadDim; // offsets in a stage
-    static constexpr uint32_t stage = scales + 2 * kTileKeys * 4;
-    static constexpr uint32_t merge = kAttentionWarps * columns * row * 4;
-    static constexpr uint32_t stage_aligned = (stage + 1023) / 1024 * 1024;
-    static constexpr int stages = int((kAttentionSmem - 2048 - merge) / stage_aligned) > 12 ? 12 : int((kAttentionSmem - 2048 - merge) / stage_aligned);
-    static constexpr size_t smem = 1024 + size_t(stages) * stage_aligned + merge;
+    static constexpr uint32_t queries = scales + 2 * kTileKeys * 4, query_row = HeadDim * 2 + 16; // the pad spreads rows over banks
+    static constexpr uint32_t stage = (queries + columns * query_row + 1023) / 1024 * 1024;
+    static __host__ __device__ constexpr uint32_t merge(int merge_columns) { return kWorkers * merge_columns * row * 4; }
 };
 
-// What the producer tells the consumers about a tile.
+// What the producer tells the workers about a tile, and they the mergers about a segment's part.
 struct TileNote {
-    int key, head, row, count, flat, limit, flags, first_cta, first_slot, slot, pad[6];
+    int key, head, row, count, flat, limit, flags, ordinal, first_cta, first_slot, slot, pad[5];
 };
-constexpr int kNoteFirst = 1, kNoteLast = 2, kNoteSplit = 4;
+constexpr int kNoteFirst = 1, kNoteFlush = 2, kNoteEnd = 4, kNoteAlone = 8, kNoteFinal = 16, kNoteSplit = 32, kNoteQuit = 64;
 
 // A sequence as the tables give it, made safe: rows and positions stay inside of what the caller passed.
 struct SequenceShape {
@@ -147,13 +152,32 @@ template <int Columns> __device__ __forceinline__ int tiles_of(const AttentionAr
 template <int Columns> __device__ __forceinline__ int query_tiles(const AttentionArgs &a, const SequenceShape &s) {
     return (s.count * a.group + Columns - 1) / Columns;
 }
-template <int Columns> __device__ __forceinline__ long long work_of(const AttentionArgs &a, const SequenceShape &s) {
-    const int tiles = query_tiles<Columns>(a, s);
-    if (a.prefix) return (long long)tiles * a.kv_heads * tiles_of<Columns>(a, s, 0);
-    long long sum = 0;
-    for (int qt = 0; qt < tiles; ++qt) sum += tiles_of<Columns>(a, s, qt);
-    return sum * a.kv_heads;
+// Tiles and segments of a sequence.
+struct Work {
+    long long tiles, segments;
+};
+template <int Columns> __device__ __forceinline__ Work work_of(const AttentionArgs &a, const SequenceShape &s) {
+    const int count = query_tiles<Columns>(a, s);
+    Work w{0, (long long)count * a.kv_heads};
+    if (a.prefix) {
+        w.tiles = w.segments * tiles_of<Columns>(a, s, 0);
+    } else {
+        for (int qt = 0; qt < count; ++qt) w.tiles += tiles_of<Columns>(a, s, qt);
+        w.tiles *= a.kv_heads;
+    }
+    return w;
 }
+__device__ __forceinline__ long long scan_warp(long long v, int lane) { // inclusive
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += other;
+    }
+    return v;
+}
+// Shares are counted in units: kTileUnits for a tile, kSegmentUnits more for a segment (its queries, its flush and its merge). A tile belongs to the
+// CTA whose share holds its first unit.
+constexpr int kTileUnits = 4, kSegmentUnits = 2;
 
 // One query row's result: the output row, or what is kept of it for the second launch.
 template <class T, int HeadDim>
@@ -175,26 +199,28 @@ template <class T, Type F, int HeadDim, int Tiles>
 __global__ void __launch_bounds__(kAttentionThreads, 1)
     cached_attention(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const AttentionArgs args) {
     using Shape = AttentionShape<HeadDim, Tiles>;
-    constexpr int kColumns = Shape::columns, kStages = Shape::stages, kSteps = HeadDim / 16, kThreads = kAttentionThreads;
+    constexpr int kColumns = Shape::columns, kSteps = HeadDim / 16, kWarps = kAttentionThreads / 32;
     extern __shared__ uint8_t raw_smem[];
-    __shared__ uint64_t full[kStages], empty[kStages], meet[2];
-    __shared__ TileNote notes[kStages];
-    __shared__ long long sums[kAttentionWarps + 1];
-    __shared__ long long found[2]; // sequence of this CTA's first tile, tiles of it that others take
+    __shared__ uint64_t full[2][kMaxRing], empty[kMaxRing], merge_full[2]; // full: of each group
+    __shared__ TileNote notes[kMaxRing], merge_notes[2];
+    __shared__ long long tile_sums[kWarps], segment_sums[kWarps];
+    __shared__ long long found[2]; // sequence of this CTA's first unit, its own first unit
     __shared__ int abort_flag;
+    __shared__ int merged; // parts that the mergers are done with, times kMergers
     const uint32_t ring = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;
-    float *merge = reinterpret_cast<float *>(raw_smem + (ring - ptx::smem_u32(raw_smem)) + kStages * Shape::stage_aligned);
+    uint8_t *const ring_bytes = raw_smem + (ring - ptx::smem_u32(raw_smem));
+    const int stages = args.stages, merge_floats = int(Shape::merge(args.merge_columns) / 4);
+    float *const merge = reinterpret_cast<float *>(ring_bytes + stages * Shape::stage);
     const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
 
     if (!threadIdx.x) {
-        for (int s = 0; s < kStages; ++s) {
-            ptx::mbar_init(ptx::smem_u32(&full[s]), 1);
-            ptx::mbar_init(ptx::smem_u32(&empty[s]), kAttentionWarps);
+        for (int s = 0; s < kMaxRing; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&full[0][s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&full[1][s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&empty[s]), kWorkers / 2);
         }
-        ptx::mbar_init(ptx::smem_u32(&meet[0]), kAttentionWarps);
-        ptx::mbar_init(ptx::smem_u32(&meet[1]), kAttentionWarps);
-        abort_flag = 0;
-        found[0] = found[1] = 0;
+        for (int b = 0; b < 2; ++b) ptx::mbar_init(ptx::smem_u32(&merge_full[b]), kWorkers);
+        abort_flag = merged = 0;
         ptx::fence_barrier_init();
         ptx::prefetch_tensormap(&key_map);
         ptx::prefetch_tensormap(&value_map);
@@ -203,42 +229,40 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     pdl_wait_upstream();
 
     // Every CTA adds up all sequences' tiles: a thread takes a run of sequences, then a scan over the threads.
-    const int run = (args.sequences + kThreads - 1) / kThreads;
+    const int run = (args.sequences + kAttentionThreads - 1) / kAttentionThreads;
     const int from = min(args.sequences, int(threadIdx.x) * run), to = min(args.sequences, from + run);
-    long long own = 0;
-    for (int b = from; b < to; ++b) own += work_of<kColumns>(args, sequence_of(args, b));
-    long long before = own;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= d) before += other;
+    Work own{0, 0};
+    for (int b = from; b < to; ++b) {
+        const Work w = work_of<kColumns>(args, sequence_of(args, b));
+        own.tiles += w.tiles, own.segments += w.segments;
     }
-    if (lane == 31) sums[warp] = before;
+    Work before{scan_warp(own.tiles, lane), scan_warp(own.segments, lane)};
+    if (lane == 31) tile_sums[warp] = before.tiles, segment_sums[warp] = before.segments;
     __syncthreads();
-    long long total = 0;
-    for (int w = 0; w <= kAttentionWarps; ++w) {
-        if (w < warp) before += sums[w];
-        total += sums[w];
+    Work all{0, 0};
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before.tiles += tile_sums[w], before.segments += segment_sums[w];
+        all.tiles += tile_sums[w], all.segments += segment_sums[w];
     }
-    before -= own;
-    // At least a tile for every CTA that takes part.
-    const long long ctas = total < gridDim.x ? total : gridDim.x;
+    // Where there is a CTA for every tile, each gets one. A share is never smaller than a tile, so that every CTA between a segment's first
+    // and its last has a part of it.
+    const long long ctas = all.tiles < gridDim.x ? all.tiles : gridDim.x;
     if (blockIdx.x >= ctas) return;
-    const long long begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-    if (before <= begin && begin < before + own) {
-        long long at = before;
+    const int extra = all.tiles > gridDim.x ? kSegmentUnits : 0;
+    auto units = [&](const Work &w) { return kTileUnits * w.tiles + extra * w.segments; };
+    const long long total = units(all), begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
+    before.tiles -= own.tiles, before.segments -= own.segments;
+    if (long long at = units(before); at <= begin && begin < at + units(own)) {
         for (int b = from; b < to; ++b) {
-            const long long work = work_of<kColumns>(args, sequence_of(args, b));
-            if (begin < at + work) {
-                found[0] = b;
-                found[1] = begin - at;
+            const long long part = units(work_of<kColumns>(args, sequence_of(args, b)));
+            if (begin < at + part) {
+                found[0] = b, found[1] = at;
                 break;
             }
-            at += work;
+            at += part;
         }
     }
     __syncthreads();
-    const int count = int(end - begin);
     // Every wait is bounded, and a warp whose wait gave up leaves as one; the others follow when theirs do.
     auto wait = [&](uint64_t &bar, uint32_t parity) {
         if (__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar), parity, &abort_flag))) return true;
@@ -246,292 +270,147 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         return false;
     };
 
-    if (warp == kAttentionWarps) { // ------------------------------------------------------------ producer
-        int b = int(found[0]), skip = int(found[1]), h = 0, qt = 0, tile = 0;
-        SequenceShape s = sequence_of(args, b);
-        int qts = query_tiles<kColumns>(args, s), tiles = tiles_of<kColumns>(args, s, 0);
-        auto next_segment = [&] { // heads outermost: their query tiles read the same keys, near one another in time
-            if (++qt == qts) {
-                qt = 0;
-                if (++h == args.kv_heads) {
-                    h = 0;
-                    do {
-                        if (++b >= args.sequences) return;
-                        s = sequence_of(args, b);
-                        qts = query_tiles<kColumns>(args, s);
-                    } while (!qts);
-                }
-            }
-            tiles = tiles_of<kColumns>(args, s, qt);
-        };
-        while (skip >= tiles) {
-            skip -= tiles;
-            next_segment();
-        }
-        tile = skip;
+    auto wait_merged = [&](int parts) {
+        bool reached = false;
+        const long long start = clock64();
+        while (!(reached = *const_cast<volatile int *>(&merged) >= parts) && !*const_cast<volatile int *>(&abort_flag))
+            if (clock64() - start > ptx::kWaitLimitCycles) abort_flag = 1;
+        reached = __all_sync(0xffffffffu, reached);
+        __threadfence_block();
+        if (!reached && !lane) *args.status = 1;
+        return reached;
+    };
+
+    // Tile i of the share goes to group i % 2 and stage i % stages. A stage may serve both groups in turn, so each group has its own barriers: waiting
+    // on a common one, a group could be two phases off. A group comes back to a stage after `period` of its tiles.
+    const int period = stages & 1 ? stages : stages / 2;
+
+    if (warp == kProducer) { // ------------------------------------------------------------------ producer
+        int stage = 0, issued = 0, ordinal = 0, b = int(found[0]);
+        uint32_t phase = 0;
+        long long at = found[1]; // first unit of the segment
         const int box = 1 << args.box_shift, boxes = kTileKeys >> args.box_shift;
         const uint32_t box_bytes = uint32_t(box) * (2 * HeadDim + 8);
-        int stage = 0, issued = 0;
-        uint32_t phase = 0;
-        for (; issued < count; ++issued) {
-            if (issued >= kStages && !wait(empty[stage], phase ^ 1)) break;
-            const int key = tile * kTileKeys, mine = lane >> 2, kind = lane & 3;
-            const uint32_t at = ring + stage * Shape::stage_aligned, bar = ptx::smem_u32(&full[stage]);
-            // Lane 4i + k copies part k (keys, values, their scales) of box i.
-            const int position = key + (mine << args.box_shift);
-            const bool wanted = mine < boxes && position < s.length;
-            int page = -1;
-            if (wanted) page = load_index(args.pages + size_t(b) * args.page_stride + (position >> args.page_shift));
-            const bool good = wanted && unsigned(page) < unsigned(args.total_pages);
-            // Positions on a page that the cache does not have read as NaN.
-            if (wanted && !good && kind >= 2) {
-                float *scales = reinterpret_cast<float *>(raw_smem + (at - ptx::smem_u32(raw_smem)) + Shape::scales) + (kind - 2) * kTileKeys;
-                for (int i = 0; i < box; ++i) scales[(mine << args.box_shift) + i] = __int_as_float(0x7fffffff);
-            }
-            __syncwarp();
-            const uint32_t copied = __popc(__ballot_sync(0xffffffffu, good)) / 4;
-            if (!lane) {
-                const long long at_tile = begin + issued, segment = at_tile - tile; // the segment's first tile
-                TileNote &n = notes[stage];
-                n.key = key, n.head = h, n.row = s.row, n.count = s.count, n.flat = qt * kColumns;
-                n.limit = args.prefix ? s.length - 1 : s.length - s.count;
-                const bool last = tile + 1 == tiles, starts_here = segment >= begin;
-                const bool split = !starts_here || segment + tiles > end;
-                n.flags = (tile == 0 || !issued ? kNoteFirst : 0) | (last || issued + 1 == count ? kNoteLast : 0) | (split ? kNoteSplit : 0);
-                n.slot = segment > begin ? 1 : 0;
-                n.first_cta = -1;
-                if (last && split) { // this CTA closes the segment: it says where its parts lie
-                    int cta = int(segment * ctas / total);
-                    while (total * (cta + 1) / ctas <= segment) ++cta;
-                    n.first_cta = cta;
-                    n.first_slot = total * cta / ctas < segment ? 1 : 0;
+        const int mine = lane >> 2, kind = lane & 3; // lane 4i + k copies part k (keys, values, their scales) of box i
+        bool open = true;
+        for (; open && b < args.sequences && at < end; ++b) {
+            const SequenceShape s = sequence_of(args, b);
+            const int query_count = query_tiles<kColumns>(args, s);
+            const int *pages = args.pages + size_t(b) * args.page_stride;
+            auto page_at = [&](int tile) {
+                const int position = tile * kTileKeys + (mine << args.box_shift);
+                return mine < boxes && position < s.length ? load_index(pages + (position >> args.page_shift)) : -1;
+            };
+            // Heads outermost: their query tiles read the same keys, near one another in time.
+            for (int segment = 0; open && segment < query_count * args.kv_heads && at < end; ++segment) {
+                const int head = segment / query_count, qt = segment - head * query_count, tiles = tiles_of<kColumns>(args, s, qt);
+                const long long first_unit = at + extra;
+                at = first_unit + (long long)kTileUnits * tiles;
+                const auto tile_from = [&](long long unit) { // first tile that starts at or behind a unit
+                    return unit <= first_unit ? 0 : unit >= at ? tiles : int((unit - first_unit + kTileUnits - 1) / kTileUnits);
+                };
+                const int low = tile_from(begin), high = tile_from(end);
+                if (low == high) continue;
+                int first_cta = -1, first_slot = 0;
+                const bool split = low || high < tiles;
+                if (split && high == tiles) { // this CTA closes the segment: it says where its parts lie
+                    first_cta = int(first_unit * ctas / total);
+                    while (total * (first_cta + 1) / ctas <= first_unit) ++first_cta;
+                    first_slot = total * first_cta / ctas < first_unit - extra ? 1 : 0;
                 }
-                ptx::mbar_arrive_expect_tx(bar, copied * box_bytes);
+                const int columns = min(kColumns, s.count * args.group - qt * kColumns);
+                int next = page_at(low);
+                for (int tile = low; tile < high; ++tile) {
+                    const int page = next;
+                    if (tile + 1 < high) next = page_at(tile + 1); // on its way while this tile's stage is waited for
+                    if (issued >= stages && !wait(empty[stage], phase ^ 1)) {
+                        open = false;
+                        break;
+                    }
+                    const uint32_t to = ring + stage * Shape::stage, bar = ptx::smem_u32(&full[issued & 1][stage]);
+                    uint8_t *const bytes = ring_bytes + stage * Shape::stage;
+                    const int position = tile * kTileKeys + (mine << args.box_shift), offset = mine << args.box_shift;
+                    const bool wanted = mine < boxes && position < s.length, good = wanted && unsigned(page) < unsigned(args.total_pages);
+                    // Positions on a page that the cache does not have read as NaN.
+                    if (wanted && !good && kind >= 2)
+                        for (int i = 0; i < box; ++i)
+                            reinterpret_cast<float *>(bytes + Shape::scales)[(kind - 2) * kTileKeys + offset + i] = __int_as_float(0x7fffffff);
+                    // Each group's first tile of the part brings the query rows.
+                    const bool first = tile - low < 2;
+                    const int flat = qt * kColumns + lane;
+                    const T *query = static_cast<const T *>(args.queries) + size_t(s.row + flat / args.group) * args.query_stride +
+                                     (head * args.group + flat % args.group) * HeadDim;
+                    if (first && !args.aligned && lane < columns)
+                        for (int d = 0; d < HeadDim; ++d) {
+                            uint16_t v;
+                            asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(query + d) : "memory");
+                            *reinterpret_cast<uint16_t *>(bytes + Shape::queries + lane * Shape::query_row + 2 * d) = v;
+                        }
+                    const bool query_copy = first && args.aligned && lane < columns;
+                    __syncwarp();
+                    const uint32_t copied = __popc(__ballot_sync(0xffffffffu, good)) / 4, rows = __popc(__ballot_sync(0xffffffffu, query_copy));
+                    if (!lane) {
+                        TileNote &n = notes[stage];
+                        n.key = tile * kTileKeys, n.head = head, n.row = s.row, n.count = s.count, n.flat = qt * kColumns;
+                        n.limit = args.prefix ? s.length - 1 : s.length - s.count;
+                        n.flags = (first ? kNoteFirst : 0) | (tile + 2 >= high ? kNoteFlush : 0) | (tile + 1 == high ? kNoteEnd : 0) |
+                                  (high - low == 1 ? kNoteAlone : 0) | (high < tiles || at + extra >= end ? kNoteFinal : 0) | (split ? kNoteSplit : 0);
+                        n.ordinal = ordinal, n.first_cta = first_cta, n.first_slot = first_slot;
+                        n.slot = first_unit - extra > begin ? 1 : 0;
+                        ptx::mbar_arrive_expect_tx(bar, copied * box_bytes + rows * HeadDim * 2);
+                    }
+                    __syncwarp();
+                    if (query_copy) copy_run(to + Shape::queries + lane * Shape::query_row, query, HeadDim * 2, bar);
+                    if (good) {
+                        const int row = (((page * args.kv_heads) + head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
+                        if (kind == 0) ptx::tma_load_2d(to + offset * HeadDim, &key_map, bar, 0, row);
+                        else if (kind == 1) ptx::tma_load_2d(to + Shape::values + offset * HeadDim, &value_map, bar, 0, row);
+                        else copy_run(to + Shape::scales + ((kind - 2) * kTileKeys + offset) * 4, (kind == 2 ? args.key_scales : args.value_scales) + row, uint32_t(box) * 4, bar);
+                    }
+                    ++issued;
+                    if (++stage == stages) stage = 0, phase ^= 1;
+                }
+                ++ordinal;
             }
-            __syncwarp();
-            if (good) {
-                const int row = (((page * args.kv_heads) + h) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
-                const uint32_t offset = uint32_t(mine << args.box_shift);
-                if (kind == 0) ptx::tma_load_2d(at + offset * HeadDim, &key_map, bar, 0, row);
-                else if (kind == 1) ptx::tma_load_2d(at + Shape::values + offset * HeadDim, &value_map, bar, 0, row);
-                else copy_run(at + Shape::scales + (kind - 2) * kTileKeys * 4 + offset * 4, (kind == 2 ? args.key_scales : args.value_scales) + row, uint32_t(box) * 4, bar);
-            }
-            if (++tile == tiles && issued + 1 < count) {
-                tile = 0;
-                next_segment();
-            }
-            if (++stage == kStages) stage = 0, phase ^= 1;
         }
-        // No copy may be in flight when the CTA leaves, whatever the consumers did.
+        for (int team = 0; team < 2 && open; ++team) { // an empty stage ends each group
+            if (issued >= stages && !wait(empty[stage], phase ^ 1)) break;
+            if (!lane) {
+                notes[stage].flags = kNoteQuit;
+                ptx::mbar_arrive(ptx::smem_u32(&full[issued & 1][stage]));
+            }
+            ++issued;
+            if (++stage == stages) stage = 0, phase ^= 1;
+        }
+        if (!ordinal && !lane) { // a share that holds no tile's first unit
+            merge_notes[0].flags = kNoteQuit;
+            for (int w = 0; w < kWorkers; ++w) ptx::mbar_arrive(ptx::smem_u32(&merge_full[0]));
+        }
+        // No copy may be in flight when the CTA leaves, whatever the workers did.
         int ignored = 0;
-        for (int i = max(0, issued - kStages); i < issued; ++i)
-            ptx::mbar_wait(ptx::smem_u32(&full[i % kStages]), uint32_t(i / kStages) & 1, &ignored);
+        for (int i = max(0, issued - stages); i < issued; ++i) ptx::mbar_wait(ptx::smem_u32(&full[i & 1][i % stages]), uint32_t((i >> 1) / period) & 1, &ignored);
         return;
     }
 
-    // ------------------------------------------------------------------------------------------- consumers
-    const int g = lane >> 2, t = lane & 3;
-    uint32_t q[Tiles][kSteps][2];
-    float out[Tiles][kSteps][4], most[Tiles][2], sum[Tiles][2], factor[Tiles][2];
-    int limit[Tiles][2], least = 0;
-    int stage = 0, segments = 0;
-    uint32_t phase = 0;
-    for (int i = 0; i < count; ++i) {
-        if (!wait(full[stage], phase)) return;
-        const TileNote &note = notes[stage];
-        const uint32_t at = ring + stage * Shape::stage_aligned;
-        const float *scales = reinterpret_cast<const float *>(raw_smem + (at - ptx::smem_u32(raw_smem)) + Shape::scales);
-        const int flags = note.flags;
-        if (flags & kNoteFirst) {
-            const int columns = note.count * args.group - note.flat;
-            least = INT_MAX;
-#pragma unroll
-            for (int n = 0; n < Tiles; ++n) {
-                // This lane's share of query row 8n + g: columns [HeadDim / 4 * t, HeadDim / 4 * (t + 1)).
-                constexpr int kShare = HeadDim / 4;
-                const int column = 8 * n + g, flat = note.flat + column;
-                const bool live = column < columns;
-                const T *row = static_cast<const T *>(args.queries) + size_t(note.row + flat / args.group) * args.query_stride +
-                               (note.head * args.group + flat % args.group) * HeadDim + kShare * t;
-                alignas(16) T share[kShare];
-                if (live && args.aligned) {
-#pragma unroll
-                    for (int c = 0; c < kShare / 8; ++c) {
-                        uint4 v;
-                        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + 8 * c) : "memory");
-                        *reinterpret_cast<uint4 *>(share + 8 * c) = v;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < kShare; ++c) {
-                        uint16_t v = 0;
-                        if (live) asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(row + c) : "memory");
-                        reinterpret_cast<uint16_t *>(share)[c] = v;
-                    }
-                }
-                unsigned largest = 0;
-#pragma unroll
-                for (int c = 0; c < kShare; ++c) largest = max(largest, __float_as_uint(float(share[c])) & 0x7fffffffu);
-                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                const int exponent = largest && largest < 0x7f800000u ? max(int(largest >> 23), 1) - 127 : 0;
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const __half2 v = __floats2half2_rn(ldexpf(float(share[4 * k + 2 * c]), -exponent), ldexpf(float(share[4 * k + 2 * c + 1]), -exponent));
-                        q[n][k][c] = *reinterpret_cast<const uint32_t *>(&v);
-                    }
-                // The scores of this lane belong to columns 2t and 2t + 1, whose rows lanes 8t and 8t + 4 hold.
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int of = __shfl_sync(0xffffffffu, exponent, 8 * t + 4 * c), seen = 8 * n + 2 * t + c;
-                    factor[n][c] = ldexpf(args.score_scale, of);
-                    limit[n][c] = seen < columns ? (args.prefix ? note.limit : note.limit + (note.flat + seen) / args.group) : -1;
-                    if (seen < columns) least = min(least, limit[n][c]);
-                    most[n][c] = -INFINITY;
-                    sum[n][c] = 0.f;
-                }
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) out[n][k][c] = 0.f;
-            }
-            least = __reduce_min_sync(0xffffffffu, least);
-        }
-
-        // Scores of this warp's 16 keys.
-        const int row = 16 * warp;
-        uint32_t keys[2][HeadDim / 16];
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int c = 0; c < HeadDim / 64; ++c)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(keys[r][4 * c]), "=r"(keys[r][4 * c + 1]), "=r"(keys[r][4 * c + 2]), "=r"(keys[r][4 * c + 3])
-                             : "r"(at + piece<HeadDim>(row + g + 8 * r, HeadDim / 64 * t + c)));
-        float scores[Tiles][2][4] = {};
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            uint32_t a[4];
-            widen<F>(biased<F>(keys[0][k]), a[0], a[2]);
-            widen<F>(biased<F>(keys[1][k]), a[1], a[3]);
-#pragma unroll
-            for (int n = 0; n < Tiles; ++n) mma_f16(scores[n][k & 1], a[0], a[1], a[2], a[3], q[n][k][0], q[n][k][1]);
-        }
-        // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9: this thread's 16 (8) columns.
-        uint32_t values[4][HeadDim / 32];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int key = row + 2 * t + (r & 1) + 8 * (r >> 1);
-            if constexpr (HeadDim == 128)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                             : "=r"(values[r][0]), "=r"(values[r][1]), "=r"(values[r][2]), "=r"(values[r][3])
-                             : "r"(at + Shape::values + piece<HeadDim>(key, g)));
-            else
-                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                             : "=r"(values[r][0]), "=r"(values[r][1])
-                             : "r"(at + Shape::values + piece<HeadDim>(key, g >> 1) + 8 * (g & 1)));
-        }
-        const float key_scale[2] = {scales[row + g], scales[row + g + 8]};
-        float value_scale[2] = {scales[kTileKeys + row + g], scales[kTileKeys + row + g + 8]};
-        const int position = note.key + row + g;
-        const bool masked = note.key + kTileKeys - 1 > least;
-        uint32_t weights[Tiles][2];
-#pragma unroll
-        for (int n = 0; n < Tiles; ++n) {
-            float x[2][2], highest[2] = {-INFINITY, -INFINITY};
-            bool seen[2][2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float shift = fmaxf(log2_approx(fabsf(value_scale[r])), -126.f);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    seen[r][c] = !masked || position + 8 * r <= limit[n][c];
-                    x[r][c] = (scores[n][0][2 * r + c] + scores[n][1][2 * r + c]) * (key_scale[r] * factor[n][c]);
-                    if (!seen[r][c]) x[r][c] = -INFINITY;
-                    else highest[c] = fmaxf(highest[c], x[r][c] + shift);
-                }
-            }
-            float raised[2];
-            bool changed = false;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int d = 4; d < 32; d <<= 1) highest[c] = fmaxf(highest[c], __shfl_xor_sync(0xffffffffu, highest[c], d));
-                raised[c] = fmaxf(most[n][c], highest[c]);
-                changed |= raised[c] > most[n][c];
-            }
-            if (__any_sync(0xffffffffu, changed)) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const float shrink = raised[c] == -INFINITY ? 1.f : exp2_approx(most[n][c] - raised[c]);
-                    sum[n][c] *= shrink;
-#pragma unroll
-                    for (int k = 0; k < kSteps; ++k) out[n][k][c] *= shrink, out[n][k][2 + c] *= shrink;
-                    most[n][c] = raised[c];
-                }
-            }
-            float w[2][2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float reference = most[n][c] == -INFINITY ? 0.f : most[n][c];
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float p = exp2_approx(x[r][c] - reference);
-                    sum[n][c] += p;
-                    w[r][c] = seen[r][c] ? p * value_scale[r] : 0.f; // a hidden row's scale may be anything
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const __half2 both = __floats2half2_rn(w[r][0], w[r][1]);
-                weights[n][r] = transpose8x8(*reinterpret_cast<const uint32_t *>(&both));
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const uint32_t order = k & 1 ? 0x7362u : 0x5140u; // bytes 2 (k & 1) and the next of two keys, side by side
-            uint32_t a[4];
-            widen<F>(biased<F>(__byte_perm(values[0][k >> 1], values[1][k >> 1], order)), a[0], a[1]);
-            widen<F>(biased<F>(__byte_perm(values[2][k >> 1], values[3][k >> 1], order)), a[2], a[3]);
-#pragma unroll
-            for (int n = 0; n < Tiles; ++n) mma_f16(out[n][k], a[0], a[1], a[2], a[3], weights[n][0], weights[n][1]);
-        }
-
-        if (flags & kNoteLast) { // the eight warps' shares of the segment meet
-            const int columns = min(kColumns, note.count * args.group - note.flat);
-            if (segments && !wait(meet[1], uint32_t(segments - 1) & 1)) return;
-#pragma unroll
-            for (int n = 0; n < Tiles; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float l = sum[n][c];
-#pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-                    const int column = 8 * n + 2 * t + c;
-                    if (column >= columns) continue;
-                    float *to = merge + (warp * kColumns + column) * Shape::row;
-#pragma unroll
-                    for (int k = 0; k < kSteps; k += 2)
-                        *reinterpret_cast<float4 *>(to + g * kSteps * 2 + 2 * k) =
-                            make_float4(out[n][k][c], out[n][k][2 + c], out[n][k + 1][c], out[n][k + 1][2 + c]);
-                    if (!g) to[HeadDim] = most[n][c], to[HeadDim + 1] = l;
-                }
-            __syncwarp();
-            if (!lane) ptx::mbar_arrive(ptx::smem_u32(&meet[0]));
-            if (!wait(meet[0], uint32_t(segments) & 1)) return;
-            for (int item = threadIdx.x; item < columns * (HeadDim / 4); item += 32 * kAttentionWarps) {
+    if (warp > kProducer) { // -------------------------------------------------------------------- mergers
+        for (int ordinal = 0;; ++ordinal) {
+            const int buffer = ordinal % args.merge_buffers;
+            if (!wait(merge_full[buffer], uint32_t(ordinal / args.merge_buffers) & 1)) return;
+            const TileNote &note = merge_notes[buffer];
+            if (note.flags & kNoteQuit) return;
+            const float *shares = merge + buffer * merge_floats;
+            const int columns = min(kColumns, note.count * args.group - note.flat), flags = note.flags;
+            const int low = flags & kNoteAlone ? note.pad[0] * (kWorkers / 2) : 0, high = flags & kNoteAlone ? low + kWorkers / 2 : kWorkers;
+            for (int item = threadIdx.x - 32 * (kProducer + 1); item < columns * (HeadDim / 4); item += 32 * kMergers) {
                 const int column = item / (HeadDim / 4), d = 4 * (item % (HeadDim / 4));
                 float highest = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kAttentionWarps; ++w) highest = fmaxf(highest, merge[(w * kColumns + column) * Shape::row + HeadDim]);
+                for (int w = low; w < high; ++w) highest = fmaxf(highest, shares[(w * args.merge_columns + column) * Shape::row + HeadDim]);
                 const float reference = highest == -INFINITY ? 0.f : highest;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                 float l = 0.f;
-#pragma unroll
-                for (int w = 0; w < kAttentionWarps; ++w) {
-                    const float *from = merge + (w * kColumns + column) * Shape::row;
+#pragma unroll 4
+                for (int w = low; w < high; ++w) {
+                    const float *from = shares + (w * args.merge_columns + column) * Shape::row;
                     const float f = exp2_approx(from[HeadDim] - reference);
                     const float4 x = *reinterpret_cast<const float4 *>(from + d);
                     v.x += f * x.x, v.y += f * x.y, v.z += f * x.z, v.w += f * x.w;
@@ -555,12 +434,224 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                 }
             }
             __syncwarp();
-            if (!lane) ptx::mbar_arrive(ptx::smem_u32(&meet[1]));
-            ++segments;
+            if (!lane) {
+                __threadfence_block();
+                atomicAdd(&merged, 1);
+            }
+            if (flags & kNoteFinal) return;
+        }
+    }
+
+    // --------------------------------------------------------------------------------------------- workers
+    const int g = lane >> 2, t = lane & 3, team = warp >> 2, row = 32 * (warp & 3);
+    uint32_t q[Tiles][kSteps][2];
+    float out[Tiles][kSteps][4], most[Tiles][2], sum[Tiles][2], factor[Tiles][2];
+    int limit[Tiles][2], least = 0;
+    int stage = team, seen_stages = 0;
+    uint32_t phase = 0;
+    for (;;) {
+        if (!wait(full[team][stage], phase)) return;
+        const TileNote &note = notes[stage];
+        const uint32_t at = ring + stage * Shape::stage;
+        const uint8_t *bytes = ring_bytes + stage * Shape::stage;
+        const float *scales = reinterpret_cast<const float *>(bytes + Shape::scales);
+        const int flags = note.flags;
+        if (flags & kNoteQuit) return;
+        if (flags & kNoteFirst) {
+            const int columns = note.count * args.group - note.flat;
+            least = INT_MAX;
+#pragma unroll
+            for (int n = 0; n < Tiles; ++n) {
+                // This lane's share of query row 8n + g: columns [HeadDim / 4 * t, HeadDim / 4 * (t + 1)).
+                constexpr int kShare = HeadDim / 4;
+                const bool live = 8 * n + g < columns;
+                alignas(16) T share[kShare];
+#pragma unroll
+                for (int c = 0; c < kShare / 8; ++c) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(bytes + Shape::queries + (8 * n + g) * Shape::query_row + (kShare * t + 8 * c) * 2);
+                    *reinterpret_cast<uint4 *>(share + 8 * c) = live ? v : make_uint4(0, 0, 0, 0);
+                }
+                unsigned largest = 0;
+#pragma unroll
+                for (int c = 0; c < kShare; ++c) largest = max(largest, __float_as_uint(float(share[c])) & 0x7fffffffu);
+                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                const int exponent = largest && largest < 0x7f800000u ? max(int(largest >> 23), 1) - 127 : 0;
+                const float down = __int_as_float(exponent < 127 ? (127 - exponent) << 23 : 0x00400000); // 2^-exponent
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const __half2 v = __floats2half2_rn(float(share[4 * k + 2 * c]) * down, float(share[4 * k + 2 * c + 1]) * down);
+                        q[n][k][c] = *reinterpret_cast<const uint32_t *>(&v);
+                    }
+                // The scores of this lane belong to columns 2t and 2t + 1, whose rows lanes 8t and 8t + 4 hold.
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int of = __shfl_sync(0xffffffffu, exponent, 8 * t + 4 * c), seen = 8 * n + 2 * t + c;
+                    factor[n][c] = ldexpf(args.score_scale, of);
+                    limit[n][c] = seen < columns ? (args.prefix ? note.limit : note.limit + (note.flat + seen) / args.group) : -1;
+                    if (seen < columns) least = min(least, limit[n][c]);
+                    most[n][c] = -INFINITY;
+                    sum[n][c] = 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) out[n][k][c] = 0.f;
+            }
+            least = __reduce_min_sync(0xffffffffu, least);
+        }
+
+        // Scores of this warp's 32 keys, two blocks of 16.
+        float scores[Tiles][2][4] = {};
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            uint32_t keys[2][HeadDim / 16];
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int c = 0; c < HeadDim / 64; ++c)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(keys[r][4 * c]), "=r"(keys[r][4 * c + 1]), "=r"(keys[r][4 * c + 2]), "=r"(keys[r][4 * c + 3])
+                                 : "r"(at + piece<HeadDim>(row + 16 * m + g + 8 * r, HeadDim / 64 * t + c)));
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t a[4];
+                widen<F>(biased<F>(keys[0][k]), a[0], a[2]);
+                widen<F>(biased<F>(keys[1][k]), a[1], a[3]);
+#pragma unroll
+                for (int n = 0; n < Tiles; ++n) mma_f16(scores[n][m], a[0], a[1], a[2], a[3], q[n][k][0], q[n][k][1]);
+            }
+        }
+        float key_scale[2][2], value_scale[2][2], shift[2][2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                key_scale[m][r] = scales[row + 16 * m + g + 8 * r];
+                value_scale[m][r] = scales[kTileKeys + row + 16 * m + g + 8 * r];
+                shift[m][r] = fmaxf(log2_approx(fabsf(value_scale[m][r])), -126.f);
+            }
+        const int position = note.key + row + g;
+        const bool masked = note.key + kTileKeys - 1 > least;
+        uint32_t weights[Tiles][2][2];
+#pragma unroll
+        for (int n = 0; n < Tiles; ++n) {
+            float highest[2] = {-INFINITY, -INFINITY};
+            unsigned hidden = 0;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        float &x = scores[n][m][2 * r + c];
+                        x *= key_scale[m][r] * factor[n][c];
+                        if (masked && position + 16 * m + 8 * r > limit[n][c]) {
+                            hidden |= 1u << (4 * m + 2 * r + c);
+                            x = -INFINITY;
+                        }
+                        highest[c] = fmaxf(highest[c], hidden & (1u << (4 * m + 2 * r + c)) ? -INFINITY : x + shift[m][r]);
+                    }
+            float raised[2];
+            bool changed = false;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) highest[c] = fmaxf(highest[c], __shfl_xor_sync(0xffffffffu, highest[c], d));
+                raised[c] = fmaxf(most[n][c], highest[c]);
+                changed |= raised[c] > most[n][c];
+            }
+            if (__any_sync(0xffffffffu, changed)) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float shrink = raised[c] == -INFINITY ? 1.f : exp2_approx(most[n][c] - raised[c]);
+                    sum[n][c] *= shrink;
+#pragma unroll
+                    for (int k = 0; k < kSteps; ++k) out[n][k][c] *= shrink, out[n][k][2 + c] *= shrink;
+                    most[n][c] = raised[c];
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float w[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float p = exp2_approx(scores[n][m][2 * r + c] - (most[n][c] == -INFINITY ? 0.f : most[n][c]));
+                        sum[n][c] += p;
+                        w[c] = hidden & (1u << (4 * m + 2 * r + c)) ? 0.f : p * value_scale[m][r]; // a hidden row's scale may be anything
+                    }
+                    const __half2 both = __floats2half2_rn(w[0], w[1]);
+                    weights[n][m][r] = transpose8x8(*reinterpret_cast<const uint32_t *>(&both));
+                }
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9 of the block: this thread's 16 (8) columns.
+            uint32_t values[4][HeadDim / 32];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int key = row + 16 * m + 2 * t + (r & 1) + 8 * (r >> 1);
+                if constexpr (HeadDim == 128)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(values[r][0]), "=r"(values[r][1]), "=r"(values[r][2]), "=r"(values[r][3])
+                                 : "r"(at + Shape::values + piece<HeadDim>(key, g)));
+                else
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                                 : "=r"(values[r][0]), "=r"(values[r][1])
+                                 : "r"(at + Shape::values + piece<HeadDim>(key, g >> 1) + 8 * (g & 1)));
+            }
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                const uint32_t order = k & 1 ? 0x7362u : 0x5140u; // bytes 2 (k & 1) and the next of two keys, side by side
+                uint32_t a[4];
+                widen<F>(biased<F>(__byte_perm(values[0][k >> 1], values[1][k >> 1], order)), a[0], a[1]);
+                widen<F>(biased<F>(__byte_perm(values[2][k >> 1], values[3][k >> 1], order)), a[2], a[3]);
+#pragma unroll
+                for (int n = 0; n < Tiles; ++n) mma_f16(out[n][k], a[0], a[1], a[2], a[3], weights[n][m][0], weights[n][m][1]);
+            }
+        }
+
+        if (flags & kNoteFlush) { // this warp's share of the segment's part; the mergers add the shares up
+            const int ordinal = note.ordinal, buffer = ordinal % args.merge_buffers;
+            const int columns = min(kColumns, note.count * args.group - note.flat);
+            // A count and not a barrier's phase: a group has no tile in some parts, and could be two phases off.
+            if (ordinal >= args.merge_buffers && !wait_merged(kMergers * (ordinal - args.merge_buffers + 1))) return;
+            float *const shares = merge + buffer * merge_floats + warp * args.merge_columns * Shape::row;
+#pragma unroll
+            for (int n = 0; n < Tiles; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float l = sum[n][c];
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                    const int column = 8 * n + 2 * t + c;
+                    if (column >= columns) continue;
+                    float *to = shares + column * Shape::row;
+#pragma unroll
+                    for (int k = 0; k < kSteps; k += 2)
+                        *reinterpret_cast<float4 *>(to + g * kSteps * 2 + 2 * k) =
+                            make_float4(out[n][k][c], out[n][k][2 + c], out[n][k + 1][c], out[n][k + 1][2 + c]);
+                    if (!g) to[HeadDim] = most[n][c], to[HeadDim + 1] = l;
+                }
+            if ((flags & kNoteEnd) && !(warp & 3) && !lane) {
+                merge_notes[buffer] = note;
+                merge_notes[buffer].pad[0] = team;
+            }
+            __syncwarp();
+            if (!lane) {
+                ptx::mbar_arrive(ptx::smem_u32(&merge_full[buffer]));
+                if (flags & kNoteAlone) ptx::mbar_arrive(ptx::smem_u32(&merge_full[buffer])); // for the group that has no tile of this part
+            }
         }
         __syncwarp();
         if (!lane) ptx::mbar_arrive(ptx::smem_u32(&empty[stage]));
-        if (++stage == kStages) stage = 0, phase ^= 1;
+        stage += 2;
+        if (stage >= stages) stage -= stages;
+        if (++seen_stages == period) seen_stages = 0, phase ^= 1;
     }
 }
 

@@ -74,7 +74,7 @@ class Batch:
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("lengths,heads,kv_heads,head_dim,page", [
     ([1], 1, 1, 64, 16), ([16], 2, 1, 128, 16), ([17, 0, 128, 1], 4, 2, 128, 16), ([129, 127, 300], 8, 1, 64, 32),
-    ([2000], 16, 8, 128, 64), ([5, 640, 0, 33, 257, 1], 12, 3, 128, 256), ([700, 90], 16, 1, 64, 1024), ([400] * 9, 10, 2, 128, 128)])
+    ([2000], 16, 8, 128, 64), ([10, 300, 20, 30, 129, 500, 7, 90] * 6, 8, 4, 64, 16), ([5, 640, 0, 33, 257, 1], 12, 3, 128, 256), ([700, 90], 16, 1, 64, 1024), ([400] * 9, 10, 2, 128, 128)])
 def test_one_query_per_sequence(ctx_factory, lengths, heads, kv_heads, head_dim, page, fmt, dtype):
     batch = Batch(len(lengths), lengths, None, heads, kv_heads, head_dim, page, FORMATS[fmt], DTYPES[dtype])
     check(batch.run(ctx_factory("int8")), *batch.want())
@@ -84,7 +84,9 @@ def test_one_query_per_sequence(ctx_factory, lengths, heads, kv_heads, head_dim,
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("lengths,counts,heads,kv_heads,head_dim,page", [
     ([40], [40], 2, 1, 128, 16), ([300, 7, 0, 130], [5, 7, 0, 1], 4, 2, 128, 32), ([260, 129], [130, 65], 3, 1, 64, 64),
-    ([3, 500], [9, 2], 8, 4, 64, 16), ([1100], [3], 16, 8, 128, 128)])
+    ([3, 500], [9, 2], 8, 4, 64, 16), ([1100], [3], 16, 8, 128, 128),
+    # More segments than multiprocessors, many of a single tile between longer ones.
+    ([100, 700, 90], [60, 50, 60], 16, 8, 64, 32), ([130, 60, 257, 40], [40, 33, 70, 40], 8, 8, 128, 16)])
 def test_some_queries_per_sequence(ctx_factory, lengths, counts, heads, kv_heads, head_dim, page, fmt, dtype):
     # The fourth has more query rows than cached tokens: the first ones see nothing. Rows behind the last sequence stay.
     batch = Batch(sum(counts), lengths, counts, heads, kv_heads, head_dim, page, FORMATS[fmt], DTYPES[dtype], spare_rows=3)
