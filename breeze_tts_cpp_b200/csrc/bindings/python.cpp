@@ -16,7 +16,9 @@
 namespace {
 PyObject *error_type = nullptr;  // breeze_tts_cpp_b200.B200QError
 PyObject *view_method = nullptr; // RowScaledView.c as defined by the package
+PyObject *cache_method = nullptr, *rotary_method = nullptr; // CacheView.c, Rotary.c
 PyObject *name_values, *name_scales, *name_format, *name_group, *name_rotation, *name_c;
+PyObject *name_keys, *name_key_scales, *name_value_scales, *name_turns, *name_interleaved, *name_scale;
 
 constexpr b200q_tensor kNone{nullptr, 0, 0, 0, 0, -1};
 
@@ -89,6 +91,57 @@ bool view_of(PyObject *object, b200q_row_scaled &out) {
     return int_of(format.p, code) && code >= 0 && values.p != Py_None && scales.p != Py_None &&
            tensor_of(values.p, out.values, code) && tensor_of(scales.p, out.scales, B200Q_F32) &&
            int_of(group.p, out.group_size) && int_of(rotation.p, out.rotation_size);
+}
+bool has_method(PyObject *object, PyObject *method) {
+    const Ref c(PyObject_GetAttr(object, name_c));
+    return c.p && PyMethod_Check(c.p) && PyMethod_GET_FUNCTION(c.p) == method;
+}
+// One of a CacheView's tensors, of the shape (or the leading shape) that its keys have; null = not one.
+void *part_of(PyObject *object, bool scales, at::IntArrayRef &shape, int &device) {
+    if (!THPVariable_Check(object)) return nullptr;
+    const at::Tensor &t = THPVariable_Unpack(object);
+    if (!t.is_cuda() || !t.is_contiguous() || t.dim() != (scales ? 3 : 4)) return nullptr;
+    if (scales ? t.scalar_type() != c10::ScalarType::Float : t.element_size() != 1) return nullptr;
+    if (device < 0) {
+        shape = t.sizes();
+        device = t.get_device();
+    } else if (t.get_device() != device || t.sizes() != shape.slice(0, scales ? 3 : 4)) {
+        return nullptr;
+    }
+    return t.data_ptr();
+}
+bool cache_of(PyObject *object, b200q_cache &out) {
+    if (!has_method(object, cache_method)) return false;
+    const Ref keys(PyObject_GetAttr(object, name_keys)), values(PyObject_GetAttr(object, name_values)),
+        key_scales(PyObject_GetAttr(object, name_key_scales)), value_scales(PyObject_GetAttr(object, name_value_scales)),
+        format(PyObject_GetAttr(object, name_format));
+    if (!keys.p || !values.p || !key_scales.p || !value_scales.p || !format.p || !int_of(format.p, out.type)) return false;
+    at::IntArrayRef shape;
+    int device = -1;
+    out.keys = part_of(keys.p, false, shape, device);
+    if (!out.keys) return false;
+    out.values = part_of(values.p, false, shape, device);
+    out.key_scales = static_cast<float *>(part_of(key_scales.p, true, shape, device));
+    out.value_scales = static_cast<float *>(part_of(value_scales.p, true, shape, device));
+    if (!out.values || !out.key_scales || !out.value_scales) return false;
+    for (const int64_t n : shape)
+        if (n > INT32_MAX) return false;
+    out.pages = int32_t(shape[0]), out.kv_heads = int32_t(shape[1]), out.page_size = int32_t(shape[2]), out.head_dim = int32_t(shape[3]);
+    out.device = device;
+    return true;
+}
+bool rotary_of(PyObject *object, b200q_rotary_plan &out) {
+    if (!has_method(object, rotary_method)) return false;
+    const Ref turns(PyObject_GetAttr(object, name_turns)), interleaved(PyObject_GetAttr(object, name_interleaved)),
+        scale(PyObject_GetAttr(object, name_scale));
+    if (!turns.p || !interleaved.p || !scale.p || !int_of(interleaved.p, out.interleaved) || !float_of(scale.p, out.scale) ||
+        !THPVariable_Check(turns.p))
+        return false;
+    const at::Tensor &t = THPVariable_Unpack(turns.p);
+    if (!t.is_cuda() || t.scalar_type() != c10::ScalarType::Double || t.dim() != 1 || !t.is_contiguous() || t.numel() > INT32_MAX / 2) return false;
+    out.turns = static_cast<const double *>(t.data_ptr());
+    out.dims = int32_t(2 * t.numel()), out.device = t.get_device();
+    return true;
 }
 // Device pointer of an int32 index tensor (the ABI takes the bare pointer).
 bool rows_of(PyObject *object, const int32_t *&out) {
@@ -289,12 +342,56 @@ PyObject *layer_norm_quantize(PyObject *, Args a, Py_ssize_t n) { // context, x,
         return b200q_layer_norm_quantize(c, &x, &out, &weight, &bias, epsilon, &f, &retained, m, s);
     });
 }
-PyObject *bind(PyObject *, Args a, Py_ssize_t n) { // error type, RowScaledView.c
-    if (n != 2) return declined();
-    Py_XDECREF(error_type);
-    Py_XDECREF(view_method);
-    error_type = Py_NewRef(a[0]);
-    view_method = Py_NewRef(a[1]);
+PyObject *rotary(PyObject *, Args a, Py_ssize_t n) { // context, x, positions, rotary, head_dim, out
+    b200q_tensor x, positions, out;
+    b200q_rotary_plan plan;
+    int32_t head_dim;
+    if (n != 6 || !tensor_of(a[1], x) || !tensor_of(a[2], positions) || !rotary_of(a[3], plan) || !int_of(a[4], head_dim) || !tensor_of(a[5], out))
+        return declined();
+    auto *c = handle_of<b200q_context>(a[0]);
+    return finish("b200q_rotary", [&](char *m, size_t s) { return b200q_rotary(c, &x, &positions, &plan, head_dim, &out, m, s); });
+}
+// context, cache, k, v, slots, positions, rotary, q, q_out, q_norm, k_norm, epsilon
+PyObject *cache_write(PyObject *, Args a, Py_ssize_t n) {
+    b200q_cache cache;
+    b200q_tensor k, v, slots, positions, q, q_out, q_norm, k_norm;
+    b200q_rotary_plan plan;
+    float epsilon;
+    if (n != 12 || !cache_of(a[1], cache) || !tensor_of(a[2], k) || !tensor_of(a[3], v) || !tensor_of(a[4], slots) || !tensor_of(a[5], positions) ||
+        (a[6] != Py_None && !rotary_of(a[6], plan)) || !tensor_of(a[7], q) || !tensor_of(a[8], q_out) || !tensor_of(a[9], q_norm) ||
+        !tensor_of(a[10], k_norm) || !float_of(a[11], epsilon))
+        return declined();
+    auto *c = handle_of<b200q_context>(a[0]);
+    const b200q_rotary_plan *turning = a[6] == Py_None ? nullptr : &plan;
+    return finish("b200q_cache_write", [&](char *m, size_t s) {
+        return b200q_cache_write(c, &cache, &k, &v, &slots, &positions, turning, &q, &q_out, &q_norm, &k_norm, epsilon, m, s);
+    });
+}
+PyObject *cache_read(PyObject *, Args a, Py_ssize_t n) { // context, cache, slots, k, v
+    b200q_cache cache;
+    b200q_tensor slots, k, v;
+    if (n != 5 || !cache_of(a[1], cache) || !tensor_of(a[2], slots) || !tensor_of(a[3], k) || !tensor_of(a[4], v)) return declined();
+    auto *c = handle_of<b200q_context>(a[0]);
+    return finish("b200q_cache_read", [&](char *m, size_t s) { return b200q_cache_read(c, &cache, &slots, &k, &v, m, s); });
+}
+// context, q, cache, pages, lengths, out, scale, query_offsets, prefix_pages, prefix_length
+PyObject *cached_attention(PyObject *, Args a, Py_ssize_t n) {
+    b200q_cache cache;
+    b200q_attention p;
+    if (n != 10 || !tensor_of(a[1], p.queries) || !cache_of(a[2], cache) || !tensor_of(a[3], p.pages) || !tensor_of(a[4], p.lengths) ||
+        !tensor_of(a[5], p.output) || !float_of(a[6], p.scale) || !tensor_of(a[7], p.query_offsets) || !tensor_of(a[8], p.prefix_pages) ||
+        !tensor_of(a[9], p.prefix_length))
+        return declined();
+    auto *c = handle_of<b200q_context>(a[0]);
+    return finish("b200q_cached_attention", [&](char *m, size_t s) { return b200q_cached_attention(c, &cache, &p, m, s); });
+}
+PyObject *bind(PyObject *, Args a, Py_ssize_t n) { // error type, RowScaledView.c, CacheView.c, Rotary.c
+    if (n != 4) return declined();
+    PyObject **const kept[] = {&error_type, &view_method, &cache_method, &rotary_method};
+    for (int i = 0; i < 4; ++i) {
+        Py_XDECREF(*kept[i]);
+        *kept[i] = Py_NewRef(a[i]);
+    }
     Py_RETURN_NONE;
 }
 
@@ -311,7 +408,8 @@ template <PyObject *(*Method)(PyObject *, Args, Py_ssize_t)> PyObject *guarded(P
 PyMethodDef methods[] = {B200Q_METHOD(row_quantize),   B200Q_METHOD(quantized_norm),      B200Q_METHOD(quantized_gated),
                          B200Q_METHOD(linear),         B200Q_METHOD(linear_forward),      B200Q_METHOD(layer_forward),
                          B200Q_METHOD(pointwise),      B200Q_METHOD(pointwise_quantize),  B200Q_METHOD(layer_norm_quantize),
-                         B200Q_METHOD(layer_normalized_forward), B200Q_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         B200Q_METHOD(layer_normalized_forward), B200Q_METHOD(rotary), B200Q_METHOD(cache_write), B200Q_METHOD(cache_read),
+                         B200Q_METHOD(cached_attention), B200Q_METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module{PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 } // namespace
 
@@ -322,5 +420,11 @@ PyMODINIT_FUNC PyInit__native() {
     name_group = PyUnicode_InternFromString("group_size");
     name_rotation = PyUnicode_InternFromString("rotation_size");
     name_c = PyUnicode_InternFromString("c");
+    name_keys = PyUnicode_InternFromString("keys");
+    name_key_scales = PyUnicode_InternFromString("key_scales");
+    name_value_scales = PyUnicode_InternFromString("value_scales");
+    name_turns = PyUnicode_InternFromString("turns");
+    name_interleaved = PyUnicode_InternFromString("interleaved");
+    name_scale = PyUnicode_InternFromString("scale");
     return PyModule_Create(&module);
 }

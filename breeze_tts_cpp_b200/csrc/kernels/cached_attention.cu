@@ -48,7 +48,7 @@ void launch_pass(AttentionArgs args, int most_columns, const CUtensorMap &keys, 
     using Shape = AttentionShape<HeadDim, Tiles>;
     // What the workers leave for the mergers, twice where that is small, and as many stages as the rest of the shared memory holds.
     args.merge_columns = std::min(Shape::columns, most_columns);
-    args.merge_buffers = args.merge_columns <= 8 ? 2 : 1;
+    args.merge_buffers = args.merge_columns <= 4 ? 2 : 1;
     const size_t merge = size_t(args.merge_buffers) * Shape::merge(args.merge_columns);
     args.stages = int(std::min<size_t>(kMaxRing, (kAttentionSmem - 1024 - merge) / Shape::stage));
     launch_pdl("cached attention", cached_attention<T, F, HeadDim, Tiles>, dim3(unsigned(ctas)), dim3(kAttentionThreads),
@@ -112,8 +112,8 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     args.page_shift = shift_of(p.cache.page_size), args.total_pages = p.cache.pages, args.offset_count = p.sequences;
     args.box_shift = std::min(args.page_shift, shift_of(kTileKeys));
     args.key_scales = p.cache.key_scales, args.value_scales = p.cache.value_scales;
-    const float format = p.cache.type == Type::FP8 ? 256.f : 1.f; // e4m3 bytes enter the products times 2^-8
-    args.score_scale = p.scale * 1.4426950408889634f * format;
+    const float format = p.cache.type == Type::FP8 ? 256.f : 1.f; // e4m3 values enter the second product times 2^-8
+    args.score_scale = p.scale * 1.4426950408889634f;
     args.output_scale = format;
     args.status = status;
 
@@ -143,7 +143,8 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
             combine.source[pass] = {args.partials, args.complete, args.table, ctas, narrow ? 8 : 16};
         }
         const long long warps = (long long)rows * heads;
-        launch_pdl("attention combine", combine_attention<T, decltype(width)::value>, dim3(unsigned((warps + 7) / 8)), dim3(256), 0, stream, combine);
+        launch_pdl("attention combine", combine_attention<T, decltype(width)::value>, dim3(unsigned((warps + kCombineThreads / 32 - 1) / (kCombineThreads / 32))),
+                   dim3(kCombineThreads), 0, stream, combine);
     });
 }
 } // namespace tts

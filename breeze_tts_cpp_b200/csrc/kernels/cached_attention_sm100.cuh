@@ -15,8 +15,8 @@
 //
 // Bound. A cached byte takes part in 2 x query rows multiply-adds and costs about 1.4 instructions of conversion; at two to eight rows per
 // head memory is the floor. One CTA per multiprocessor streams 128-token tiles (box copies by the tensor map, 128-byte swizzle, so that no
-// shared load has a bank conflict; the segment's query rows come with its first tiles) through a ring. Two groups of four warps take alternate
-// tiles, 32 keys a warp, so that a warp has two independent chains and its scheduler another warp; each warp keeps its own softmax state and output.
+// shared load has a bank conflict; the segment's query rows come with its first tiles) through a ring. Groups of four warps take the
+// tiles in turn, 32 keys a warp, so that a warp has two independent chains and its scheduler other warps; each warp keeps its own softmax state and output.
 // At a segment's end the warps leave theirs in shared memory and go on; two further warps add them up and store.
 //
 // Division. A segment is a sequence, a cached head and a tile of query rows. All CTAs get an equal run of the same list of tiles, whatever
@@ -30,9 +30,9 @@
 #include <cuda_fp16.h>
 
 namespace tts::b200 {
-constexpr int kTileKeys = 128, kWorkers = 8, kMergers = 2; // workers: two groups of four warps
-constexpr int kProducer = kWorkers, kAttentionThreads = 32 * (kWorkers + 1 + kMergers);
-constexpr int kMaxRing = 12;
+constexpr int kTileKeys = 128, kTeam = 4, kTeams = 2, kWorkers = kTeam * kTeams, kProducers = 2, kMergers = 2, kMaxRing = 12;
+constexpr int kAttentionWarps = kWorkers + kProducers + kMergers, kAttentionThreads = 32 * kAttentionWarps; // three per scheduler: 168 registers a thread
+constexpr int kScanAlone = 256; // up to here each producer warp adds the sequences' work up by itself
 constexpr int kPartialExtra = 4; // maximum and sum behind a partial row, padded to 16 bytes
 constexpr size_t kAttentionSmem = 224 * 1024;
 
@@ -81,6 +81,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+__device__ __forceinline__ void copy_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 // Untiled copy of a run of bytes (both ends and the size multiples of 16).
 __device__ __forceinline__ void copy_run(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
@@ -100,6 +103,12 @@ template <Type F> __device__ __forceinline__ void widen(uint32_t x, uint32_t &lo
         hi = (b & 0x80008000u) | ((b >> 1) & 0x3f803f80u);
     }
 }
+// The same for key bytes, e4m3 without a factor: a key that is not a number makes a score that is none, and hidden scores are replaced.
+template <Type F> __device__ __forceinline__ void widen_key(uint32_t x, uint32_t &lo, uint32_t &hi) {
+    if constexpr (F == Type::I8) widen<F>(x ^ 0x80808080u, lo, hi);
+    else
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(x));
+}
 template <Type F> __device__ __forceinline__ uint32_t biased(uint32_t x) { return F == Type::I8 ? x ^ 0x80808080u : x; }
 
 // Where a row's 16-byte piece lies in a tile as the tensor map's swizzle lays it down.
@@ -118,9 +127,9 @@ template <int HeadDim, int Tiles> struct AttentionShape {
 
 // What the producer tells the workers about a tile, and they the mergers about a segment's part.
 struct TileNote {
-    int key, head, row, count, flat, limit, flags, ordinal, first_cta, first_slot, slot, pad[5];
+    int key, head, row, count, flat, limit, flags, ordinal, first_cta, first_slot, slot, parts, first_team, pad[3];
 };
-constexpr int kNoteFirst = 1, kNoteFlush = 2, kNoteEnd = 4, kNoteAlone = 8, kNoteFinal = 16, kNoteSplit = 32, kNoteQuit = 64;
+constexpr int kNoteFirst = 1, kNoteFlush = 2, kNoteEnd = 4, kNoteFinal = 16, kNoteSplit = 32, kNoteQuit = 64;
 
 // A sequence as the tables give it, made safe: rows and positions stay inside of what the caller passed.
 struct SequenceShape {
@@ -152,20 +161,19 @@ template <int Columns> __device__ __forceinline__ int tiles_of(const AttentionAr
 template <int Columns> __device__ __forceinline__ int query_tiles(const AttentionArgs &a, const SequenceShape &s) {
     return (s.count * a.group + Columns - 1) / Columns;
 }
-// Tiles and segments of a sequence.
-struct Work {
-    long long tiles, segments;
-};
-template <int Columns> __device__ __forceinline__ Work work_of(const AttentionArgs &a, const SequenceShape &s) {
+// Tiles of one head of a sequence, over its query tiles.
+template <int Columns> __device__ __forceinline__ long long head_tiles(const AttentionArgs &a, const SequenceShape &s, int count) {
+    if (a.prefix) return (long long)count * tiles_of<Columns>(a, s, 0);
+    long long tiles = 0;
+    for (int qt = 0; qt < count; ++qt) tiles += tiles_of<Columns>(a, s, qt);
+    return tiles;
+}
+// Work of a run of sequences: tiles, and segments in the 24 high bits (the host refuses more), so that one scan adds up both.
+constexpr int kSegmentShift = 40;
+template <int Columns> __device__ __forceinline__ long long work_of(const AttentionArgs &a, int b) {
+    const SequenceShape s = sequence_of(a, b);
     const int count = query_tiles<Columns>(a, s);
-    Work w{0, (long long)count * a.kv_heads};
-    if (a.prefix) {
-        w.tiles = w.segments * tiles_of<Columns>(a, s, 0);
-    } else {
-        for (int qt = 0; qt < count; ++qt) w.tiles += tiles_of<Columns>(a, s, qt);
-        w.tiles *= a.kv_heads;
-    }
-    return w;
+    return a.kv_heads * (head_tiles<Columns>(a, s, count) + ((long long)count << kSegmentShift));
 }
 __device__ __forceinline__ long long scan_warp(long long v, int lane) { // inclusive
 #pragma unroll
@@ -174,6 +182,10 @@ __device__ __forceinline__ long long scan_warp(long long v, int lane) { // inclu
         if (lane >= d) v += other;
     }
     return v;
+}
+// 64-bit quotients take a hundred cycles, 32-bit ones a fifth; the operands are not negative.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)(uint32_t(a) / uint32_t(b));
 }
 // Shares are counted in units: kTileUnits for a tile, kSegmentUnits more for a segment (its queries, its flush and its merge). A tile belongs to the
 // CTA whose share holds its first unit.
@@ -199,12 +211,11 @@ template <class T, Type F, int HeadDim, int Tiles>
 __global__ void __launch_bounds__(kAttentionThreads, 1)
     cached_attention(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const AttentionArgs args) {
     using Shape = AttentionShape<HeadDim, Tiles>;
-    constexpr int kColumns = Shape::columns, kSteps = HeadDim / 16, kWarps = kAttentionThreads / 32;
+    constexpr int kColumns = Shape::columns, kSteps = HeadDim / 16, kProducer = kWorkers, kMerger = kProducer + kProducers;
     extern __shared__ uint8_t raw_smem[];
-    __shared__ uint64_t full[2][kMaxRing], empty[kMaxRing], merge_full[2]; // full: of each group
+    __shared__ uint64_t full[kTeams][kMaxRing], empty[kMaxRing], merge_full[2]; // full: of each team
     __shared__ TileNote notes[kMaxRing], merge_notes[2];
-    __shared__ long long tile_sums[kWarps], segment_sums[kWarps];
-    __shared__ long long found[2]; // sequence of this CTA's first unit, its own first unit
+    __shared__ long long sums[kAttentionWarps], found[3]; // found: sequence of this CTA's first unit, the sequence's first unit, all work
     __shared__ int abort_flag;
     __shared__ int merged; // parts that the mergers are done with, times kMergers
     const uint32_t ring = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;
@@ -214,10 +225,9 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     const int warp = ptx::warp_index(), lane = threadIdx.x & 31;
 
     if (!threadIdx.x) {
-        for (int s = 0; s < kMaxRing; ++s) {
-            ptx::mbar_init(ptx::smem_u32(&full[0][s]), 1);
-            ptx::mbar_init(ptx::smem_u32(&full[1][s]), 1);
-            ptx::mbar_init(ptx::smem_u32(&empty[s]), kWorkers / 2);
+        for (int s = 0; s < stages; ++s) {
+            for (int team = 0; team < kTeams; ++team) ptx::mbar_init(ptx::smem_u32(&full[team][s]), 33); // the leading producer's, and a lane's scales each
+            ptx::mbar_init(ptx::smem_u32(&empty[s]), kTeam);
         }
         for (int b = 0; b < 2; ++b) ptx::mbar_init(ptx::smem_u32(&merge_full[b]), kWorkers);
         abort_flag = merged = 0;
@@ -226,43 +236,49 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         ptx::prefetch_tensormap(&value_map);
     }
     pdl_launch_dependents();
-    pdl_wait_upstream();
-
-    // Every CTA adds up all sequences' tiles: a thread takes a run of sequences, then a scan over the threads.
-    const int run = (args.sequences + kAttentionThreads - 1) / kAttentionThreads;
-    const int from = min(args.sequences, int(threadIdx.x) * run), to = min(args.sequences, from + run);
-    Work own{0, 0};
-    for (int b = from; b < to; ++b) {
-        const Work w = work_of<kColumns>(args, sequence_of(args, b));
-        own.tiles += w.tiles, own.segments += w.segments;
-    }
-    Work before{scan_warp(own.tiles, lane), scan_warp(own.segments, lane)};
-    if (lane == 31) tile_sums[warp] = before.tiles, segment_sums[warp] = before.segments;
     __syncthreads();
-    Work all{0, 0};
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before.tiles += tile_sums[w], before.segments += segment_sums[w];
-        all.tiles += tile_sums[w], all.segments += segment_sums[w];
-    }
-    // Where there is a CTA for every tile, each gets one. A share is never smaller than a tile, so that every CTA between a segment's first
-    // and its last has a part of it.
-    const long long ctas = all.tiles < gridDim.x ? all.tiles : gridDim.x;
-    if (blockIdx.x >= ctas) return;
-    const int extra = all.tiles > gridDim.x ? kSegmentUnits : 0;
-    auto units = [&](const Work &w) { return kTileUnits * w.tiles + extra * w.segments; };
-    const long long total = units(all), begin = total * blockIdx.x / ctas, end = total * (blockIdx.x + 1) / ctas;
-    before.tiles -= own.tiles, before.segments -= own.segments;
-    if (long long at = units(before); at <= begin && begin < at + units(own)) {
+
+    // The producers need the work of all sequences, and where their CTA's share lies among them: a lane takes a run of sequences, then a scan over
+    // the lanes. For a long batch all threads do.
+    auto spread = [&](int threads, int thread, long long base, long long own, long long all, auto &&keep) {
+        const long long tiles = all & ((1ll << kSegmentShift) - 1), ctas = tiles < gridDim.x ? tiles : gridDim.x;
+        if (blockIdx.x >= ctas) return;
+        const int extra = tiles > gridDim.x ? kSegmentUnits : 0;
+        auto units = [&](long long work) { return kTileUnits * (work & ((1ll << kSegmentShift) - 1)) + extra * (work >> kSegmentShift); };
+        const long long total = units(all), each = quotient(total, ctas), rest = total - each * ctas;
+        const long long begin = each * blockIdx.x + min((long long)blockIdx.x, rest);
+        long long at = units(base);
+        if (at > begin || begin >= at + units(own)) return;
+        const int run = (args.sequences + threads - 1) / threads, from = thread * run, to = min(args.sequences, from + run);
         for (int b = from; b < to; ++b) {
-            const long long part = units(work_of<kColumns>(args, sequence_of(args, b)));
+            const long long part = units(work_of<kColumns>(args, b));
             if (begin < at + part) {
-                found[0] = b, found[1] = at;
+                keep(b, at);
                 break;
             }
             at += part;
         }
+    };
+    auto work_of_run = [&](int threads, int thread) {
+        const int run = (args.sequences + threads - 1) / threads, from = min(args.sequences, thread * run), to = min(args.sequences, from + run);
+        long long own = 0;
+        for (int b = from; b < to; ++b) own += work_of<kColumns>(args, b);
+        return own;
+    };
+    if (args.sequences > kScanAlone) {
+        pdl_wait_upstream();
+        const long long own = work_of_run(kAttentionThreads, int(threadIdx.x));
+        long long before = scan_warp(own, lane), all = 0;
+        if (lane == 31) sums[warp] = before;
+        __syncthreads();
+        for (int w = 0; w < kAttentionWarps; ++w) {
+            if (w < warp) before += sums[w];
+            all += sums[w];
+        }
+        if (!threadIdx.x) found[2] = all;
+        spread(kAttentionThreads, int(threadIdx.x), before - own, own, all, [&](int b, long long at) { found[0] = b, found[1] = at; });
+        __syncthreads();
     }
-    __syncthreads();
     // Every wait is bounded, and a warp whose wait gave up leaves as one; the others follow when theirs do.
     auto wait = [&](uint64_t &bar, uint32_t parity) {
         if (__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar), parity, &abort_flag))) return true;
@@ -281,28 +297,57 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         return reached;
     };
 
-    // Tile i of the share goes to group i % 2 and stage i % stages. A stage may serve both groups in turn, so each group has its own barriers: waiting
-    // on a common one, a group could be two phases off. A group comes back to a stage after `period` of its tiles.
-    const int period = stages & 1 ? stages : stages / 2;
+    // Tile i of the share goes to team i % kTeams and stage i % stages. A stage may serve the teams in turn, so each team has its own barriers: waiting
+    // on a common one, a team could be two phases off. A team comes back to a stage after `period` of its tiles.
+    const int period = stages % kTeams ? stages : stages / kTeams;
 
-    if (warp == kProducer) { // ------------------------------------------------------------------ producer
-        int stage = 0, issued = 0, ordinal = 0, b = int(found[0]);
+    if (warp >= kProducer && warp < kMerger) { // --------------------------------------------------- producers
+        // Two warps walk the same list: one copies keys and queries and writes the notes, the other copies values and scales. A tensor copy costs its
+        // issuer 50 to 100 cycles and a tile of 16-token pages takes sixteen of them, so one warp would be what the ring waits for.
+        const bool leads = warp == kProducer;
+        int stage = 0, issued = 0, ordinal = 0, b = 0, team = 0;
         uint32_t phase = 0;
-        long long at = found[1]; // first unit of the segment
+        long long at = 0, all; // at: first unit of the segment
+        if (args.sequences > kScanAlone) {
+            b = int(found[0]), at = found[1], all = found[2];
+        } else {
+            pdl_wait_upstream();
+            const long long own = work_of_run(32, lane), through = scan_warp(own, lane);
+            all = __shfl_sync(0xffffffffu, through, 31);
+            bool here = false;
+            spread(32, lane, through - own, own, all, [&](int sequence, long long unit) { here = true, b = sequence, at = unit; });
+            if (const unsigned who = __ballot_sync(0xffffffffu, here)) {
+                b = __shfl_sync(0xffffffffu, b, __ffs(who) - 1);
+                at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1);
+            }
+        }
+        // Where there is a CTA for every tile, each gets one. A share is never smaller than a tile, so that every CTA between a segment's first
+        // and its last has a part of it.
+        const long long all_tiles = all & ((1ll << kSegmentShift) - 1), ctas = all_tiles < gridDim.x ? all_tiles : gridDim.x;
+        const int extra = all_tiles > gridDim.x ? kSegmentUnits : 0;
+        const long long total = kTileUnits * all_tiles + extra * (all >> kSegmentShift), each = ctas ? quotient(total, ctas) : 0, rest = total - each * ctas;
+        auto share_of = [&](long long cta) { return each * cta + min(cta, rest); }; // its first unit
+        const long long begin = share_of(min((long long)blockIdx.x, ctas)), end = share_of(min((long long)blockIdx.x + 1, ctas));
         const int box = 1 << args.box_shift, boxes = kTileKeys >> args.box_shift;
-        const uint32_t box_bytes = uint32_t(box) * (2 * HeadDim + 8);
-        const int mine = lane >> 2, kind = lane & 3; // lane 4i + k copies part k (keys, values, their scales) of box i
+        const uint32_t box_bytes = uint32_t(box) * 2 * HeadDim;
+        if (begin >= end) b = args.sequences; // nothing to do here
         bool open = true;
         for (; open && b < args.sequences && at < end; ++b) {
             const SequenceShape s = sequence_of(args, b);
             const int query_count = query_tiles<kColumns>(args, s);
             const int *pages = args.pages + size_t(b) * args.page_stride;
+            // Lane i's page of a tile: its box i. Always a load, of the last page where there is none, so that nothing waits for it here.
             auto page_at = [&](int tile) {
-                const int position = tile * kTileKeys + (mine << args.box_shift);
-                return mine < boxes && position < s.length ? load_index(pages + (position >> args.page_shift)) : -1;
+                return load_index(pages + (max(0, min(tile * kTileKeys + (min(lane, boxes - 1) << args.box_shift), s.length - 1)) >> args.page_shift));
             };
+            int segment = 0;
+            if (begin > at) { // whole heads in front of the share
+                const long long head_units = kTileUnits * head_tiles<kColumns>(args, s, query_count) + (long long)extra * query_count;
+                const long long heads = head_units ? min(quotient(begin - at, head_units), (long long)args.kv_heads) : 0;
+                segment = int(heads) * query_count, at += heads * head_units;
+            }
             // Heads outermost: their query tiles read the same keys, near one another in time.
-            for (int segment = 0; open && segment < query_count * args.kv_heads && at < end; ++segment) {
+            for (; open && segment < query_count * args.kv_heads && at < end; ++segment) {
                 const int head = segment / query_count, qt = segment - head * query_count, tiles = tiles_of<kColumns>(args, s, qt);
                 const long long first_unit = at + extra;
                 at = first_unit + (long long)kTileUnits * tiles;
@@ -314,9 +359,9 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                 int first_cta = -1, first_slot = 0;
                 const bool split = low || high < tiles;
                 if (split && high == tiles) { // this CTA closes the segment: it says where its parts lie
-                    first_cta = int(first_unit * ctas / total);
-                    while (total * (first_cta + 1) / ctas <= first_unit) ++first_cta;
-                    first_slot = total * first_cta / ctas < first_unit - extra ? 1 : 0;
+                    const long long larger = rest * (each + 1); // units of the shares that have one more
+                    first_cta = int(first_unit < larger ? quotient(first_unit, each + 1) : rest + quotient(first_unit - larger, each));
+                    first_slot = share_of(first_cta) < first_unit - extra ? 1 : 0;
                 }
                 const int columns = min(kColumns, s.count * args.group - qt * kColumns);
                 int next = page_at(low);
@@ -327,72 +372,100 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                         open = false;
                         break;
                     }
-                    const uint32_t to = ring + stage * Shape::stage, bar = ptx::smem_u32(&full[issued & 1][stage]);
+                    const uint32_t to = ring + stage * Shape::stage, bar = ptx::smem_u32(&full[team][stage]);
                     uint8_t *const bytes = ring_bytes + stage * Shape::stage;
-                    const int position = tile * kTileKeys + (mine << args.box_shift), offset = mine << args.box_shift;
-                    const bool wanted = mine < boxes && position < s.length, good = wanted && unsigned(page) < unsigned(args.total_pages);
-                    // Positions on a page that the cache does not have read as NaN.
-                    if (wanted && !good && kind >= 2)
-                        for (int i = 0; i < box; ++i)
-                            reinterpret_cast<float *>(bytes + Shape::scales)[(kind - 2) * kTileKeys + offset + i] = __int_as_float(0x7fffffff);
-                    // Each group's first tile of the part brings the query rows.
-                    const bool first = tile - low < 2;
-                    const int flat = qt * kColumns + lane;
-                    const T *query = static_cast<const T *>(args.queries) + size_t(s.row + flat / args.group) * args.query_stride +
-                                     (head * args.group + flat % args.group) * HeadDim;
-                    if (first && !args.aligned && lane < columns)
-                        for (int d = 0; d < HeadDim; ++d) {
-                            uint16_t v;
-                            asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(query + d) : "memory");
-                            *reinterpret_cast<uint16_t *>(bytes + Shape::queries + lane * Shape::query_row + 2 * d) = v;
+                    const int key = tile * kTileKeys, position = key + (lane << args.box_shift);
+                    const bool good = lane < boxes && position < s.length && unsigned(page) < unsigned(args.total_pages);
+                    const uint32_t held = __ballot_sync(0xffffffffu, good);
+                    const int row = (((page * args.kv_heads) + head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
+                    if (leads) {
+                        // Each team's first tile of the part brings the query rows.
+                        const bool first = tile - low < kTeams, flush = tile + kTeams >= high;
+                        const T *query = nullptr;
+                        uint32_t query_bytes = 0;
+                        if (first) {
+                            const int flat = qt * kColumns + lane;
+                            query = static_cast<const T *>(args.queries) + size_t(s.row + flat / args.group) * args.query_stride +
+                                    (head * args.group + flat % args.group) * HeadDim;
+                            if (args.aligned) query_bytes = uint32_t(columns) * HeadDim * 2;
+                            else if (lane < columns)
+                                for (int d = 0; d < HeadDim; ++d) {
+                                    uint16_t v;
+                                    asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(query + d) : "memory");
+                                    *reinterpret_cast<uint16_t *>(bytes + Shape::queries + lane * Shape::query_row + 2 * d) = v;
+                                }
+                            __syncwarp();
                         }
-                    const bool query_copy = first && args.aligned && lane < columns;
-                    __syncwarp();
-                    const uint32_t copied = __popc(__ballot_sync(0xffffffffu, good)) / 4, rows = __popc(__ballot_sync(0xffffffffu, query_copy));
-                    if (!lane) {
-                        TileNote &n = notes[stage];
-                        n.key = tile * kTileKeys, n.head = head, n.row = s.row, n.count = s.count, n.flat = qt * kColumns;
-                        n.limit = args.prefix ? s.length - 1 : s.length - s.count;
-                        n.flags = (first ? kNoteFirst : 0) | (tile + 2 >= high ? kNoteFlush : 0) | (tile + 1 == high ? kNoteEnd : 0) |
-                                  (high - low == 1 ? kNoteAlone : 0) | (high < tiles || at + extra >= end ? kNoteFinal : 0) | (split ? kNoteSplit : 0);
-                        n.ordinal = ordinal, n.first_cta = first_cta, n.first_slot = first_slot;
-                        n.slot = first_unit - extra > begin ? 1 : 0;
-                        ptx::mbar_arrive_expect_tx(bar, copied * box_bytes + rows * HeadDim * 2);
+                        if (!lane) {
+                            TileNote &n = notes[stage];
+                            n.key = key;
+                            n.flags = (first ? kNoteFirst : 0) | (flush ? kNoteFlush : 0) | (tile + 1 == high ? kNoteEnd : 0) |
+                                      (high < tiles || at + extra >= end ? kNoteFinal : 0) | (split ? kNoteSplit : 0);
+                            if (first || flush) { // what the workers read at a part's ends only
+                                n.head = head, n.row = s.row, n.count = s.count, n.flat = qt * kColumns;
+                                n.limit = args.prefix ? s.length - 1 : s.length - s.count;
+                                n.ordinal = ordinal, n.first_cta = first_cta, n.first_slot = first_slot;
+                                n.slot = first_unit - extra > begin ? 1 : 0;
+                                n.parts = min(kTeams, high - low), n.first_team = (issued - (tile - low)) % kTeams;
+                            }
+                            ptx::mbar_arrive_expect_tx(bar, __popc(held) * box_bytes + query_bytes);
+                        }
+                        __syncwarp();
+                        if (query_bytes && lane < columns) copy_run(to + Shape::queries + lane * Shape::query_row, query, HeadDim * 2, bar);
+                    } else {
+                        // Scales: a lane copies four of the keys' and four of the values'. Positions on a page that the cache does not have read as NaN.
+                        const int owner = (4 * lane) >> args.box_shift;
+                        const int its_row = __shfl_sync(0xffffffffu, row, owner) + ((4 * lane) & (box - 1));
+                        if (held >> owner & 1) {
+                            const uint32_t scales = to + Shape::scales + 16 * lane;
+                            copy_async16(scales, args.key_scales + its_row);
+                            copy_async16(scales + kTileKeys * 4, args.value_scales + its_row);
+                            ptx::copy_async_arrive(bar);
+                        } else {
+                            const float nan = __int_as_float(0x7fffffff);
+                            *reinterpret_cast<float4 *>(bytes + Shape::scales + 16 * lane) = make_float4(nan, nan, nan, nan);
+                            *reinterpret_cast<float4 *>(bytes + Shape::scales + kTileKeys * 4 + 16 * lane) = make_float4(nan, nan, nan, nan);
+                            ptx::mbar_arrive(bar);
+                        }
+                    }
+                    // One thread issues the boxes, from rows gathered beforehand.
+                    int from_row[kTileKeys / 16];
+#pragma unroll
+                    for (int i = 0; i < kTileKeys / 16; ++i) from_row[i] = __shfl_sync(0xffffffffu, row, i);
+                    if (ptx::elect_one()) {
+                        const CUtensorMap *map = leads ? &key_map : &value_map;
+                        const uint32_t into = to + (leads ? 0u : Shape::values), box_size = uint32_t(box) * HeadDim;
+#pragma unroll
+                        for (int i = 0; i < kTileKeys / 16; ++i)
+                            if (held >> i & 1) ptx::tma_load_2d(into + i * box_size, map, bar, 0, from_row[i]);
                     }
                     __syncwarp();
-                    if (query_copy) copy_run(to + Shape::queries + lane * Shape::query_row, query, HeadDim * 2, bar);
-                    if (good) {
-                        const int row = (((page * args.kv_heads) + head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
-                        if (kind == 0) ptx::tma_load_2d(to + offset * HeadDim, &key_map, bar, 0, row);
-                        else if (kind == 1) ptx::tma_load_2d(to + Shape::values + offset * HeadDim, &value_map, bar, 0, row);
-                        else copy_run(to + Shape::scales + ((kind - 2) * kTileKeys + offset) * 4, (kind == 2 ? args.key_scales : args.value_scales) + row, uint32_t(box) * 4, bar);
-                    }
                     ++issued;
                     if (++stage == stages) stage = 0, phase ^= 1;
+                    if (++team == kTeams) team = 0;
                 }
                 ++ordinal;
             }
         }
-        for (int team = 0; team < 2 && open; ++team) { // an empty stage ends each group
+        for (int i = 0; i < kTeams && open; ++i) { // an empty stage ends each team
             if (issued >= stages && !wait(empty[stage], phase ^ 1)) break;
-            if (!lane) {
-                notes[stage].flags = kNoteQuit;
-                ptx::mbar_arrive(ptx::smem_u32(&full[issued & 1][stage]));
-            }
+            if (leads && !lane) notes[stage].flags = kNoteQuit;
+            if (!leads || !lane) ptx::mbar_arrive(ptx::smem_u32(&full[team][stage]));
             ++issued;
             if (++stage == stages) stage = 0, phase ^= 1;
+            if (++team == kTeams) team = 0;
         }
-        if (!ordinal && !lane) { // a share that holds no tile's first unit
+        if (!ordinal && leads && !lane) { // a share that holds no tile's first unit
             merge_notes[0].flags = kNoteQuit;
             for (int w = 0; w < kWorkers; ++w) ptx::mbar_arrive(ptx::smem_u32(&merge_full[0]));
         }
         // No copy may be in flight when the CTA leaves, whatever the workers did.
         int ignored = 0;
-        for (int i = max(0, issued - stages); i < issued; ++i) ptx::mbar_wait(ptx::smem_u32(&full[i & 1][i % stages]), uint32_t((i >> 1) / period) & 1, &ignored);
+        for (int i = max(0, issued - stages); i < issued; ++i) ptx::mbar_wait(ptx::smem_u32(&full[i % kTeams][i % stages]), uint32_t((i / kTeams) / period) & 1, &ignored);
         return;
     }
 
-    if (warp > kProducer) { // -------------------------------------------------------------------- mergers
+    if (warp >= kMerger) { // ---------------------------------------------------------------------- mergers
         for (int ordinal = 0;; ++ordinal) {
             const int buffer = ordinal % args.merge_buffers;
             if (!wait(merge_full[buffer], uint32_t(ordinal / args.merge_buffers) & 1)) return;
@@ -400,16 +473,19 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
             if (note.flags & kNoteQuit) return;
             const float *shares = merge + buffer * merge_floats;
             const int columns = min(kColumns, note.count * args.group - note.flat), flags = note.flags;
-            const int low = flags & kNoteAlone ? note.pad[0] * (kWorkers / 2) : 0, high = flags & kNoteAlone ? low + kWorkers / 2 : kWorkers;
-            for (int item = threadIdx.x - 32 * (kProducer + 1); item < columns * (HeadDim / 4); item += 32 * kMergers) {
+            const int count = kTeam * note.parts; // shares
+            for (int item = int(threadIdx.x) - 32 * kMerger; item < columns * (HeadDim / 4); item += 32 * kMergers) {
                 const int column = item / (HeadDim / 4), d = 4 * (item % (HeadDim / 4));
                 float highest = -INFINITY;
-                for (int w = low; w < high; ++w) highest = fmaxf(highest, shares[(w * args.merge_columns + column) * Shape::row + HeadDim]);
+#pragma unroll
+                for (int w = 0; w < kWorkers; ++w)
+                    if (w < count) highest = fmaxf(highest, shares[(w * args.merge_columns + column) * Shape::row + HeadDim]);
                 const float reference = highest == -INFINITY ? 0.f : highest;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                 float l = 0.f;
-#pragma unroll 4
-                for (int w = low; w < high; ++w) {
+#pragma unroll
+                for (int w = 0; w < kWorkers; ++w) {
+                    if (w >= count) break;
                     const float *from = shares + (w * args.merge_columns + column) * Shape::row;
                     const float f = exp2_approx(from[HeadDim] - reference);
                     const float4 x = *reinterpret_cast<const float4 *>(from + d);
@@ -443,7 +519,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     }
 
     // --------------------------------------------------------------------------------------------- workers
-    const int g = lane >> 2, t = lane & 3, team = warp >> 2, row = 32 * (warp & 3);
+    const int g = lane >> 2, t = lane & 3, team = warp / kTeam, row = 32 * (warp % kTeam);
     uint32_t q[Tiles][kSteps][2];
     float out[Tiles][kSteps][4], most[Tiles][2], sum[Tiles][2], factor[Tiles][2];
     int limit[Tiles][2], least = 0;
@@ -503,38 +579,70 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
             least = __reduce_min_sync(0xffffffffu, least);
         }
 
-        // Scores of this warp's 32 keys, two blocks of 16.
-        float scores[Tiles][2][4] = {};
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            uint32_t keys[2][HeadDim / 16];
+        // This warp's 32 keys, two blocks of 16: all of its bytes into registers, so that the stage can be filled again while the warp computes
+        // (the ring, not the arithmetic, is what bounds a long context). Not with 16 query rows, whose state needs the registers.
+        constexpr bool kEarly = Tiles == 1;
+        uint32_t keys[2][2][HeadDim / 16], values[2][4][HeadDim / 32];
+        float key_scale[2][2], value_scale[2][2], shift[2][2];
+        auto load_keys = [&](int m) {
 #pragma unroll
             for (int r = 0; r < 2; ++r)
 #pragma unroll
                 for (int c = 0; c < HeadDim / 64; ++c)
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(keys[r][4 * c]), "=r"(keys[r][4 * c + 1]), "=r"(keys[r][4 * c + 2]), "=r"(keys[r][4 * c + 3])
+                                 : "=r"(keys[m][r][4 * c]), "=r"(keys[m][r][4 * c + 1]), "=r"(keys[m][r][4 * c + 2]), "=r"(keys[m][r][4 * c + 3])
                                  : "r"(at + piece<HeadDim>(row + 16 * m + g + 8 * r, HeadDim / 64 * t + c)));
+        };
+        // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9 of the block: this thread's 16 (8) columns.
+        auto load_values = [&](int m) {
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                uint32_t a[4];
-                widen<F>(biased<F>(keys[0][k]), a[0], a[2]);
-                widen<F>(biased<F>(keys[1][k]), a[1], a[3]);
-#pragma unroll
-                for (int n = 0; n < Tiles; ++n) mma_f16(scores[n][m], a[0], a[1], a[2], a[3], q[n][k][0], q[n][k][1]);
+            for (int r = 0; r < 4; ++r) {
+                const int key = row + 16 * m + 2 * t + (r & 1) + 8 * (r >> 1);
+                if constexpr (HeadDim == 128)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(values[m][r][0]), "=r"(values[m][r][1]), "=r"(values[m][r][2]), "=r"(values[m][r][3])
+                                 : "r"(at + Shape::values + piece<HeadDim>(key, g)));
+                else
+                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                                 : "=r"(values[m][r][0]), "=r"(values[m][r][1])
+                                 : "r"(at + Shape::values + piece<HeadDim>(key, g >> 1) + 8 * (g & 1)));
             }
-        }
-        float key_scale[2][2], value_scale[2][2], shift[2][2];
+        };
+        const int first_key = note.key;
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < 2; ++m) {
+            if (kEarly) load_keys(m);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 key_scale[m][r] = scales[row + 16 * m + g + 8 * r];
                 value_scale[m][r] = scales[kTileKeys + row + 16 * m + g + 8 * r];
-                shift[m][r] = fmaxf(log2_approx(fabsf(value_scale[m][r])), -126.f);
             }
-        const int position = note.key + row + g;
-        const bool masked = note.key + kTileKeys - 1 > least;
+        }
+        if (kEarly) {
+            load_values(0);
+            load_values(1);
+            if (!(flags & kNoteFlush)) { // a flush still needs the note
+                __syncwarp();
+                if (!lane) ptx::mbar_arrive(ptx::smem_u32(&empty[stage]));
+            }
+        }
+        float scores[Tiles][2][4] = {};
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            if (!kEarly) load_keys(m);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                uint32_t a[4];
+                widen_key<F>(keys[m][0][k], a[0], a[2]);
+                widen_key<F>(keys[m][1][k], a[1], a[3]);
+#pragma unroll
+                for (int n = 0; n < Tiles; ++n) mma_f16(scores[n][m], a[0], a[1], a[2], a[3], q[n][k][0], q[n][k][1]);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) shift[m][r] = fmaxf(log2_approx(fabsf(value_scale[m][r])), -126.f);
+        }
+        const int position = first_key + row + g;
+        const bool masked = first_key + kTileKeys - 1 > least;
         uint32_t weights[Tiles][2][2];
 #pragma unroll
         for (int n = 0; n < Tiles; ++n) {
@@ -590,26 +698,13 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            // Values of keys 2t, 2t + 1, 2t + 8, 2t + 9 of the block: this thread's 16 (8) columns.
-            uint32_t values[4][HeadDim / 32];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int key = row + 16 * m + 2 * t + (r & 1) + 8 * (r >> 1);
-                if constexpr (HeadDim == 128)
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(values[r][0]), "=r"(values[r][1]), "=r"(values[r][2]), "=r"(values[r][3])
-                                 : "r"(at + Shape::values + piece<HeadDim>(key, g)));
-                else
-                    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
-                                 : "=r"(values[r][0]), "=r"(values[r][1])
-                                 : "r"(at + Shape::values + piece<HeadDim>(key, g >> 1) + 8 * (g & 1)));
-            }
+            if (!kEarly) load_values(m);
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) {
                 const uint32_t order = k & 1 ? 0x7362u : 0x5140u; // bytes 2 (k & 1) and the next of two keys, side by side
                 uint32_t a[4];
-                widen<F>(biased<F>(__byte_perm(values[0][k >> 1], values[1][k >> 1], order)), a[0], a[1]);
-                widen<F>(biased<F>(__byte_perm(values[2][k >> 1], values[3][k >> 1], order)), a[2], a[3]);
+                widen<F>(biased<F>(__byte_perm(values[m][0][k >> 1], values[m][1][k >> 1], order)), a[0], a[1]);
+                widen<F>(biased<F>(__byte_perm(values[m][2][k >> 1], values[m][3][k >> 1], order)), a[2], a[3]);
 #pragma unroll
                 for (int n = 0; n < Tiles; ++n) mma_f16(out[n][k], a[0], a[1], a[2], a[3], weights[n][m][0], weights[n][m][1]);
             }
@@ -620,7 +715,8 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
             const int columns = min(kColumns, note.count * args.group - note.flat);
             // A count and not a barrier's phase: a group has no tile in some parts, and could be two phases off.
             if (ordinal >= args.merge_buffers && !wait_merged(kMergers * (ordinal - args.merge_buffers + 1))) return;
-            float *const shares = merge + buffer * merge_floats + warp * args.merge_columns * Shape::row;
+            const int share = (team - note.first_team + kTeams) % kTeams * kTeam + warp % kTeam;
+            float *const shares = merge + buffer * merge_floats + share * args.merge_columns * Shape::row;
 #pragma unroll
             for (int n = 0; n < Tiles; ++n)
 #pragma unroll
@@ -637,19 +733,19 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                             make_float4(out[n][k][c], out[n][k][2 + c], out[n][k + 1][c], out[n][k + 1][2 + c]);
                     if (!g) to[HeadDim] = most[n][c], to[HeadDim + 1] = l;
                 }
-            if ((flags & kNoteEnd) && !(warp & 3) && !lane) {
-                merge_notes[buffer] = note;
-                merge_notes[buffer].pad[0] = team;
-            }
+            if ((flags & kNoteEnd) && !(warp % kTeam) && !lane) merge_notes[buffer] = note;
             __syncwarp();
-            if (!lane) {
+            if (!lane) { // the team of the last tile also arrives for those that have none of this part
                 ptx::mbar_arrive(ptx::smem_u32(&merge_full[buffer]));
-                if (flags & kNoteAlone) ptx::mbar_arrive(ptx::smem_u32(&merge_full[buffer])); // for the group that has no tile of this part
+                if (flags & kNoteEnd)
+                    for (int i = note.parts; i < kTeams; ++i) ptx::mbar_arrive(ptx::smem_u32(&merge_full[buffer]));
             }
         }
-        __syncwarp();
-        if (!lane) ptx::mbar_arrive(ptx::smem_u32(&empty[stage]));
-        stage += 2;
+        if (!kEarly || (flags & kNoteFlush)) {
+            __syncwarp();
+            if (!lane) ptx::mbar_arrive(ptx::smem_u32(&empty[stage]));
+        }
+        stage += kTeams;
         if (stage >= stages) stage -= stages;
         if (++seen_stages == period) seen_stages = 0, phase ^= 1;
     }
@@ -670,35 +766,76 @@ struct CombineArgs {
     void *output;
     float output_scale;
 };
-template <class T, int HeadDim> __global__ void __launch_bounds__(256) combine_attention(const CombineArgs args) {
+constexpr int kCombineThreads = 128;
+template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThreads) combine_attention(const CombineArgs args) {
     constexpr int kRow = HeadDim + kPartialExtra, kShare = HeadDim / 32;
     pdl_launch_dependents();
     pdl_wait_upstream();
     const int lane = threadIdx.x & 31;
-    const long long index = (long long)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+    const long long index = (long long)blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5);
     const int rows = args.row_count ? min(args.rows, load_index(args.row_count)) : args.rows;
     if (index >= (long long)rows * args.heads) return;
     float highest = -INFINITY, l = 0.f, v[kShare] = {};
     bool written = args.sources == 1;
-    for (int i = 0; i < args.sources; ++i) {
+    int4 entries[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (i < args.sources)
+            asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(entries[i].x), "=r"(entries[i].y), "=r"(entries[i].z), "=r"(entries[i].w)
+                         : "l"(args.source[i].table + index)
+                         : "memory");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (i >= args.sources) break;
         const CombineSource &s = args.source[i];
-        int4 entry;
-        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(entry.x), "=r"(entry.y), "=r"(entry.z), "=r"(entry.w) : "l"(s.table + index) : "memory");
+        const int4 entry = entries[i];
         const bool whole = entry.y <= 0;
         if (whole && !s.complete) continue;
         // Rows that no sequence covers have no entry: whatever stands there stays inside the workspace.
         if (!whole && (entry.x < 0 || entry.y > s.ctas - entry.x || unsigned(entry.z) > 1u || unsigned(entry.w) >= unsigned(s.columns))) continue;
         written = false;
         const int parts = whole ? 1 : entry.y;
-        for (int part = 0; part < parts; ++part) {
-            const float *from = whole ? s.complete + size_t(index) * kRow
-                                      : s.partials + (size_t((entry.x + part) * 2 + (part ? 0 : entry.z)) * s.columns + entry.w) * kRow;
-            const float other = from[HeadDim], raised = fmaxf(highest, other), reference = raised == -INFINITY ? 0.f : raised;
-            const float a = exp2_approx(highest - reference), b = exp2_approx(other - reference);
+        auto part_of = [&](int part) {
+            return whole ? s.complete + size_t(index) * kRow
+                         : s.partials + (size_t((entry.x + part) * 2 + (part ? 0 : entry.z)) * s.columns + entry.w) * kRow;
+        };
+        // 32 parts at a time: a lane reads the maximum and the sum of one, so that the rows' loads depend on nothing but the loop.
+        for (int first = 0; first < parts; first += 32) {
+            const int count = min(32, parts - first);
+            float most = -INFINITY, sum = 0.f;
+            if (lane < count) {
+                const float2 stats = *reinterpret_cast<const float2 *>(part_of(first + lane) + HeadDim);
+                most = stats.x, sum = stats.y;
+            }
+            float raised = most;
 #pragma unroll
-            for (int c = 0; c < kShare; ++c) v[c] = v[c] * a + from[kShare * lane + c] * b;
-            l = l * a + from[HeadDim + 1] * b;
+            for (int d = 16; d; d >>= 1) raised = fmaxf(raised, __shfl_xor_sync(0xffffffffu, raised, d));
+            raised = fmaxf(raised, highest);
+            const float reference = raised == -INFINITY ? 0.f : raised, shrink = exp2_approx(highest - reference);
+            const float factor = exp2_approx(most - reference);
+            sum *= factor;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            l = l * shrink + sum; // the same in all lanes
+#pragma unroll
+            for (int c = 0; c < kShare; ++c) v[c] *= shrink;
             highest = raised;
+#pragma unroll 8
+            for (int part = 0; part < count; ++part) {
+                const float *from = part_of(first + part) + kShare * lane;
+                const float f = __shfl_sync(0xffffffffu, factor, part);
+                float x[kShare];
+                if constexpr (kShare == 4) {
+                    const float4 w = *reinterpret_cast<const float4 *>(from);
+                    x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+                } else {
+                    const float2 w = *reinterpret_cast<const float2 *>(from);
+                    x[0] = w.x, x[1] = w.y;
+                }
+#pragma unroll
+                for (int c = 0; c < kShare; ++c) v[c] += x[c] * f;
+            }
         }
     }
     if (written) return;

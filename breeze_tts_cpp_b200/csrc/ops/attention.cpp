@@ -169,6 +169,9 @@ void validate_cached_attention(const CacheView &cache, const Attention &a) {
             refuse("prefix pages must be int32 [1, pages]");
         check_index(a.prefix_length, 1, "the prefix length is one int32");
     }
+    // Segments (a sequence, a cached head, a tile of at least eight query rows) are counted in 24 bits on the device.
+    const int64_t group = heads / cache.kv_heads, segments = (int64_t(a.queries.rows) * group / 8 + std::max(a.pages.rows, 1)) * cache.kv_heads;
+    if (segments >= int64_t(1) << 24) refuse("too many query rows");
     if (!std::isfinite(a.scale)) refuse("attention scale is not finite");
     if (cache.overlaps(a.output)) refuse("attention output overlaps the cache");
     for (const TensorView &v : {a.queries, a.pages, a.lengths, a.query_offsets, a.prefix_pages, a.prefix_length})

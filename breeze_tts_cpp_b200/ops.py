@@ -163,7 +163,7 @@ def _fusion(residual=None, projection_bias=None, raw=None, gate=None, shift=None
 
 
 if not isinstance(_native, _lib.MissingBinding):
-    _native.bind(_lib.B200QError, RowScaledView.c)
+    _native.bind(_lib.B200QError, RowScaledView.c, CacheView.c, Rotary.c)
 
 
 class Context:
@@ -295,8 +295,9 @@ class Context:
         """Turns every head of x [rows, heads * head_dim] by positions [rows] (int32). out may be x."""
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _lib.call("b200q_rotary", self._handle, C.byref(_tensor(x)), C.byref(_tensor(positions)), C.byref(rotary.c()), head_dim,
-                  C.byref(_tensor(out)))
+        if _native.rotary(self._address, x, positions, rotary, head_dim, out) is NotImplemented:
+            _lib.call("b200q_rotary", self._handle, C.byref(_tensor(x)), C.byref(_tensor(positions)), C.byref(rotary.c()), head_dim,
+                      C.byref(_tensor(out)))
         return out
 
     def cache_write(self, cache: CacheView, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor | None = None,
@@ -304,13 +305,15 @@ class Context:
                     q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None, epsilon: float = 1e-6) -> None:
         """Quantizes row r of k and v [rows, kv_heads * head_dim] into slot slots[r] (int32, each at most once; negative or past the
         cache: left out). k, and q into q_out (may be q), are normalised over each head and turned first, where the arguments say so."""
-        _lib.call("b200q_cache_write", self._handle, C.byref(cache.c()), C.byref(_tensor(k)), C.byref(_tensor(v)), C.byref(_tensor(slots)),
-                  C.byref(_tensor(positions)), C.byref(rotary.c()) if rotary is not None else None, C.byref(_tensor(q)),
-                  C.byref(_tensor(q_out)), C.byref(_tensor(q_norm)), C.byref(_tensor(k_norm)), epsilon)
+        if _native.cache_write(self._address, cache, k, v, slots, positions, rotary, q, q_out, q_norm, k_norm, epsilon) is NotImplemented:
+            _lib.call("b200q_cache_write", self._handle, C.byref(cache.c()), C.byref(_tensor(k)), C.byref(_tensor(v)), C.byref(_tensor(slots)),
+                      C.byref(_tensor(positions)), C.byref(rotary.c()) if rotary is not None else None, C.byref(_tensor(q)),
+                      C.byref(_tensor(q_out)), C.byref(_tensor(q_norm)), C.byref(_tensor(k_norm)), epsilon)
 
     def cache_read(self, cache: CacheView, slots: torch.Tensor, k: torch.Tensor | None, v: torch.Tensor | None) -> None:
         """Row r of k and v (either may be None) = what slot slots[r] holds; zeros for a slot outside of the cache."""
-        _lib.call("b200q_cache_read", self._handle, C.byref(cache.c()), C.byref(_tensor(slots)), C.byref(_tensor(k)), C.byref(_tensor(v)))
+        if _native.cache_read(self._address, cache, slots, k, v) is NotImplemented:
+            _lib.call("b200q_cache_read", self._handle, C.byref(cache.c()), C.byref(_tensor(slots)), C.byref(_tensor(k)), C.byref(_tensor(v)))
 
     def cached_attention(self, q: torch.Tensor, cache: CacheView, pages: torch.Tensor, lengths: torch.Tensor, out: torch.Tensor,
                          scale: float = 0.0, query_offsets: torch.Tensor | None = None, prefix_pages: torch.Tensor | None = None,
@@ -319,9 +322,11 @@ class Context:
         sequence's cached tokens, the query rows' own among them; query_offsets [sequences + 1] its rows (without it, one each). All
         rows also see the prefix_length [1] tokens on prefix_pages [m], which are read once for the batch. Rows that see nothing are
         zero, rows behind the last offset are left alone. scale 0: 1 / sqrt(head_dim)."""
-        arguments = Attention(_tensor(q), _tensor(out), _tensor(pages), _tensor(lengths), _tensor(query_offsets), _tensor(prefix_pages),
-                              _tensor(prefix_length), scale)
-        _lib.call("b200q_cached_attention", self._handle, C.byref(cache.c()), C.byref(arguments))
+        if _native.cached_attention(self._address, q, cache, pages, lengths, out, scale, query_offsets, prefix_pages,
+                                    prefix_length) is NotImplemented:
+            arguments = Attention(_tensor(q), _tensor(out), _tensor(pages), _tensor(lengths), _tensor(query_offsets), _tensor(prefix_pages),
+                                  _tensor(prefix_length), scale)
+            _lib.call("b200q_cached_attention", self._handle, C.byref(cache.c()), C.byref(arguments))
         return out
 
     def status(self) -> int:

@@ -104,6 +104,22 @@ def test_shared_prefix(ctx_factory, lengths, counts, prefix, heads, kv_heads, he
     check(batch.run(ctx_factory("int8")), *batch.want())
 
 
+def test_many_sequences(ctx_factory):
+    """More than a warp adds up by itself."""
+    g = torch.Generator().manual_seed(1)
+    batch = Batch(20, torch.randint(0, 300, (700,), generator=g).tolist(), None, heads=2, kv_heads=2, head_dim=64, page=32)
+    check(batch.run(ctx_factory("int8")), *batch.want())
+    batch = Batch(21, torch.randint(0, 40, (300,), generator=g).tolist(), torch.randint(0, 3, (300,), generator=g).tolist(), heads=2, kv_heads=1,
+                  head_dim=64, page=16, prefix=50, spare_rows=1)
+    check(batch.run(ctx_factory("int8")), *batch.want())
+
+
+@pytest.mark.parametrize("prefix", [None, 20])
+def test_no_queries_at_all(ctx_factory, prefix):
+    batch = Batch(22, [30, 0], [0, 0], spare_rows=2, prefix=prefix)
+    assert (batch.run(ctx_factory("int8")) == 5).all()
+
+
 def test_lengths_beyond_the_tables_are_clamped(ctx_factory):
     batch = Batch(3, [48, 32], None, page=16)
     batch.pages = batch.pages[:, :2].contiguous()  # 32 positions each
