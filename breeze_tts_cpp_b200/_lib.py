@@ -88,7 +88,7 @@ SIGNATURES = {
     "b200q_cache_write": (C.c_int, (C.c_void_p, _PC, _PT, _PT, _PT, _PT, _PO, _PT, _PT, _PT, _PT, C.c_float, *_ERR)),
     "b200q_cache_read": (C.c_int, (C.c_void_p, _PC, _PT, _PT, _PT, *_ERR)),
     "b200q_cached_attention": (C.c_int, (C.c_void_p, _PC, C.POINTER(Attention), *_ERR)),
-    "b200q_attention_workspace": (C.c_int, (C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+    "b200q_attention_workspace": (C.c_int, (C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                                             C.POINTER(C.c_size_t), *_ERR)),
     "b200q_linear_layer_create": (C.c_int, (C.c_void_p, _PT, C.c_int32, _PT, C.POINTER(C.c_void_p), *_ERR)),
     "b200q_linear_layer_destroy": (None, (C.c_void_p,)),

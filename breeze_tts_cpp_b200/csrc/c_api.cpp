@@ -360,11 +360,11 @@ int b200q_cached_attention(b200q_context *c, const b200q_cache *cache, const b20
         ops::cached_attention(cache_of(cache), arguments);
     });
 }
-int b200q_attention_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t prefix, int32_t multiprocessors,
+int b200q_attention_workspace(int32_t rows, int32_t sequences, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t prefix, int32_t multiprocessors,
                               size_t *needed, char *error, size_t capacity) {
     return guarded(error, capacity, [&] {
         if (!needed) throw std::invalid_argument("null size");
-        *needed = ops::cached_attention_workspace(rows, heads, kv_heads, head_dim, prefix != 0, multiprocessors);
+        *needed = ops::cached_attention_workspace(rows, sequences, heads, kv_heads, head_dim, prefix != 0, multiprocessors);
     });
 }
 

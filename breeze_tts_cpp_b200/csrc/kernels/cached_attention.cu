@@ -1,6 +1,6 @@
 // Host side of the attention over the quantized cache: workspace, tensor maps, choice of the instance.
 #include "kernels/cached_attention.h"
-#include "kernels/cached_attention_sm100.cuh"
+#include "kernels/cached_attention_tiles_sm100.cuh"
 #include "kernels/tensor_map.h"
 #include <algorithm>
 #include <climits>
@@ -27,22 +27,37 @@ CUtensorMap cache_map(const void *base, const CacheView &cache, int box_rows) {
     return map;
 }
 
+constexpr int kFewRows = 16; // query rows of a cached head up to which a segment of at most sixteen is the better one
 constexpr size_t kPiece = 256; // parts of the workspace start on multiples of this
 size_t padded(size_t bytes) { return (bytes + kPiece - 1) / kPiece * kPiece; }
-constexpr int kMostColumns = 16;
 
-// The workspace of one pass: the table, the parts, and for a shared prefix the rows that were done in one part.
+// How one pass over a set of page tables is done.
+struct PassPlan {
+    bool many, narrow; // 128 query rows per segment on the tensor cores' own memory; else eight, or sixteen
+    int part_columns;
+};
+PassPlan plan_pass(int rows, int sequences, int group, bool prefix) {
+    // Query rows of a cached head, on the average: all of them share a prefix.
+    const int64_t all = int64_t(rows) * group, each = prefix ? all : all / std::max(sequences, 1);
+    PassPlan plan{each > kFewRows, each <= 8, 16};
+    if (plan.many) plan.part_columns = int(std::min<int64_t>(kManyRows, all));
+    return plan;
+}
+// A pass's workspace: the table, the partial sums, and with a shared prefix the rows that were done in one part.
 struct Carve {
     size_t table, partials, complete, bytes;
-    Carve(int rows, int heads, int head_dim, bool prefix, int ctas) {
+    Carve(int rows, int heads, int head_dim, bool prefix, int part_columns, int ctas) {
         const size_t row = size_t(head_dim + kPartialExtra) * 4;
         table = 0;
         partials = padded(size_t(rows) * heads * sizeof(int4));
-        complete = partials + padded(size_t(ctas) * 2 * kMostColumns * row);
+        complete = partials + padded(size_t(ctas) * 2 * part_columns * row);
         bytes = complete + (prefix ? padded(size_t(rows) * heads * row) : 0);
     }
 };
 
+template <class T, Type F, int HeadDim> void launch_many(const AttentionArgs &args, int ctas, cudaStream_t stream) {
+    launch_pdl("cached attention", cached_attention_many<T, F, HeadDim>, dim3(unsigned(ctas)), dim3(kManyThreads), ManyShape<HeadDim>::smem, stream, args);
+}
 template <class T, Type F, int HeadDim, int Tiles>
 void launch_pass(AttentionArgs args, int most_columns, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
     using Shape = AttentionShape<HeadDim, Tiles>;
@@ -76,10 +91,13 @@ bool aligned16(const TensorView &v) {
     return reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && (v.rows <= 1 || v.ld() % 8 == 0);
 }
 template <class T, Type F, int HeadDim> void raise_limit() {
-    for (auto *kernel : {cached_attention<T, F, HeadDim, 1>, cached_attention<T, F, HeadDim, 2>}) {
-        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kAttentionSmem));
+    auto raise = [](auto *kernel, size_t bytes) {
+        const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
         if (status != cudaSuccess) throw std::runtime_error(std::string("cudaFuncSetAttribute(attention): ") + cudaGetErrorString(status));
-    }
+    };
+    raise(cached_attention<T, F, HeadDim, 1>, kAttentionSmem);
+    raise(cached_attention<T, F, HeadDim, 2>, kAttentionSmem);
+    raise(cached_attention_many<T, F, HeadDim>, ManyShape<HeadDim>::smem);
 }
 } // namespace
 
@@ -90,8 +108,11 @@ void raise_attention_limits() {
                 by_type(element, format, head_dim, [](auto t, auto f, auto width) { raise_limit<decltype(t), decltype(f)::value, decltype(width)::value>(); });
 }
 
-size_t attention_workspace_bytes(int rows, int heads, int, int head_dim, bool prefix, int multiprocessors) {
-    return Carve(rows, heads, head_dim, prefix, multiprocessors).bytes * (prefix ? 2 : 1);
+size_t attention_workspace_bytes(int rows, int sequences, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors) {
+    size_t bytes = 0;
+    for (int pass = 0; pass < (prefix ? 2 : 1); ++pass)
+        bytes += Carve(rows, heads, head_dim, prefix, plan_pass(rows, sequences, heads / kv_heads, pass).part_columns, multiprocessors).bytes;
+    return bytes;
 }
 
 void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t workspace_bytes, int *status, int multiprocessors,
@@ -99,8 +120,8 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     const int rows = p.queries.rows, head_dim = p.cache.head_dim, heads = p.queries.cols / head_dim, ctas = multiprocessors;
     const bool prefix = p.prefix_pages != nullptr;
     if (!rows) return;
-    const Carve carve(rows, heads, head_dim, prefix, ctas);
-    if (workspace_bytes < carve.bytes * (prefix ? 2 : 1)) throw std::invalid_argument("attention workspace is too small");
+    if (workspace_bytes < attention_workspace_bytes(rows, p.sequences, heads, p.cache.kv_heads, head_dim, prefix, ctas))
+        throw std::invalid_argument("attention workspace is too small");
 
     AttentionArgs args{};
     args.queries = p.queries.data, args.output = p.output.data;
@@ -111,6 +132,7 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     args.sequences = p.sequences, args.page_columns = p.page_columns, args.page_stride = p.page_stride;
     args.page_shift = shift_of(p.cache.page_size), args.total_pages = p.cache.pages, args.offset_count = p.sequences;
     args.box_shift = std::min(args.page_shift, shift_of(kTileKeys));
+    args.cached_keys = p.cache.keys, args.cached_values = p.cache.values;
     args.key_scales = p.cache.key_scales, args.value_scales = p.cache.value_scales;
     const float format = p.cache.type == Type::FP8 ? 256.f : 1.f; // e4m3 values enter the second product times 2^-8
     args.score_scale = p.scale * 1.4426950408889634f;
@@ -124,23 +146,25 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     const CUtensorMap keys = cache_map(p.cache.keys, p.cache, 1 << args.box_shift), values = cache_map(p.cache.values, p.cache, 1 << args.box_shift);
     by_type(p.queries.type, p.cache.type, head_dim, [&](auto element, auto format, auto width) {
         using T = decltype(element);
+        char *base = static_cast<char *>(workspace);
         for (int pass = 0; pass < combine.sources; ++pass) {
-            char *base = static_cast<char *>(workspace) + pass * carve.bytes;
+            const PassPlan plan = plan_pass(rows, p.sequences, args.group, pass);
+            const Carve carve(rows, heads, head_dim, prefix, plan.part_columns, ctas);
+            args.part_columns = plan.part_columns;
             args.table = reinterpret_cast<int4 *>(base + carve.table);
             args.partials = reinterpret_cast<float *>(base + carve.partials);
             args.complete = prefix ? reinterpret_cast<float *>(base + carve.complete) : nullptr;
-            // Eight query rows per segment, or sixteen where a sequence has more than eight: each cached byte is then widened for both halves.
-            bool narrow = args.group <= 8 && (!p.query_offsets || rows <= p.sequences);
+            base += carve.bytes;
             if (pass) {
                 args.prefix = true;
                 args.pages = p.prefix_pages, args.lengths = p.prefix_length, args.sequences = 1;
                 args.page_columns = args.page_stride = p.prefix_columns;
-                narrow = (long long)rows * args.group <= 8;
             }
             // Query rows of one segment at most: where each sequence has one row, those of a cached head.
             const int most = !pass && !p.query_offsets ? args.group : INT_MAX;
-            launch_pass<T, decltype(format)::value, decltype(width)::value>(narrow, most, args, keys, values, ctas, stream);
-            combine.source[pass] = {args.partials, args.complete, args.table, ctas, narrow ? 8 : 16};
+            if (plan.many) launch_many<T, decltype(format)::value, decltype(width)::value>(args, ctas, stream);
+            else launch_pass<T, decltype(format)::value, decltype(width)::value>(plan.narrow, most, args, keys, values, ctas, stream);
+            combine.source[pass] = {args.partials, args.complete, args.table, ctas, plan.part_columns};
         }
         const long long warps = (long long)rows * heads;
         launch_pdl("attention combine", combine_attention<T, decltype(width)::value>, dim3(unsigned((warps + kCombineThreads / 32 - 1) / (kCombineThreads / 32))),

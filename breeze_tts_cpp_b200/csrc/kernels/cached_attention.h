@@ -17,7 +17,7 @@ struct AttentionProblem {
     float scale = 0.f;
 };
 // Bytes of workspace behind the context's header that a launch uses.
-size_t attention_workspace_bytes(int rows, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors);
+size_t attention_workspace_bytes(int rows, int sequences, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors);
 void launch_cached_attention(const AttentionProblem &, void *workspace, size_t workspace_bytes, int *status, int multiprocessors,
                              cudaStream_t stream);
 // Part of quant_linear_initialize: the instances' dynamic shared memory, on the current device.

@@ -23,44 +23,14 @@
 // the lengths are, a segment's fixed cost counted as a part of a tile; a segment that runs over a share's end leaves partial sums, which a second launch adds in
 // a fixed order.
 #pragma once
-#include "kernels/launch.cuh"
+#include "kernels/cached_attention_work.cuh"
 #include "kernels/sm100_ptx.cuh"
-#include "core/tensor.h"
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 
 namespace tts::b200 {
-constexpr int kTileKeys = 128, kTeam = 4, kTeams = 2, kWorkers = kTeam * kTeams, kProducers = 2, kMergers = 2, kMaxRing = 12;
+constexpr int kTeam = 4, kTeams = 2, kWorkers = kTeam * kTeams, kProducers = 2, kMergers = 2, kMaxRing = 12;
 constexpr int kAttentionWarps = kWorkers + kProducers + kMergers, kAttentionThreads = 32 * kAttentionWarps; // three per scheduler: 168 registers a thread
-constexpr int kScanAlone = 256; // up to here each producer warp adds the sequences' work up by itself
-constexpr int kPartialExtra = 4; // maximum and sum behind a partial row, padded to 16 bytes
-constexpr size_t kAttentionSmem = 224 * 1024;
+constexpr int kFewSegmentUnits = 2; // a segment's queries, flush and merge next to a tile's kTileUnits
 
-// One pass over one set of page tables: the sequences' own, or the shared prefix as one sequence of all query rows.
-struct AttentionArgs {
-    const void *queries;
-    void *output;
-    int query_stride, output_stride, rows, heads, group, kv_heads;
-    bool aligned;
-    const int *pages, *lengths, *query_offsets;
-    int sequences, page_columns, page_stride, page_shift, total_pages, box_shift;
-    int offset_count; // entries of query_offsets behind the first; the last one counts the rows
-    bool prefix;
-    const float *key_scales, *value_scales;
-    float score_scale; // softmax scale, log2 e and the key format's factor
-    float output_scale;
-    int stages, merge_columns, merge_buffers;
-    float *partials; // [ctas][2][columns][head_dim + kPartialExtra]
-    int4 *table;     // [rows * heads]: first CTA, parts, slot of the first part, column; parts == 0: complete
-    float *complete; // [rows * heads][head_dim + kPartialExtra], or null: complete segments go to the output
-    int *status;
-};
-
-__device__ __forceinline__ int load_index(const int *p) {
-    int v;
-    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -131,81 +101,6 @@ struct TileNote {
 };
 constexpr int kNoteFirst = 1, kNoteFlush = 2, kNoteEnd = 4, kNoteFinal = 16, kNoteSplit = 32, kNoteQuit = 64;
 
-// A sequence as the tables give it, made safe: rows and positions stay inside of what the caller passed.
-struct SequenceShape {
-    int length, count, row;
-};
-__device__ __forceinline__ SequenceShape sequence_of(const AttentionArgs &a, int b) {
-    SequenceShape s;
-    if (a.prefix) {
-        s.row = 0;
-        s.count = a.query_offsets ? load_index(a.query_offsets + a.offset_count) : a.rows;
-    } else if (a.query_offsets) {
-        s.row = load_index(a.query_offsets + b);
-        s.count = load_index(a.query_offsets + b + 1) - s.row;
-    } else {
-        s.row = b;
-        s.count = 1;
-    }
-    s.row = max(s.row, 0);
-    s.count = max(0, min(s.count, a.rows - s.row));
-    s.length = max(0, min(load_index(a.lengths + b), a.page_columns << a.page_shift));
-    return s;
-}
-// Tiles of keys that query tile `qt` of a sequence sees; at least one, so that rows that see nothing are written too.
-template <int Columns> __device__ __forceinline__ int tiles_of(const AttentionArgs &a, const SequenceShape &s, int qt) {
-    int end = s.length;
-    if (!a.prefix) end += min(s.count - 1, (qt * Columns + Columns - 1) / a.group) + 1 - s.count;
-    return max(1, (end + kTileKeys - 1) / kTileKeys);
-}
-template <int Columns> __device__ __forceinline__ int query_tiles(const AttentionArgs &a, const SequenceShape &s) {
-    return (s.count * a.group + Columns - 1) / Columns;
-}
-// Tiles of one head of a sequence, over its query tiles.
-template <int Columns> __device__ __forceinline__ long long head_tiles(const AttentionArgs &a, const SequenceShape &s, int count) {
-    if (a.prefix) return (long long)count * tiles_of<Columns>(a, s, 0);
-    long long tiles = 0;
-    for (int qt = 0; qt < count; ++qt) tiles += tiles_of<Columns>(a, s, qt);
-    return tiles;
-}
-// Work of a run of sequences: tiles, and segments in the 24 high bits (the host refuses more), so that one scan adds up both.
-constexpr int kSegmentShift = 40;
-template <int Columns> __device__ __forceinline__ long long work_of(const AttentionArgs &a, int b) {
-    const SequenceShape s = sequence_of(a, b);
-    const int count = query_tiles<Columns>(a, s);
-    return a.kv_heads * (head_tiles<Columns>(a, s, count) + ((long long)count << kSegmentShift));
-}
-__device__ __forceinline__ long long scan_warp(long long v, int lane) { // inclusive
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v += other;
-    }
-    return v;
-}
-// 64-bit quotients take a hundred cycles, 32-bit ones a fifth; the operands are not negative.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return (a | b) >> 32 ? a / b : (long long)(uint32_t(a) / uint32_t(b));
-}
-// Shares are counted in units: kTileUnits for a tile, kSegmentUnits more for a segment (its queries, its flush and its merge). A tile belongs to the
-// CTA whose share holds its first unit.
-constexpr int kTileUnits = 4, kSegmentUnits = 2;
-
-// One query row's result: the output row, or what is kept of it for the second launch.
-template <class T, int HeadDim>
-__device__ __forceinline__ void store_row4(const AttentionArgs &a, T *to, float4 v, float factor) {
-    union {
-        uint2 word;
-        T e[4];
-    } out;
-    out.e[0] = T(v.x * factor), out.e[1] = T(v.y * factor), out.e[2] = T(v.z * factor), out.e[3] = T(v.w * factor);
-    if (a.aligned) {
-        *reinterpret_cast<uint2 *>(to) = out.word;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[i] = out.e[i];
-    }
-}
 
 template <class T, Type F, int HeadDim, int Tiles>
 __global__ void __launch_bounds__(kAttentionThreads, 1)
@@ -215,7 +110,8 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t full[kTeams][kMaxRing], empty[kMaxRing], merge_full[2]; // full: of each team
     __shared__ TileNote notes[kMaxRing], merge_notes[2];
-    __shared__ long long sums[kAttentionWarps], found[3]; // found: sequence of this CTA's first unit, the sequence's first unit, all work
+    __shared__ long long sums[kAttentionWarps];
+    __shared__ Start found;
     __shared__ int abort_flag;
     __shared__ int merged; // parts that the mergers are done with, times kMergers
     const uint32_t ring = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;
@@ -238,46 +134,10 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     pdl_launch_dependents();
     __syncthreads();
 
-    // The producers need the work of all sequences, and where their CTA's share lies among them: a lane takes a run of sequences, then a scan over
-    // the lanes. For a long batch all threads do.
-    auto spread = [&](int threads, int thread, long long base, long long own, long long all, auto &&keep) {
-        const long long tiles = all & ((1ll << kSegmentShift) - 1), ctas = tiles < gridDim.x ? tiles : gridDim.x;
-        if (blockIdx.x >= ctas) return;
-        const int extra = tiles > gridDim.x ? kSegmentUnits : 0;
-        auto units = [&](long long work) { return kTileUnits * (work & ((1ll << kSegmentShift) - 1)) + extra * (work >> kSegmentShift); };
-        const long long total = units(all), each = quotient(total, ctas), rest = total - each * ctas;
-        const long long begin = each * blockIdx.x + min((long long)blockIdx.x, rest);
-        long long at = units(base);
-        if (at > begin || begin >= at + units(own)) return;
-        const int run = (args.sequences + threads - 1) / threads, from = thread * run, to = min(args.sequences, from + run);
-        for (int b = from; b < to; ++b) {
-            const long long part = units(work_of<kColumns>(args, b));
-            if (begin < at + part) {
-                keep(b, at);
-                break;
-            }
-            at += part;
-        }
-    };
-    auto work_of_run = [&](int threads, int thread) {
-        const int run = (args.sequences + threads - 1) / threads, from = min(args.sequences, thread * run), to = min(args.sequences, from + run);
-        long long own = 0;
-        for (int b = from; b < to; ++b) own += work_of<kColumns>(args, b);
-        return own;
-    };
+    // Only the producers need to know where the CTA's share lies; for a long batch all threads find out.
     if (args.sequences > kScanAlone) {
         pdl_wait_upstream();
-        const long long own = work_of_run(kAttentionThreads, int(threadIdx.x));
-        long long before = scan_warp(own, lane), all = 0;
-        if (lane == 31) sums[warp] = before;
-        __syncthreads();
-        for (int w = 0; w < kAttentionWarps; ++w) {
-            if (w < warp) before += sums[w];
-            all += sums[w];
-        }
-        if (!threadIdx.x) found[2] = all;
-        spread(kAttentionThreads, int(threadIdx.x), before - own, own, all, [&](int b, long long at) { found[0] = b, found[1] = at; });
-        __syncthreads();
+        start_together<kColumns, kAttentionWarps>(args, kFewSegmentUnits, sums, &found);
     }
     // Every wait is bounded, and a warp whose wait gave up leaves as one; the others follow when theirs do.
     auto wait = [&](uint64_t &bar, uint32_t parity) {
@@ -305,148 +165,100 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         // Two warps walk the same list: one copies keys and queries and writes the notes, the other copies values and scales. A tensor copy costs its
         // issuer 50 to 100 cycles and a tile of 16-token pages takes sixteen of them, so one warp would be what the ring waits for.
         const bool leads = warp == kProducer;
-        int stage = 0, issued = 0, ordinal = 0, b = 0, team = 0;
+        int stage = 0, issued = 0, team = 0;
         uint32_t phase = 0;
-        long long at = 0, all; // at: first unit of the segment
-        if (args.sequences > kScanAlone) {
-            b = int(found[0]), at = found[1], all = found[2];
-        } else {
-            pdl_wait_upstream();
-            const long long own = work_of_run(32, lane), through = scan_warp(own, lane);
-            all = __shfl_sync(0xffffffffu, through, 31);
-            bool here = false;
-            spread(32, lane, through - own, own, all, [&](int sequence, long long unit) { here = true, b = sequence, at = unit; });
-            if (const unsigned who = __ballot_sync(0xffffffffu, here)) {
-                b = __shfl_sync(0xffffffffu, b, __ffs(who) - 1);
-                at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1);
-            }
-        }
-        // Where there is a CTA for every tile, each gets one. A share is never smaller than a tile, so that every CTA between a segment's first
-        // and its last has a part of it.
-        const long long all_tiles = all & ((1ll << kSegmentShift) - 1), ctas = all_tiles < gridDim.x ? all_tiles : gridDim.x;
-        const int extra = all_tiles > gridDim.x ? kSegmentUnits : 0;
-        const long long total = kTileUnits * all_tiles + extra * (all >> kSegmentShift), each = ctas ? quotient(total, ctas) : 0, rest = total - each * ctas;
-        auto share_of = [&](long long cta) { return each * cta + min(cta, rest); }; // its first unit
-        const long long begin = share_of(min((long long)blockIdx.x, ctas)), end = share_of(min((long long)blockIdx.x + 1, ctas));
+        if (args.sequences <= kScanAlone) pdl_wait_upstream();
+        const Start start = args.sequences > kScanAlone ? found : start_alone<kColumns>(args, kFewSegmentUnits);
         const int box = 1 << args.box_shift, boxes = kTileKeys >> args.box_shift;
         const uint32_t box_bytes = uint32_t(box) * 2 * HeadDim;
-        if (begin >= end) b = args.sequences; // nothing to do here
         bool open = true;
-        for (; open && b < args.sequences && at < end; ++b) {
-            const SequenceShape s = sequence_of(args, b);
-            const int query_count = query_tiles<kColumns>(args, s);
-            const int *pages = args.pages + size_t(b) * args.page_stride;
+        const int parts = walk_share<kColumns>(args, kFewSegmentUnits, start, [&](const SegmentPart &part) {
+            const SequenceShape &s = part.s;
+            const int low = part.low, high = part.high, head = part.head, columns = part.columns;
+            const int *pages = args.pages + size_t(part.sequence) * args.page_stride;
             // Lane i's page of a tile: its box i. Always a load, of the last page where there is none, so that nothing waits for it here.
             auto page_at = [&](int tile) {
                 return load_index(pages + (max(0, min(tile * kTileKeys + (min(lane, boxes - 1) << args.box_shift), s.length - 1)) >> args.page_shift));
             };
-            int segment = 0;
-            if (begin > at) { // whole heads in front of the share
-                const long long head_units = kTileUnits * head_tiles<kColumns>(args, s, query_count) + (long long)extra * query_count;
-                const long long heads = head_units ? min(quotient(begin - at, head_units), (long long)args.kv_heads) : 0;
-                segment = int(heads) * query_count, at += heads * head_units;
-            }
-            // Heads outermost: their query tiles read the same keys, near one another in time.
-            for (; open && segment < query_count * args.kv_heads && at < end; ++segment) {
-                const int head = segment / query_count, qt = segment - head * query_count, tiles = tiles_of<kColumns>(args, s, qt);
-                const long long first_unit = at + extra;
-                at = first_unit + (long long)kTileUnits * tiles;
-                const auto tile_from = [&](long long unit) { // first tile that starts at or behind a unit
-                    return unit <= first_unit ? 0 : unit >= at ? tiles : int((unit - first_unit + kTileUnits - 1) / kTileUnits);
-                };
-                const int low = tile_from(begin), high = tile_from(end);
-                if (low == high) continue;
-                int first_cta = -1, first_slot = 0;
-                const bool split = low || high < tiles;
-                if (split && high == tiles) { // this CTA closes the segment: it says where its parts lie
-                    const long long larger = rest * (each + 1); // units of the shares that have one more
-                    first_cta = int(first_unit < larger ? quotient(first_unit, each + 1) : rest + quotient(first_unit - larger, each));
-                    first_slot = share_of(first_cta) < first_unit - extra ? 1 : 0;
-                }
-                const int columns = min(kColumns, s.count * args.group - qt * kColumns);
-                int next = page_at(low);
-                for (int tile = low; tile < high; ++tile) {
-                    const int page = next;
-                    if (tile + 1 < high) next = page_at(tile + 1); // on its way while this tile's stage is waited for
-                    if (issued >= stages && !wait(empty[stage], phase ^ 1)) {
-                        open = false;
-                        break;
-                    }
-                    const uint32_t to = ring + stage * Shape::stage, bar = ptx::smem_u32(&full[team][stage]);
-                    uint8_t *const bytes = ring_bytes + stage * Shape::stage;
-                    const int key = tile * kTileKeys, position = key + (lane << args.box_shift);
-                    const bool good = lane < boxes && position < s.length && unsigned(page) < unsigned(args.total_pages);
-                    const uint32_t held = __ballot_sync(0xffffffffu, good);
-                    const int row = (((page * args.kv_heads) + head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
-                    if (leads) {
-                        // Each team's first tile of the part brings the query rows.
-                        const bool first = tile - low < kTeams, flush = tile + kTeams >= high;
-                        const T *query = nullptr;
-                        uint32_t query_bytes = 0;
-                        if (first) {
-                            const int flat = qt * kColumns + lane;
-                            query = static_cast<const T *>(args.queries) + size_t(s.row + flat / args.group) * args.query_stride +
-                                    (head * args.group + flat % args.group) * HeadDim;
-                            if (args.aligned) query_bytes = uint32_t(columns) * HeadDim * 2;
-                            else if (lane < columns)
-                                for (int d = 0; d < HeadDim; ++d) {
-                                    uint16_t v;
-                                    asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(query + d) : "memory");
-                                    *reinterpret_cast<uint16_t *>(bytes + Shape::queries + lane * Shape::query_row + 2 * d) = v;
-                                }
-                            __syncwarp();
-                        }
-                        if (!lane) {
-                            TileNote &n = notes[stage];
-                            n.key = key;
-                            n.flags = (first ? kNoteFirst : 0) | (flush ? kNoteFlush : 0) | (tile + 1 == high ? kNoteEnd : 0) |
-                                      (high < tiles || at + extra >= end ? kNoteFinal : 0) | (split ? kNoteSplit : 0);
-                            if (first || flush) { // what the workers read at a part's ends only
-                                n.head = head, n.row = s.row, n.count = s.count, n.flat = qt * kColumns;
-                                n.limit = args.prefix ? s.length - 1 : s.length - s.count;
-                                n.ordinal = ordinal, n.first_cta = first_cta, n.first_slot = first_slot;
-                                n.slot = first_unit - extra > begin ? 1 : 0;
-                                n.parts = min(kTeams, high - low), n.first_team = (issued - (tile - low)) % kTeams;
+            int next = page_at(low);
+            for (int tile = low; tile < high; ++tile) {
+                const int page = next;
+                if (tile + 1 < high) next = page_at(tile + 1); // on its way while this tile's stage is waited for
+                if (issued >= stages && !wait(empty[stage], phase ^ 1)) return open = false;
+                const uint32_t to = ring + stage * Shape::stage, bar = ptx::smem_u32(&full[team][stage]);
+                uint8_t *const bytes = ring_bytes + stage * Shape::stage;
+                const int key = tile * kTileKeys, position = key + (lane << args.box_shift);
+                const bool good = lane < boxes && position < s.length && unsigned(page) < unsigned(args.total_pages);
+                const uint32_t held = __ballot_sync(0xffffffffu, good);
+                const int row = (((page * args.kv_heads) + head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
+                if (leads) {
+                    // Each team's first tile of the part brings the query rows.
+                    const bool first = tile - low < kTeams, flush = tile + kTeams >= high;
+                    const T *query = nullptr;
+                    uint32_t query_bytes = 0;
+                    if (first) {
+                        const int flat = part.query_tile * kColumns + lane;
+                        query = static_cast<const T *>(args.queries) + size_t(s.row + flat / args.group) * args.query_stride +
+                                (head * args.group + flat % args.group) * HeadDim;
+                        if (args.aligned) query_bytes = uint32_t(columns) * HeadDim * 2;
+                        else if (lane < columns)
+                            for (int d = 0; d < HeadDim; ++d) {
+                                uint16_t v;
+                                asm volatile("ld.global.b16 %0, [%1];" : "=h"(v) : "l"(query + d) : "memory");
+                                *reinterpret_cast<uint16_t *>(bytes + Shape::queries + lane * Shape::query_row + 2 * d) = v;
                             }
-                            ptx::mbar_arrive_expect_tx(bar, __popc(held) * box_bytes + query_bytes);
-                        }
                         __syncwarp();
-                        if (query_bytes && lane < columns) copy_run(to + Shape::queries + lane * Shape::query_row, query, HeadDim * 2, bar);
-                    } else {
-                        // Scales: a lane copies four of the keys' and four of the values'. Positions on a page that the cache does not have read as NaN.
-                        const int owner = (4 * lane) >> args.box_shift;
-                        const int its_row = __shfl_sync(0xffffffffu, row, owner) + ((4 * lane) & (box - 1));
-                        if (held >> owner & 1) {
-                            const uint32_t scales = to + Shape::scales + 16 * lane;
-                            copy_async16(scales, args.key_scales + its_row);
-                            copy_async16(scales + kTileKeys * 4, args.value_scales + its_row);
-                            ptx::copy_async_arrive(bar);
-                        } else {
-                            const float nan = __int_as_float(0x7fffffff);
-                            *reinterpret_cast<float4 *>(bytes + Shape::scales + 16 * lane) = make_float4(nan, nan, nan, nan);
-                            *reinterpret_cast<float4 *>(bytes + Shape::scales + kTileKeys * 4 + 16 * lane) = make_float4(nan, nan, nan, nan);
-                            ptx::mbar_arrive(bar);
-                        }
                     }
-                    // One thread issues the boxes, from rows gathered beforehand.
-                    int from_row[kTileKeys / 16];
-#pragma unroll
-                    for (int i = 0; i < kTileKeys / 16; ++i) from_row[i] = __shfl_sync(0xffffffffu, row, i);
-                    if (ptx::elect_one()) {
-                        const CUtensorMap *map = leads ? &key_map : &value_map;
-                        const uint32_t into = to + (leads ? 0u : Shape::values), box_size = uint32_t(box) * HeadDim;
-#pragma unroll
-                        for (int i = 0; i < kTileKeys / 16; ++i)
-                            if (held >> i & 1) ptx::tma_load_2d(into + i * box_size, map, bar, 0, from_row[i]);
+                    if (!lane) {
+                        TileNote &n = notes[stage];
+                        n.key = key;
+                        n.flags = (first ? kNoteFirst : 0) | (flush ? kNoteFlush : 0) | (tile + 1 == high ? kNoteEnd : 0) |
+                                  (part.final ? kNoteFinal : 0) | (part.split ? kNoteSplit : 0);
+                        if (first || flush) { // what the workers read at a part's ends only
+                            n.head = head, n.row = s.row, n.count = s.count, n.flat = part.query_tile * kColumns;
+                            n.limit = args.prefix ? s.length - 1 : s.length - s.count;
+                            n.ordinal = part.ordinal, n.first_cta = part.first_cta, n.first_slot = part.first_slot;
+                            n.slot = part.slot;
+                            n.parts = min(kTeams, high - low), n.first_team = (issued - (tile - low)) % kTeams;
+                        }
+                        ptx::mbar_arrive_expect_tx(bar, __popc(held) * box_bytes + query_bytes);
                     }
                     __syncwarp();
-                    ++issued;
-                    if (++stage == stages) stage = 0, phase ^= 1;
-                    if (++team == kTeams) team = 0;
+                    if (query_bytes && lane < columns) copy_run(to + Shape::queries + lane * Shape::query_row, query, HeadDim * 2, bar);
+                } else {
+                    // Scales: a lane copies four of the keys' and four of the values'. Positions on a page that the cache does not have read as NaN.
+                    const int owner = (4 * lane) >> args.box_shift;
+                    const int its_row = __shfl_sync(0xffffffffu, row, owner) + ((4 * lane) & (box - 1));
+                    if (held >> owner & 1) {
+                        const uint32_t scales = to + Shape::scales + 16 * lane;
+                        copy_async16(scales, args.key_scales + its_row);
+                        copy_async16(scales + kTileKeys * 4, args.value_scales + its_row);
+                        ptx::copy_async_arrive(bar);
+                    } else {
+                        const float nan = __int_as_float(0x7fffffff);
+                        *reinterpret_cast<float4 *>(bytes + Shape::scales + 16 * lane) = make_float4(nan, nan, nan, nan);
+                        *reinterpret_cast<float4 *>(bytes + Shape::scales + kTileKeys * 4 + 16 * lane) = make_float4(nan, nan, nan, nan);
+                        ptx::mbar_arrive(bar);
+                    }
                 }
-                ++ordinal;
+                // One thread issues the boxes, from rows gathered beforehand.
+                int from_row[kTileKeys / 16];
+#pragma unroll
+                for (int i = 0; i < kTileKeys / 16; ++i) from_row[i] = __shfl_sync(0xffffffffu, row, i);
+                if (ptx::elect_one()) {
+                    const CUtensorMap *map = leads ? &key_map : &value_map;
+                    const uint32_t into = to + (leads ? 0u : Shape::values), box_size = uint32_t(box) * HeadDim;
+#pragma unroll
+                    for (int i = 0; i < kTileKeys / 16; ++i)
+                        if (held >> i & 1) ptx::tma_load_2d(into + i * box_size, map, bar, 0, from_row[i]);
+                }
+                __syncwarp();
+                ++issued;
+                if (++stage == stages) stage = 0, phase ^= 1;
+                if (++team == kTeams) team = 0;
             }
-        }
+            return true;
+        });
         for (int i = 0; i < kTeams && open; ++i) { // an empty stage ends each team
             if (issued >= stages && !wait(empty[stage], phase ^ 1)) break;
             if (leads && !lane) notes[stage].flags = kNoteQuit;
@@ -455,7 +267,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
             if (++stage == stages) stage = 0, phase ^= 1;
             if (++team == kTeams) team = 0;
         }
-        if (!ordinal && leads && !lane) { // a share that holds no tile's first unit
+        if (!parts && leads && !lane) { // a share that holds no tile's first unit
             merge_notes[0].flags = kNoteQuit;
             for (int w = 0; w < kWorkers; ++w) ptx::mbar_arrive(ptx::smem_u32(&merge_full[0]));
         }
@@ -494,14 +306,14 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                 }
                 const int flat = note.flat + column, head = note.head * args.group + flat % args.group;
                 const size_t at_row = size_t(note.row + flat / args.group), index = at_row * args.heads + head;
-                float *kept = flags & kNoteSplit ? args.partials + (size_t(blockIdx.x * 2 + note.slot) * kColumns + column) * Shape::row
+                float *kept = flags & kNoteSplit ? args.partials + (size_t(blockIdx.x * 2 + note.slot) * args.part_columns + column) * Shape::row
                               : args.complete    ? args.complete + index * Shape::row
                                                  : nullptr;
                 if (kept) {
                     *reinterpret_cast<float4 *>(kept + d) = v;
                     if (!d) kept[HeadDim] = highest, kept[HeadDim + 1] = l;
                 } else {
-                    store_row4<T, HeadDim>(args, static_cast<T *>(args.output) + at_row * args.output_stride + head * HeadDim + d, v,
+                    store_row4<T>(args, static_cast<T *>(args.output) + at_row * args.output_stride + head * HeadDim + d, v,
                                            l == 0.f ? 0.f : args.output_scale / l);
                 }
                 if (!d) {

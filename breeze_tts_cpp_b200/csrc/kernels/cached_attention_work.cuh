@@ -1,0 +1,250 @@
+// What the attention kernels share: their arguments, and the division of the work over the CTAs.
+//
+// A segment is a sequence, a cached head and a tile of query rows; a tile is 128 keys of a segment. All CTAs get an equal run of the same list
+// of tiles, whatever the lengths are, a segment's fixed cost counted as parts of a tile; a segment that runs over a share's end leaves partial
+// sums, which a last launch adds in a fixed order. Lengths are on the device only, so every CTA adds the list up for itself.
+#pragma once
+#include "core/tensor.h"
+#include "kernels/launch.cuh"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <climits>
+#include <type_traits>
+
+namespace tts::b200 {
+constexpr int kTileKeys = 128;
+constexpr int kPartialExtra = 4; // maximum and sum behind a partial row, padded to 16 bytes
+constexpr int kScanAlone = 256;  // up to here a warp adds the sequences' work up by itself
+constexpr size_t kAttentionSmem = 224 * 1024;
+
+// One pass over one set of page tables: the sequences' own, or the shared prefix as one sequence of all query rows.
+struct AttentionArgs {
+    const void *queries;
+    void *output;
+    int query_stride, output_stride, rows, heads, group, kv_heads;
+    bool aligned;
+    const int *pages, *lengths, *query_offsets;
+    int sequences, page_columns, page_stride, page_shift, total_pages, box_shift;
+    int offset_count; // entries of query_offsets behind the first; the last one counts the rows
+    bool prefix;
+    const void *cached_keys, *cached_values;
+    const float *key_scales, *value_scales;
+    float score_scale; // softmax scale, log2 e and the key format's factor
+    float output_scale;
+    int stages, merge_columns, merge_buffers;
+    int part_columns; // query rows that a partial sum has room for
+    float *partials; // [ctas][2][part_columns][head_dim + kPartialExtra]
+    int4 *table;     // [rows * heads]: first CTA, parts, slot of the first part, column; parts == 0: complete
+    float *complete; // [rows * heads][head_dim + kPartialExtra], or null: complete segments go to the output
+    int *status;
+};
+
+__device__ __forceinline__ int load_index(const int *p) {
+    int v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+// A sequence as the tables give it, made safe: rows and positions stay inside of what the caller passed.
+struct SequenceShape {
+    int length, count, row;
+};
+__device__ __forceinline__ SequenceShape sequence_of(const AttentionArgs &a, int b) {
+    SequenceShape s;
+    if (a.prefix) {
+        s.row = 0;
+        s.count = a.query_offsets ? load_index(a.query_offsets + a.offset_count) : a.rows;
+    } else if (a.query_offsets) {
+        s.row = load_index(a.query_offsets + b);
+        s.count = load_index(a.query_offsets + b + 1) - s.row;
+    } else {
+        s.row = b;
+        s.count = 1;
+    }
+    s.row = max(s.row, 0);
+    s.count = max(0, min(s.count, a.rows - s.row));
+    s.length = max(0, min(load_index(a.lengths + b), a.page_columns << a.page_shift));
+    return s;
+}
+// Tiles of keys that query tile `qt` of a sequence sees; at least one, so that rows that see nothing are written too.
+template <int Columns> __device__ __forceinline__ int tiles_of(const AttentionArgs &a, const SequenceShape &s, int qt) {
+    int end = s.length;
+    if (!a.prefix) end += min(s.count - 1, (qt * Columns + Columns - 1) / a.group) + 1 - s.count;
+    return max(1, (end + kTileKeys - 1) / kTileKeys);
+}
+template <int Columns> __device__ __forceinline__ int query_tiles(const AttentionArgs &a, const SequenceShape &s) {
+    return (s.count * a.group + Columns - 1) / Columns;
+}
+// Tiles of one head of a sequence, over its query tiles.
+template <int Columns> __device__ __forceinline__ long long head_tiles(const AttentionArgs &a, const SequenceShape &s, int count) {
+    if (a.prefix) return (long long)count * tiles_of<Columns>(a, s, 0);
+    long long tiles = 0;
+    for (int qt = 0; qt < count; ++qt) tiles += tiles_of<Columns>(a, s, qt);
+    return tiles;
+}
+// Work of a run of sequences: tiles, and segments in the 24 high bits (the host refuses more), so that one scan adds up both.
+constexpr int kSegmentShift = 40;
+template <int Columns> __device__ __forceinline__ long long work_of(const AttentionArgs &a, int b) {
+    const SequenceShape s = sequence_of(a, b);
+    const int count = query_tiles<Columns>(a, s);
+    return a.kv_heads * (head_tiles<Columns>(a, s, count) + ((long long)count << kSegmentShift));
+}
+__device__ __forceinline__ long long scan_warp(long long v, int lane) { // inclusive
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long other = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += other;
+    }
+    return v;
+}
+// 64-bit quotients take a hundred cycles, 32-bit ones a fifth; the operands are not negative.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)(uint32_t(a) / uint32_t(b));
+}
+// Shares are counted in units: kTileUnits for a tile, `segment_units` more for a segment. A tile belongs to the CTA whose share holds its first unit.
+constexpr int kTileUnits = 4;
+struct Division {
+    long long each = 0, rest = 0, ctas = 0; // units per share, shares that have one more, shares
+    int extra = 0;
+
+    // Where there is a CTA for every tile, each gets one. A share is never smaller than a tile, so that every CTA between a segment's first and
+    // its last has a part of it.
+    __device__ Division(long long all, int segment_units) {
+        const long long tiles = all & ((1ll << kSegmentShift) - 1);
+        ctas = tiles < gridDim.x ? tiles : gridDim.x;
+        if (!ctas) return;
+        extra = tiles > gridDim.x ? segment_units : 0;
+        const long long total = units(all);
+        each = quotient(total, ctas), rest = total - each * ctas;
+    }
+    __device__ long long units(long long work) const { return kTileUnits * (work & ((1ll << kSegmentShift) - 1)) + extra * (work >> kSegmentShift); }
+    __device__ long long share_of(long long cta) const { return each * min(cta, ctas) + min(min(cta, ctas), rest); } // its first unit
+    __device__ int cta_of(long long unit) const {
+        const long long larger = rest * (each + 1);
+        return int(unit < larger ? quotient(unit, each + 1) : rest + quotient(unit - larger, each));
+    }
+};
+// Where a CTA's share begins: the sequence, and that sequence's first unit.
+struct Start {
+    long long all = 0, unit = 0;
+    int sequence = 0;
+};
+template <int Columns> __device__ __forceinline__ long long work_of_run(const AttentionArgs &a, int threads, int thread) {
+    const int run = (a.sequences + threads - 1) / threads, from = min(a.sequences, thread * run), to = min(a.sequences, from + run);
+    long long own = 0;
+    for (int b = from; b < to; ++b) own += work_of<Columns>(a, b);
+    return own;
+}
+// Whether this thread's run of sequences, with `base` in front of it, holds the start of the CTA's share.
+template <int Columns>
+__device__ __forceinline__ bool holds_start(const AttentionArgs &a, int segment_units, int threads, int thread, long long base, long long own, Start &start) {
+    const Division d(start.all, segment_units);
+    const long long begin = d.share_of(blockIdx.x);
+    if (blockIdx.x >= d.ctas || d.units(base) > begin || begin >= d.units(base + own)) return false;
+    const int run = (a.sequences + threads - 1) / threads, to = min(a.sequences, thread * run + run);
+    start.unit = d.units(base);
+    for (start.sequence = thread * run; start.sequence < to; ++start.sequence) {
+        const long long part = d.units(work_of<Columns>(a, start.sequence));
+        if (begin < start.unit + part) break;
+        start.unit += part;
+    }
+    return true;
+}
+// By one warp, for a batch of up to kScanAlone sequences.
+template <int Columns> __device__ __forceinline__ Start start_alone(const AttentionArgs &a, int segment_units) {
+    const int lane = threadIdx.x & 31;
+    const long long own = work_of_run<Columns>(a, 32, lane), through = scan_warp(own, lane);
+    Start start;
+    start.all = __shfl_sync(0xffffffffu, through, 31);
+    const bool here = holds_start<Columns>(a, segment_units, 32, lane, through - own, own, start);
+    if (const unsigned who = __ballot_sync(0xffffffffu, here)) {
+        start.sequence = __shfl_sync(0xffffffffu, start.sequence, __ffs(who) - 1);
+        start.unit = __shfl_sync(0xffffffffu, start.unit, __ffs(who) - 1);
+    }
+    return start;
+}
+// By all threads of the CTA; `found` is for everyone behind the last barrier.
+template <int Columns, int Warps> __device__ __forceinline__ void start_together(const AttentionArgs &a, int segment_units, long long *sums, Start *found) {
+    const int warp = int(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const long long own = work_of_run<Columns>(a, 32 * Warps, int(threadIdx.x));
+    long long before = scan_warp(own, lane);
+    Start start;
+    if (lane == 31) sums[warp] = before;
+    __syncthreads();
+    for (int w = 0; w < Warps; ++w) {
+        if (w < warp) before += sums[w];
+        start.all += sums[w];
+    }
+    if (!threadIdx.x) *found = start; // shares that hold nothing keep this
+    __syncthreads();
+    if (holds_start<Columns>(a, segment_units, 32 * Warps, int(threadIdx.x), before - own, own, start)) *found = start;
+    __syncthreads();
+}
+
+// The part of a segment that a CTA's share holds: tiles [low, high) of `tiles`.
+struct SegmentPart {
+    SequenceShape s;
+    int sequence, head, query_tile, columns, tiles, low, high, ordinal;
+    int first_cta, first_slot; // of all parts, for the CTA that closes a split segment; -1 elsewhere
+    int slot;                  // where a partial sum goes: 0 for a share's first part, 1 for a later one
+    bool split, final;
+};
+// Calls `each` for every part of this CTA's share, in order, until it returns false. Returns the number of parts.
+template <int Columns, class Each>
+__device__ __forceinline__ int walk_share(const AttentionArgs &a, int segment_units, const Start &start, Each &&each) {
+    const Division d(start.all, segment_units);
+    const long long begin = d.share_of(blockIdx.x), end = d.share_of((long long)blockIdx.x + 1);
+    long long at = start.unit;
+    SegmentPart p;
+    p.ordinal = 0;
+    for (p.sequence = start.sequence; begin < end && p.sequence < a.sequences && at < end; ++p.sequence) {
+        p.s = sequence_of(a, p.sequence);
+        const int count = query_tiles<Columns>(a, p.s);
+        int segment = 0;
+        if (begin > at) { // whole heads in front of the share
+            const long long head_units = kTileUnits * head_tiles<Columns>(a, p.s, count) + (long long)d.extra * count;
+            const long long heads = head_units ? min(quotient(begin - at, head_units), (long long)a.kv_heads) : 0;
+            segment = int(heads) * count, at += heads * head_units;
+        }
+        // Heads outermost: their query tiles read the same keys, near one another in time.
+        for (; segment < count * a.kv_heads && at < end; ++segment) {
+            p.head = segment / count, p.query_tile = segment - p.head * count, p.tiles = tiles_of<Columns>(a, p.s, p.query_tile);
+            const long long first_unit = at + d.extra;
+            at = first_unit + (long long)kTileUnits * p.tiles;
+            const auto tile_from = [&](long long unit) { // first tile that starts at or behind a unit
+                return unit <= first_unit ? 0 : unit >= at ? p.tiles : int((unit - first_unit + kTileUnits - 1) / kTileUnits);
+            };
+            p.low = tile_from(begin), p.high = tile_from(end);
+            if (p.low == p.high) continue;
+            p.split = p.low || p.high < p.tiles;
+            p.first_cta = -1, p.first_slot = 0;
+            if (p.split && p.high == p.tiles) { // this CTA closes the segment: it says where its parts lie
+                p.first_cta = d.cta_of(first_unit);
+                p.first_slot = d.share_of(p.first_cta) < first_unit - d.extra ? 1 : 0;
+            }
+            p.slot = first_unit - d.extra > begin ? 1 : 0;
+            p.columns = min(Columns, p.s.count * a.group - p.query_tile * Columns);
+            p.final = p.high < p.tiles || at + d.extra >= end;
+            if (!each(p)) return p.ordinal;
+            ++p.ordinal;
+        }
+    }
+    return p.ordinal;
+}
+
+// One query row's result: the output row, or what is kept of it for the second launch.
+template <class T>
+__device__ __forceinline__ void store_row4(const AttentionArgs &a, T *to, float4 v, float factor) {
+    union {
+        uint2 word;
+        T e[4];
+    } out;
+    out.e[0] = T(v.x * factor), out.e[1] = T(v.y * factor), out.e[2] = T(v.z * factor), out.e[3] = T(v.w * factor);
+    if (a.aligned) {
+        *reinterpret_cast<uint2 *>(to) = out.word;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = out.e[i];
+    }
+}
+
+} // namespace tts::b200

@@ -142,10 +142,10 @@ void cache_read(const CacheView &cache, TensorView slots, TensorView keys, Tenso
     launch_cache_read(cache, slots.ptr<int>(), keys, values, gpu.stream);
 }
 
-size_t cached_attention_workspace(int rows, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors) {
-    if (rows < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128) || multiprocessors < 1)
+size_t cached_attention_workspace(int rows, int sequences, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors) {
+    if (rows < 0 || sequences < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || (head_dim != 64 && head_dim != 128) || multiprocessors < 1)
         refuse("invalid attention shape");
-    return quant_linear_header_bytes() + attention_workspace_bytes(rows, heads, kv_heads, head_dim, prefix, multiprocessors);
+    return quant_linear_header_bytes() + attention_workspace_bytes(rows, sequences, heads, kv_heads, head_dim, prefix, multiprocessors);
 }
 
 void validate_cached_attention(const CacheView &cache, const Attention &a) {
@@ -182,7 +182,7 @@ void cached_attention(const CacheView &cache, const Attention &a) {
     auto &gpu = execution_context(a.queries);
     const int heads = a.queries.cols / cache.head_dim;
     const bool prefix = a.prefix_pages.data != nullptr;
-    const size_t needed = cached_attention_workspace(a.queries.rows, heads, cache.kv_heads, cache.head_dim, prefix, gpu.multiprocessors);
+    const size_t needed = cached_attention_workspace(a.queries.rows, a.pages.rows, heads, cache.kv_heads, cache.head_dim, prefix, gpu.multiprocessors);
     if (!gpu.gemm_workspace.data() || gpu.gemm_workspace.size() < needed)
         throw std::invalid_argument("attention needs a context workspace of " + std::to_string(needed) + " bytes");
     AttentionProblem p;

@@ -50,5 +50,5 @@ struct Attention {
 void cached_attention(const CacheView &cache, const Attention &);
 void validate_cached_attention(const CacheView &cache, const Attention &);
 // Context workspace that cached_attention needs for these shapes. Host only.
-size_t cached_attention_workspace(int rows, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors);
+size_t cached_attention_workspace(int rows, int sequences, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors);
 } // namespace tts::ops

@@ -137,10 +137,11 @@ class Rotary:
         return RotaryPlan(self.turns.data_ptr(), 2 * self.turns.numel(), int(self.interleaved), self.scale, self.turns.device.index)
 
 
-def attention_workspace(rows: int, heads: int, kv_heads: int, head_dim: int, prefix: bool = False, multiprocessors: int = 148) -> int:
+def attention_workspace(rows: int, sequences: int, heads: int, kv_heads: int, head_dim: int, prefix: bool = False,
+                        multiprocessors: int = 148) -> int:
     """Bytes of context workspace that Context.cached_attention needs."""
     needed = C.c_size_t()
-    _lib.call("b200q_attention_workspace", rows, heads, kv_heads, head_dim, int(prefix), multiprocessors, C.byref(needed))
+    _lib.call("b200q_attention_workspace", rows, sequences, heads, kv_heads, head_dim, int(prefix), multiprocessors, C.byref(needed))
     return needed.value
 
 

@@ -230,7 +230,7 @@ typedef struct b200q_attention {
 } b200q_attention;
 int b200q_cached_attention(b200q_context *, const b200q_cache *cache, const b200q_attention *arguments, char *error, size_t error_capacity);
 /* Host only: bytes of context workspace that b200q_cached_attention needs. */
-int b200q_attention_workspace(int32_t rows, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t prefix, int32_t multiprocessors,
+int b200q_attention_workspace(int32_t rows, int32_t sequences, int32_t heads, int32_t kv_heads, int32_t head_dim, int32_t prefix, int32_t multiprocessors,
                               size_t *needed, char *error, size_t error_capacity);
 
 /* ---- Linear layer object --------------------------------------------------------------------
