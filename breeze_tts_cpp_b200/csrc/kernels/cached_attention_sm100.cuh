@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t full[kTeams][kMaxRing], empty[kMaxRing], merge_full[2]; // full: of each team
     __shared__ TileNote notes[kMaxRing], merge_notes[2];
-    __shared__ long long sums[kAttentionWarps];
+    __shared__ Work sums[kAttentionWarps];
     __shared__ Start found;
     __shared__ int abort_flag;
     __shared__ int merged; // parts that the mergers are done with, times kMergers

@@ -5,20 +5,22 @@
 // when a tile's maximum passes it by 2^8, so that the accumulated output is rescaled hardly ever.
 //
 // Layout. A segment is 128 query rows of one cached head (tokens times the group's heads; of a prefix: of all sequences), a tile 128 keys. Per tile
-// a CTA does S = Q K^T and O += P V as tcgen05.mma of 128 x 128 (x 64 or 128), with S, P and O in tensor memory; P overwrites S, two halves to a column. Tiles
-// alternate between two teams of four softmax warps, a thread per query row, and each team has a softmax state and an output of its own: one team's
-// exponentials run under the other's products, and the two meet once per segment. Four warps turn bytes into fp16 operands: keys as they are, values
-// transposed, so that both are K-major with the 128-byte swizzle. Tables of a tile's scales go to the softmax warps through shared memory.
+// a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Tiles alternate between
+// two teams of four softmax warps, a thread per query row, and each team has a softmax state, an output and an issuing warp of its own; the two
+// meet once per segment. A team takes its tile in two halves of 64 keys: while it works on one half, the product of the half before and the scores
+// of the next tile's run. Four warps turn bytes into fp16 operands: keys as they are, values transposed, so that both are K-major with the 128-byte
+// swizzle. Tables of a tile's scales go to the softmax warps through shared memory.
 //
-// Bound. A 128 x 128 x 128 tile costs the tensor pipe 1024 cycles, its exponentials the special-function units 1024, the conversions about
-// 450 issue cycles, so all three have to overlap; what the two teams leave open is the latency from a product to its softmax and back.
+// Bound. A 128 x 128 x 128 tile costs the tensor pipe about 1300 cycles, its exponentials the special-function units 1024, conversions and softmax
+// about 1600 issue cycles, so all of them have to overlap.
 #pragma once
 #include "kernels/cached_attention_sm100.cuh"
 
 namespace tts::b200 {
 constexpr int kManyRows = 128;
 constexpr int kManySegmentUnits = 6; // a segment's queries, the meeting of the teams and the store next to a tile's kTileUnits
-constexpr int kSoftmaxWarps = 8, kConverters = 4, kManyWarps = kSoftmaxWarps + kConverters + 2, kManyThreads = 32 * kManyWarps;
+constexpr int kSoftmaxWarps = 8, kConverters = 4, kManyWarps = kSoftmaxWarps + kConverters + 3, kManyThreads = 32 * kManyWarps;
+constexpr int kPartsAhead = 4;
 constexpr float kReferenceSlack = 8.f; // powers of two that a weight may exceed one by
 
 template <int HeadDim> struct ManyShape {
@@ -49,30 +51,47 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
+__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return ptx::pack2(__uint_as_float(lo), __uint_as_float(hi)); }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 // 16-byte chunk `chunk` of row `row` in a K-major operand panel (rows of 64 halves, 128-byte swizzle).
 __device__ __forceinline__ uint32_t panel_at(int row, int chunk) { return uint32_t(row * 128 + ((chunk ^ (row & 7)) << 4)); }
+template <class T> __device__ __forceinline__ void store_row8(const AttentionArgs &a, T *to, const float (&v)[8], float factor) {
+    union {
+        uint4 words;
+        T e[8];
+    } out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out.e[i] = T(v[i] * factor);
+    if (a.aligned) {
+        *reinterpret_cast<uint4 *>(to) = out.words;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i] = out.e[i];
+    }
+}
 } // namespace many
 
 template <class T, Type F, int HeadDim>
 __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const AttentionArgs args) {
     using namespace many;
     using Shape = ManyShape<HeadDim>;
-    constexpr int kRows = kManyRows, kSlots = Shape::slots, kConverter = kSoftmaxWarps, kProducer = kConverter + kConverters, kIssuer = kProducer + 1;
+    constexpr int kRows = kManyRows, kSlots = Shape::slots, kConverter = kSoftmaxWarps, kProducer = kConverter + kConverters, kIssuer = kProducer + 1; // an issuer per team
     constexpr uint32_t kOut = 2 * kTileKeys; // tensor memory: two teams' scores, then their outputs
     extern __shared__ uint8_t raw_smem[];
-    // Tile i of the share is team i % 2's, and its barriers' use i / 2. scored: S is done (and the keys' buffer free); weighted: O is (and the
-    // values' buffer, the tables and P's place are free); keys/values: operands are ready; softmaxed: P is.
-    __shared__ uint64_t raw_full[kSlots], raw_free[kSlots], keys_ready[2], values_ready[2], scored[2], softmaxed[2], weighted[2];
-    __shared__ uint64_t queries_ready, largest_known, meet, outputs_free, drained; // once per segment part, the last once
+    // Tile i of the share is team i % 2's, and its barriers' use i / 2. Of each half: scored: S is done (of both: the keys' buffer is free);
+    // softmaxed: P is ready; weighted: O has it (of both: the values' buffer and the tables are free). keys/values: operands are ready.
+    __shared__ uint64_t raw_full[kSlots], raw_free[kSlots], keys_ready[2], values_ready[2], scored[2][2], softmaxed[2][2], weighted[2][2];
+    __shared__ uint64_t queries_ready, largest_known, meet, outputs_free, drained[2]; // once per segment part, the last once
     __shared__ __align__(16) float table_key[2][kTileKeys], table_shift[2][kTileKeys], table_value[2][kTileKeys];
     __shared__ float2 stats[2][kRows];
     __shared__ unsigned largest[2]; // of a part's queries, by the part's parity
-    __shared__ long long sums[kManyWarps];
+    __shared__ Work sums[kManyWarps];
     __shared__ Start found;
+    __shared__ SegmentPart parts[kPartsAhead];
+    __shared__ uint64_t part_full[kPartsAhead], part_free[kPartsAhead];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_flag;
     const uint32_t base = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;
@@ -87,16 +106,22 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         for (int t = 0; t < 2; ++t) {
             ptx::mbar_init(ptx::smem_u32(&keys_ready[t]), kConverters);
             ptx::mbar_init(ptx::smem_u32(&values_ready[t]), kConverters);
-            ptx::mbar_init(ptx::smem_u32(&scored[t]), 1);
-            ptx::mbar_init(ptx::smem_u32(&softmaxed[t]), kSoftmaxWarps / 2);
-            ptx::mbar_init(ptx::smem_u32(&weighted[t]), 1);
+            for (int h = 0; h < 2; ++h) {
+                ptx::mbar_init(ptx::smem_u32(&scored[t][h]), 1);
+                ptx::mbar_init(ptx::smem_u32(&softmaxed[t][h]), kSoftmaxWarps / 2);
+                ptx::mbar_init(ptx::smem_u32(&weighted[t][h]), 1);
+            }
+            ptx::mbar_init(ptx::smem_u32(&drained[t]), 1);
             largest[t] = 0;
         }
         ptx::mbar_init(ptx::smem_u32(&queries_ready), kConverters);
         ptx::mbar_init(ptx::smem_u32(&largest_known), kConverters);
         ptx::mbar_init(ptx::smem_u32(&meet), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&outputs_free), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&drained), 1);
+        for (int p = 0; p < kPartsAhead; ++p) {
+            ptx::mbar_init(ptx::smem_u32(&part_full[p]), 1);
+            ptx::mbar_init(ptx::smem_u32(&part_free[p]), kSoftmaxWarps + kConverters + 2);
+        }
         abort_flag = 0;
         ptx::fence_barrier_init();
     }
@@ -119,14 +144,36 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         __syncwarp();
         if (!lane) ptx::mbar_arrive(ptx::smem_u32(&bar));
     };
-    // Every role walks the share for itself.
-    const Start start = args.sequences > kScanAlone ? found : start_alone<kRows>(args, kManySegmentUnits);
+    // The producer walks the share and hands its parts to the others. Calls `each` for every part until it returns false.
+    auto for_parts = [&](auto &&each) {
+        for (int ordinal = 0;; ++ordinal) {
+            const int at = ordinal % kPartsAhead;
+            if (!wait(part_full[at], ordinal / kPartsAhead)) return;
+            const SegmentPart &part = parts[at];
+            if (part.low == part.high || !each(part)) return;
+            arrive(part_free[at]);
+        }
+    };
     int first_tile = 0; // of the part, in the share
 
     if (warp == kProducer) { // ------------------------------------------------------------------ bytes and scales
         const int box = 1 << args.box_shift, boxes = kTileKeys >> args.box_shift;
         int slot = 0, item = 0, reuse = -1; // reuse: the slot's use before this one
-        auto raw_tiles = [&](const SegmentPart &part) {
+        auto publish = [&](const SegmentPart &part) {
+            const int at = part.ordinal % kPartsAhead;
+            if (part.ordinal >= kPartsAhead && !wait(part_free[at], part.ordinal / kPartsAhead - 1)) return false;
+            if (!lane) {
+                parts[at] = part;
+                ptx::mbar_arrive(ptx::smem_u32(&part_full[at]));
+            }
+            __syncwarp();
+            return true;
+        };
+        const Start start = args.sequences > kScanAlone ? found : start_alone<kRows>(args, kManySegmentUnits);
+        bool open = true;
+        SegmentPart nothing{};
+        nothing.ordinal = walk_share<kRows>(args, kManySegmentUnits, start, [&](const SegmentPart &part) {
+            if (!publish(part)) return open = false;
             const int *pages = args.pages + size_t(part.sequence) * args.page_stride;
             for (int tile = part.low; tile < part.high; ++tile) {
                 const int key = tile * kTileKeys, position = key + (lane << args.box_shift);
@@ -136,7 +183,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 const uint32_t held = __ballot_sync(0xffffffffu, good);
                 const int row = (((page * args.kv_heads) + part.head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
                 for (int values = 0; values < 2; ++values, ++item) {
-                    if (reuse >= 0 && !wait(raw_free[slot], reuse)) return false;
+                    if (reuse >= 0 && !wait(raw_free[slot], reuse)) return open = false;
                     const uint32_t to = base + Shape::ring + slot * Shape::raw, bar = ptx::smem_u32(&raw_full[slot]);
                     if (!lane) ptx::mbar_arrive_expect_tx(bar, __popc(held) * box * HeadDim);
                     __syncwarp();
@@ -161,95 +208,106 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 }
             }
             return true;
-        };
-        walk_share<kRows>(args, kManySegmentUnits, start, raw_tiles);
+        });
+        if (open) publish(nothing);
         // No copy may be in flight when the CTA leaves, whatever the others did.
         int ignored = 0;
         for (int i = max(0, item - kSlots); i < item; ++i) ptx::mbar_wait(ptx::smem_u32(&raw_full[i % kSlots]), uint32_t(i / kSlots) & 1, &ignored);
-    } else if (warp == kIssuer) { // -------------------------------------------------------------- products
-        constexpr uint32_t kScoreIdesc = idesc_f16(kRows, kTileKeys), kOutIdesc = idesc_f16(kRows, HeadDim);
-        auto score = [&](int i) { // S of tile i
-            const int team = i & 1;
-            if (!wait(keys_ready[team], i >> 1) || (i >= 2 && !wait(weighted[team], (i >> 1) - 1))) return false;
+    } else if (warp >= kIssuer) { // -------------------------------------------------------------- products
+        constexpr uint32_t kScoreIdesc = idesc_f16(kRows, kTileKeys / 2), kOutIdesc = idesc_f16(kRows, HeadDim);
+        const int team = warp - kIssuer;
+        auto score = [&](int i, int half) { // S of half a tile, where the weights of the team's tile before stood
+            if ((!half && !wait(keys_ready[team], i >> 1)) || (i >= 2 && !wait(weighted[team][half], (i >> 1) - 1))) return false;
             ptx::tcgen05_fence_after();
             if (ptx::elect_one()) {
-                const uint32_t q = ptx::smem_desc_lo_k128(base), k = ptx::smem_desc_lo_k128(base + Shape::keys + team * Shape::operand);
+                const uint32_t q = ptx::smem_desc_lo_k128(base), k = ptx::smem_desc_lo_k128(base + Shape::keys + team * Shape::operand + half * (kTileKeys / 2 * 128));
 #pragma unroll
                 for (int s = 0; s < HeadDim / 16; ++s) {
                     const uint32_t at = uint32_t(s >> 2) * (kRows * 128 >> 4) + uint32_t(s & 3) * 2;
-                    mma_smem(tmem + team * kTileKeys, q + at, k + at, kScoreIdesc, s > 0);
+                    mma_smem(tmem + team * kTileKeys + half * (kTileKeys / 2), q + at, k + at, kScoreIdesc, s > 0);
                 }
-                ptx::tcgen05_commit(ptx::smem_u32(&scored[team]));
+                ptx::tcgen05_commit(ptx::smem_u32(&scored[team][half]));
             }
             __syncwarp();
             return true;
         };
-        walk_share<kRows>(args, kManySegmentUnits, start, [&](const SegmentPart &part) {
-            const int count = part.high - part.low, end = first_tile + count;
-            if (!wait(queries_ready, part.ordinal) || !score(first_tile)) return false;
-            for (int i = first_tile; i < end; ++i) {
-                const int team = i & 1;
-                if (i + 1 < end && !score(i + 1)) return false;
-                if (i == first_tile && part.ordinal && !wait(outputs_free, part.ordinal - 1)) return false;
-                if (!wait(values_ready[team], i >> 1) || !wait(softmaxed[team], i >> 1)) return false;
-                ptx::tcgen05_fence_after();
-                if (ptx::elect_one()) {
-                    const uint32_t v = ptx::smem_desc_lo_k128(base + Shape::values + team * Shape::operand);
+        for_parts([&](const SegmentPart &part) {
+            const int end = first_tile + part.high - part.low, first = first_tile + ((first_tile ^ team) & 1);
+            if (!wait(queries_ready, part.ordinal)) return false;
+            if (first < end && (!score(first, 0) || !score(first, 1))) return false;
+            if (part.ordinal && !wait(outputs_free, part.ordinal - 1)) return false;
+            for (int i = first; i < end; i += 2) {
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    if ((!half && !wait(values_ready[team], i >> 1)) || !wait(softmaxed[team][half], i >> 1)) return false;
+                    ptx::tcgen05_fence_after();
+                    if (ptx::elect_one()) {
+                        const uint32_t v = ptx::smem_desc_lo_k128(base + Shape::values + team * Shape::operand + half * (HeadDim * 128));
 #pragma unroll
-                    for (int s = 0; s < kTileKeys / 16; ++s)
-                        mma_tmem(tmem + kOut + team * HeadDim, tmem + team * kTileKeys + 8 * s,
-                                 v + uint32_t(s >> 2) * (HeadDim * 128 >> 4) + uint32_t(s & 3) * 2, kOutIdesc, s > 0 || i >= first_tile + 2);
-                    ptx::tcgen05_commit(ptx::smem_u32(&weighted[team]));
+                        for (int s = 0; s < kTileKeys / 32; ++s)
+                            mma_tmem(tmem + kOut + team * HeadDim, tmem + team * kTileKeys + half * (kTileKeys / 2) + 8 * s, v + uint32_t(s) * 2, kOutIdesc,
+                                     s > 0 || half || i > first);
+                        ptx::tcgen05_commit(ptx::smem_u32(&weighted[team][half]));
+                    }
+                    __syncwarp();
+                    if (i + 2 < end && !score(i + 2, half)) return false;
                 }
-                __syncwarp();
             }
             first_tile = end;
             return true;
         });
         // No product may be in flight when the tensor memory is given back, whatever the others did.
-        if (ptx::elect_one()) ptx::tcgen05_commit(ptx::smem_u32(&drained));
+        if (ptx::elect_one()) ptx::tcgen05_commit(ptx::smem_u32(&drained[team]));
         __syncwarp();
         int ignored = 0;
-        ptx::mbar_wait(ptx::smem_u32(&drained), 0, &ignored);
+        ptx::mbar_wait(ptx::smem_u32(&drained[team]), 0, &ignored);
     } else if (warp >= kConverter) { // ----------------------------------------------------------- bytes to operands
         const int mine = warp - kConverter, thread = 32 * mine + lane;
         int slot = 0, use = 0;
         auto next_slot = [&] {
             if (++slot == kSlots) slot = 0, ++use;
         };
-        walk_share<kRows>(args, kManySegmentUnits, start, [&](const SegmentPart &part) {
+        for_parts([&](const SegmentPart &part) {
             // Queries, once the products of the part before have read theirs. Rows past the segment are zero. BF16 rows are divided by the power of
             // two of their largest element of all, which brings them into fp16's range; what that costs the small ones is small next to the others.
             for (int i = max(0, first_tile - 2); i < first_tile; ++i)
-                if (!wait(scored[i & 1], i >> 1)) return false;
-            constexpr int kChunks = HeadDim / 8, kTurns = kRows * kChunks / (32 * kConverters);
-            float scale_up = 1.f;
-            uint4 chunk[kTurns];
-            unsigned most = 0;
-#pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-                const int piece = thread + 32 * kConverters * i, row = piece / kChunks, c = piece % kChunks;
-                const int flat = part.query_tile * kRows + row;
-                chunk[i] = make_uint4(0, 0, 0, 0);
-                if (row >= part.columns) continue;
-                const T *from = static_cast<const T *>(args.queries) + size_t(part.s.row + flat / args.group) * args.query_stride +
-                                (part.head * args.group + flat % args.group) * HeadDim + 8 * c;
-                if (args.aligned) {
-                    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(chunk[i].x), "=r"(chunk[i].y), "=r"(chunk[i].z), "=r"(chunk[i].w)
-                                 : "l"(from)
-                                 : "memory");
+                if (!wait(scored[i & 1][1], i >> 1)) return false;
+            constexpr int kChunks = HeadDim / 8, kTurns = kRows * kChunks / (32 * kConverters); // kChunks: threads to a row
+            const int flat = part.query_tile * kRows, chunk = thread % kChunks;
+            const auto place = [&](int i) { // where this thread's piece of turn i goes; rows of a turn are a multiple of eight apart
+                return base + uint32_t(chunk >> 3) * (kRows * 128) + panel_at(thread / kChunks, chunk & 7) + uint32_t(i) * (32 * kConverters / kChunks * 128);
+            };
+            static_assert(32 * kConverters / kChunks % 8 == 0);
+#pragma unroll 1
+            for (int i = 0; i < kTurns; ++i) { // all rows in flight at once, as they are
+                const int row = thread / kChunks + 32 * kConverters / kChunks * i, token = (flat + row) / args.group;
+                const T *at = static_cast<const T *>(args.queries) + size_t(part.s.row + token) * args.query_stride +
+                              (part.head * args.group + flat + row - token * args.group) * HeadDim + 8 * chunk;
+                if (row >= part.columns) {
+                    st_shared16(place(i), 0, 0, 0, 0);
+                } else if (args.aligned) {
+                    copy_async16(place(i), at);
                 } else {
                     uint16_t v[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) asm volatile("ld.global.b16 %0, [%1];" : "=h"(v[e]) : "l"(from + e) : "memory");
-                    chunk[i] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+                    for (int e = 0; e < 8; ++e) asm volatile("ld.global.b16 %0, [%1];" : "=h"(v[e]) : "l"(at + e) : "memory");
+                    st_shared16(place(i), v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
                 }
             }
-            if (std::is_same<T, __nv_bfloat16>::value) {
+            ptx::copy_async_wait_all();
+            float scale_up = 1.f;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                auto load = [&](int i, uint32_t(&w)[4]) {
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place(i)) : "memory");
+                };
+                unsigned most = 0;
+#pragma unroll 4
+                for (int i = 0; i < kTurns; ++i) {
+                    uint32_t w[4];
+                    load(i, w);
 #pragma unroll
-                for (int i = 0; i < kTurns; ++i)
-                    for (const uint32_t w : {chunk[i].x, chunk[i].y, chunk[i].z, chunk[i].w}) most = max(most, max(w << 16 & 0x7fffffffu, w & 0x7fff0000u));
+                    for (int e = 0; e < 4; ++e) most = max(most, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
+                }
                 most = __reduce_max_sync(0xffffffffu, most);
                 if (!lane) atomicMax(&largest[part.ordinal & 1], most);
                 arrive(largest_known);
@@ -258,20 +316,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 const int exponent = most && most < 0x7f800000u ? max(int(most >> 23), 1) - 127 : 0;
                 const float down = __int_as_float(exponent < 127 ? (127 - exponent) << 23 : 0x00400000); // 2^-exponent
                 scale_up = __int_as_float(exponent > -127 ? (127 + exponent) << 23 : 0x00400000);
-#pragma unroll
+#pragma unroll 4
                 for (int i = 0; i < kTurns; ++i) {
-                    uint32_t *w = &chunk[i].x;
+                    uint32_t w[4];
+                    load(i, w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const __half2 v = __floats2half2_rn(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xffff0000u) * down);
                         w[e] = *reinterpret_cast<const uint32_t *>(&v);
                     }
+                    st_shared16(place(i), w[0], w[1], w[2], w[3]);
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < kTurns; ++i) {
-                const int piece = thread + 32 * kConverters * i, row = piece / kChunks, c = piece % kChunks;
-                st_shared16(base + uint32_t(c >> 3) * (kRows * 128) + panel_at(row, c & 7), chunk[i].x, chunk[i].y, chunk[i].z, chunk[i].w);
             }
             ptx::fence_proxy_async_smem();
             arrive(queries_ready);
@@ -280,64 +335,73 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             const float score_scale = args.score_scale * scale_up;
             for (int tile = part.low; tile < part.high; ++tile, ++first_tile) {
                 const int team = first_tile & 1, before = (first_tile >> 1) - 1;
-                if (!wait(raw_full[slot], use) || (before >= 0 && !wait(scored[team], before))) return false;
+                if (!wait(raw_full[slot], use) || (before >= 0 && !wait(scored[team][1], before))) return false;
                 {
                     const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::keys + team * Shape::operand;
-                    constexpr int kPieces = HeadDim / 16; // lanes to a key row
-#pragma unroll 4
-                    for (int i = 0; i < kTileKeys * kPieces / (32 * kConverters); ++i) {
-                        const int piece = thread + 32 * kConverters * i, row = piece / kPieces, c = piece % kPieces;
-                        uint32_t w[4], h[8];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from + row * HeadDim + 16 * c));
+                    constexpr int kPieces = HeadDim / 16, kTurns = kTileKeys * kPieces / (32 * kConverters); // kPieces: lanes to a key row
+                    uint32_t w[kTurns][4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) widen_key<F>(w[e], h[2 * e], h[2 * e + 1]);
-                        const uint32_t panel = to + uint32_t(c >> 2) * (kTileKeys * 128);
-                        // The second panel's lanes store their chunks in the other order: eight lanes then meet eight banks.
-                        const int odd = (c >> 2) & 1;
+                    for (int i = 0; i < kTurns; ++i) // row HeadDim bytes long, so thread t's pieces lie 16 t bytes in and one turn apart
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
+                                     : "r"(from + 16 * (thread + 32 * kConverters * i)));
+                    arrive(raw_free[slot]);
+                    const int c = thread % kPieces, row = thread / kPieces;
+                    // The second panel's lanes store their chunks in the other order: eight lanes then meet eight banks. Rows of a turn are a
+                    // multiple of eight apart, so the swizzle is the same in all of them.
+                    static_assert(32 * kConverters / kPieces % 8 == 0);
+                    const int odd = (c >> 2) & 1;
+                    const uint32_t panel = to + uint32_t(c >> 2) * (kTileKeys * 128), near = panel + panel_at(row, 2 * (c & 3) + odd),
+                                   far = panel + panel_at(row, 2 * (c & 3) + 1 - odd);
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const bool upper = e ^ odd;
-                            st_shared16(panel + panel_at(row, 2 * (c & 3) + upper), upper ? h[4] : h[0], upper ? h[5] : h[1], upper ? h[6] : h[2], upper ? h[7] : h[3]);
-                        }
+                    for (int i = 0; i < kTurns; ++i) {
+                        uint32_t h[8];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) widen_key<F>(odd ? w[i][e ^ 2] : w[i][e], h[2 * e], h[2 * e + 1]);
+                        constexpr uint32_t kApart = 32 * kConverters / kPieces * 128;
+                        st_shared16(near + i * kApart, h[0], h[1], h[2], h[3]);
+                        st_shared16(far + i * kApart, h[4], h[5], h[6], h[7]);
                     }
                 }
                 ptx::fence_proxy_async_smem();
-                arrive(raw_free[slot]);
-                if (!lane) ptx::mbar_arrive(ptx::smem_u32(&keys_ready[team]));
+                arrive(keys_ready[team]);
                 next_slot();
-                if (!wait(raw_full[slot], use) || (before >= 0 && !wait(weighted[team], before))) return false;
+                if (!wait(raw_full[slot], use) || (before >= 0 && !wait(weighted[team][1], before))) return false;
                 {
                     const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::values + team * Shape::operand;
                     const float *scales = reinterpret_cast<const float *>(base_bytes + Shape::ring + slot * Shape::raw + kTileKeys * HeadDim);
                     const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
+                    // A lane takes four columns (a word) of eight keys, and stores eight keys of each column. Pairs of lanes take other groups of keys, so that
+                    // eight lanes meet eight banks when they store.
+                    constexpr int kWords = HeadDim / 4, kSets = 32 * kConverters / kWords, kTurns = kTileKeys / 8 / kSets; // kSets: threads that share a word
+                    const int word = thread % kWords, set = thread / kWords;
+                    const int first = kSets == 4 ? ((word >> 1) + set) & 3 : (((word >> 1) & 3) + set) & 7; // group of keys, kSets apart from turn to turn
+                    uint32_t w[kTurns][8];
+#pragma unroll
+                    for (int i = 0; i < kTurns; ++i)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i][k]) : "r"(from + (8 * (kSets * i + first) + k) * HeadDim + 4 * word));
+                    arrive(raw_free[slot]);
                     table_key[team][thread] = key_scale * score_scale;
                     table_value[team][thread] = value_scale;
                     table_shift[team][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
-                    // A lane takes four columns (a word) of eight keys, and stores eight keys of each column. Pairs of lanes take other groups of keys, so that
-                    // eight lanes meet eight banks when they store.
-                    constexpr int kWords = HeadDim / 4, kGroups = kTileKeys / 8, kSets = 32 * kConverters / kWords; // kSets: threads that share a word
-                    const int word = thread % kWords, set = thread / kWords;
-#pragma unroll 2
-                    for (int i = 0; i < kGroups / kSets; ++i) {
-                        const int group = kSets == 4 ? 4 * i + (((word >> 1) + set) & 3) : 8 * i + ((((word >> 1) & 3) + set) & 7);
-                        uint32_t w[8];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[k]) : "r"(from + (8 * group + k) * HeadDim + 4 * word));
+                    for (int i = 0; i < kTurns; ++i) {
+                        const int group = kSets * i + first;
                         uint32_t h[4][4]; // [column][pair of keys]
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
 #pragma unroll
                             for (int c = 0; c < 2; ++c)
-                                widen<F>(biased<F>(__byte_perm(w[2 * k], w[2 * k + 1], c ? 0x7362u : 0x5140u)), h[2 * c][k], h[2 * c + 1][k]);
+                                widen<F>(biased<F>(__byte_perm(w[i][2 * k], w[i][2 * k + 1], c ? 0x7362u : 0x5140u)), h[2 * c][k], h[2 * c + 1][k]);
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
                             st_shared16(to + uint32_t(group >> 3) * (HeadDim * 128) + panel_at(4 * word + c, group & 7), h[c][0], h[c][1], h[c][2], h[c][3]);
                     }
                 }
                 ptx::fence_proxy_async_smem();
-                arrive(raw_free[slot]);
-                if (!lane) ptx::mbar_arrive(ptx::smem_u32(&values_ready[team]));
+                arrive(values_ready[team]);
                 next_slot();
             }
             return true;
@@ -345,7 +409,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     } else { // ----------------------------------------------------------------------------------- softmax
         const int team = warp >> 2, row = 32 * (warp & 3) + lane;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16, at_scores = tmem + lanes + team * kTileKeys, at_out = tmem + lanes + kOut;
-        walk_share<kRows>(args, kManySegmentUnits, start, [&](const SegmentPart &part) {
+        for_parts([&](const SegmentPart &part) {
             const int count = part.high - part.low, end = first_tile + count, flat = part.query_tile * kRows + row;
             const bool live = row < part.columns;
             const int limit = !live ? -1 : args.prefix ? part.s.length - 1 : part.s.length - part.s.count + flat / args.group;
@@ -353,81 +417,111 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             float most = -INFINITY, sum = 0.f;
             int last = -1;
             for (int i = first_tile + ((first_tile ^ team) & 1); i < end; i += 2) {
-                const int key = (part.low + i - first_tile) * kTileKeys;
-                const bool masked = key + kTileKeys - 1 > least;
-                if (!wait(scored[team], i >> 1) || !wait(values_ready[team], i >> 1)) return false; // the tables come with the values
-                ptx::tcgen05_fence_after();
-                float highest = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < kTileKeys; c += 32) {
-                    uint32_t s[32];
-                    ptx::tmem_load32(at_scores + c, s);
-                    ptx::tmem_load_wait();
+                for (int half = 0; half < 2; ++half) {
+                    constexpr int kHalf = kTileKeys / 2;
+                    const int key = (part.low + i - first_tile) * kTileKeys + half * kHalf;
+                    const uint32_t at = at_scores + half * kHalf;
+                    const float *const of_key = table_key[team] + half * kHalf, *const of_shift = table_shift[team] + half * kHalf,
+                                      *const of_value = table_value[team] + half * kHalf;
+                    const bool masked = key + kHalf - 1 > least;
+                    if (!wait(scored[team][half], i >> 1) || (!half && !wait(values_ready[team], i >> 1))) return false; // the tables come with the values
+                    ptx::tcgen05_fence_after();
+                    // Scores come 32 columns at a time, the next ones on their way while these are worked on.
+                    float highest = -INFINITY;
+                    auto find_highest = [&](auto masked_tile) {
+                        constexpr bool kMasked = decltype(masked_tile)::value;
+                        uint32_t s[2][32];
+                        ptx::tmem_load32(at, s[0]);
+                        float parts[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 k = *reinterpret_cast<const float4 *>(&table_key[team][c + j]), shift = *reinterpret_cast<const float4 *>(&table_shift[team][c + j]);
-                        float t[4];
-                        ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), ptx::pack2(k.x, k.y), ptx::pack2(shift.x, shift.y)), t[0], t[1]);
-                        ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])), ptx::pack2(k.z, k.w), ptx::pack2(shift.z, shift.w)), t[2], t[3]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (!masked || key + c + j + e <= limit) highest = fmaxf(highest, t[e]);
-                    }
-                }
-                const bool raise = highest > most + kReferenceSlack; // also from no reference at all
-                if (__any_sync(0xffffffffu, raise)) {
-                    const float shrink = raise ? exp2_approx(most - highest) : 1.f;
-                    if (raise) most = highest;
-                    sum *= shrink;
-                    if (last >= 0) // this team's output so far; the product that made it is done, or this tile's scores would not be
-#pragma unroll 1
-                        for (int c = 0; c < HeadDim; c += 16) {
-                            uint32_t o[16];
-                            ptx::tmem_load16(at_out + team * HeadDim + c, o);
+                        for (int c = 0; c < kHalf; c += 32) {
                             ptx::tmem_load_wait();
+                            if (c + 32 < kHalf) ptx::tmem_load32(at + c + 32, s[(c / 32 + 1) & 1]);
+                            const uint32_t(&now)[32] = s[(c / 32) & 1];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-                            tmem_store16(at_out + team * HeadDim + c, o);
+                            for (int j = 0; j < 32; j += 4) {
+                                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(of_key + c + j);
+                                const ulonglong2 shift = *reinterpret_cast<const ulonglong2 *>(of_shift + c + j);
+                                float t[4];
+                                ptx::unpack2(ptx::fma2(pair(now[j], now[j + 1]), k.x, shift.x), t[0], t[1]);
+                                ptx::unpack2(ptx::fma2(pair(now[j + 2], now[j + 3]), k.y, shift.y), t[2], t[3]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) parts[e] = fmaxf(parts[e], kMasked && key + c + j + e > limit ? -INFINITY : t[e]);
+                            }
                         }
-                }
-                const float reference = most == -INFINITY ? 0.f : most;
-                const uint64_t minus = ptx::pack2(-reference, -reference);
-                uint64_t total = 0;
+                        highest = fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3]));
+                    };
+                    if (masked) find_highest(std::true_type{});
+                    else find_highest(std::false_type{});
+                    const bool raise = highest > most + kReferenceSlack; // also from no reference at all
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float shrink = raise ? exp2_approx(most - highest) : 1.f;
+                        if (raise) most = highest;
+                        sum *= shrink;
+                        if (last >= 0 || half) { // this team's output so far, once the product before this half is in it
+                            if (!wait(weighted[team][half ^ 1], (half ? i : last) >> 1)) return false;
+                            ptx::tcgen05_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < kTileKeys; c += 32) {
-                    uint32_t s[32], p[16];
-                    ptx::tmem_load32(at_scores + c, s);
-                    ptx::tmem_load_wait();
+                            for (int c = 0; c < HeadDim; c += 16) {
+                                uint32_t o[16];
+                                ptx::tmem_load16(at_out + team * HeadDim + c, o);
+                                ptx::tmem_load_wait();
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 k = *reinterpret_cast<const float4 *>(&table_key[team][c + j]), v = *reinterpret_cast<const float4 *>(&table_value[team][c + j]);
-                        float x[4], w[4];
-                        ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), ptx::pack2(k.x, k.y), minus), x[0], x[1]);
-                        ptx::unpack2(ptx::fma2(ptx::pack2(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])), ptx::pack2(k.z, k.w), minus), x[2], x[3]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) x[e] = masked && key + c + j + e > limit ? 0.f : exp2_approx(x[e]);
-                        const uint64_t low = ptx::pack2(x[0], x[1]), high = ptx::pack2(x[2], x[3]);
-                        total = ptx::add2(total, ptx::add2(low, high));
-                        ptx::unpack2(ptx::mul2(low, ptx::pack2(v.x, v.y)), w[0], w[1]);
-                        ptx::unpack2(ptx::mul2(high, ptx::pack2(v.z, v.w)), w[2], w[3]);
-                        if (masked) // a hidden row's scale may be anything
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) w[e] = key + c + j + e > limit ? 0.f : w[e];
-                        const __half2 a = __floats2half2_rn(w[0], w[1]), b = __floats2half2_rn(w[2], w[3]);
-                        p[j / 2] = *reinterpret_cast<const uint32_t *>(&a), p[j / 2 + 1] = *reinterpret_cast<const uint32_t *>(&b);
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
+                                tmem_store16(at_out + team * HeadDim + c, o);
+                            }
+                        }
                     }
-                    tmem_store16(at_scores + c / 2, p); // over scores that have been read
+                    const float reference = most == -INFINITY ? 0.f : most;
+                    const uint64_t minus = ptx::pack2(-reference, -reference);
+                    uint64_t total = 0;
+                    auto weigh = [&](auto masked_tile) {
+                        constexpr bool kMasked = decltype(masked_tile)::value;
+                        uint32_t s[2][32];
+                        ptx::tmem_load32(at, s[0]);
+#pragma unroll
+                        for (int c = 0; c < kHalf; c += 32) {
+                            ptx::tmem_load_wait();
+                            if (c + 32 < kHalf) ptx::tmem_load32(at + c + 32, s[(c / 32 + 1) & 1]);
+                            const uint32_t(&now)[32] = s[(c / 32) & 1];
+                            uint32_t p[16];
+#pragma unroll
+                            for (int j = 0; j < 32; j += 4) {
+                                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(of_key + c + j);
+                                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(of_value + c + j);
+                                float x[4], w[4];
+                                ptx::unpack2(ptx::fma2(pair(now[j], now[j + 1]), k.x, minus), x[0], x[1]);
+                                ptx::unpack2(ptx::fma2(pair(now[j + 2], now[j + 3]), k.y, minus), x[2], x[3]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) x[e] = exp2_approx(kMasked && key + c + j + e > limit ? -INFINITY : x[e]);
+                                const uint64_t low = ptx::pack2(x[0], x[1]), high = ptx::pack2(x[2], x[3]);
+                                total = ptx::add2(total, ptx::add2(low, high));
+                                ptx::unpack2(ptx::mul2(low, v.x), w[0], w[1]);
+                                ptx::unpack2(ptx::mul2(high, v.y), w[2], w[3]);
+                                if (kMasked) // a hidden row's scale may be anything
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) w[e] = key + c + j + e > limit ? 0.f : w[e];
+                                const __half2 a = __floats2half2_rn(w[0], w[1]), b = __floats2half2_rn(w[2], w[3]);
+                                p[j / 2] = *reinterpret_cast<const uint32_t *>(&a), p[j / 2 + 1] = *reinterpret_cast<const uint32_t *>(&b);
+                            }
+                            // Over scores that have been read: those on their way lie behind these columns.
+                            tmem_store16(at + c / 2, p);
+                        }
+                    };
+                    if (masked) weigh(std::true_type{});
+                    else weigh(std::false_type{});
+                    tmem_store_wait();
+                    float a, b;
+                    ptx::unpack2(total, a, b);
+                    sum += a + b;
+                    ptx::tcgen05_fence_before();
+                    arrive(softmaxed[team][half]);
                 }
-                tmem_store_wait();
-                float a, b;
-                ptx::unpack2(total, a, b);
-                sum += a + b;
-                ptx::tcgen05_fence_before();
-                arrive(softmaxed[team]);
                 last = i;
             }
             if (last >= 0) {
-                if (!wait(weighted[team], last >> 1)) return false;
+                if (!wait(weighted[team][1], last >> 1)) return false;
                 stats[team][row] = make_float2(most, sum);
             }
             arrive(meet);
@@ -465,13 +559,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 ptx::tmem_load_wait();
                 if (!live) continue;
 #pragma unroll
-                for (int j = 0; j < 16; j += 4) {
-                    float v[4];
+                for (int j = 0; j < 16; j += 8) {
+                    float v[8];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = factor[0] * __uint_as_float(o[0][j + e]) + factor[1] * __uint_as_float(o[1][j + e]);
-                    const float4 four = make_float4(v[0], v[1], v[2], v[3]);
-                    if (kept) *reinterpret_cast<float4 *>(kept + c + j) = four;
-                    else store_row4<T>(args, static_cast<T *>(args.output) + at_row * args.output_stride + size_t(head) * HeadDim + c + j, four, scale);
+                    for (int e = 0; e < 8; ++e) v[e] = factor[0] * __uint_as_float(o[0][j + e]) + factor[1] * __uint_as_float(o[1][j + e]);
+                    if (kept) {
+                        *reinterpret_cast<float4 *>(kept + c + j) = make_float4(v[0], v[1], v[2], v[3]);
+                        *reinterpret_cast<float4 *>(kept + c + j + 4) = make_float4(v[4], v[5], v[6], v[7]);
+                    } else {
+                        store_row8(args, static_cast<T *>(args.output) + at_row * args.output_stride + size_t(head) * HeadDim + c + j, v, scale);
+                    }
                 }
             }
             if (live && !team) {

@@ -75,75 +75,75 @@ template <int Columns> __device__ __forceinline__ int query_tiles(const Attentio
     return (s.count * a.group + Columns - 1) / Columns;
 }
 // Tiles of one head of a sequence, over its query tiles.
-template <int Columns> __device__ __forceinline__ long long head_tiles(const AttentionArgs &a, const SequenceShape &s, int count) {
-    if (a.prefix) return (long long)count * tiles_of<Columns>(a, s, 0);
-    long long tiles = 0;
+template <int Columns> __device__ __forceinline__ int head_tiles(const AttentionArgs &a, const SequenceShape &s, int count) {
+    if (a.prefix || count <= 1) return count * tiles_of<Columns>(a, s, 0);
+    int tiles = 0;
     for (int qt = 0; qt < count; ++qt) tiles += tiles_of<Columns>(a, s, qt);
     return tiles;
 }
-// Work of a run of sequences: tiles, and segments in the 24 high bits (the host refuses more), so that one scan adds up both.
-constexpr int kSegmentShift = 40;
-template <int Columns> __device__ __forceinline__ long long work_of(const AttentionArgs &a, int b) {
+// Work of a run of sequences. The host refuses problems of more than kMostTiles, so all of it, in units, fits an int.
+constexpr long long kMostTiles = 1ll << 27;
+struct Work {
+    int tiles = 0, segments = 0;
+};
+template <int Columns> __device__ __forceinline__ Work work_of(const AttentionArgs &a, int b) {
     const SequenceShape s = sequence_of(a, b);
     const int count = query_tiles<Columns>(a, s);
-    return a.kv_heads * (head_tiles<Columns>(a, s, count) + ((long long)count << kSegmentShift));
+    return {a.kv_heads * head_tiles<Columns>(a, s, count), a.kv_heads * count};
 }
-__device__ __forceinline__ long long scan_warp(long long v, int lane) { // inclusive
+__device__ __forceinline__ int scan_warp(int v, int lane) { // inclusive
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, v, d);
+        const int other = __shfl_up_sync(0xffffffffu, v, d);
         if (lane >= d) v += other;
     }
     return v;
 }
-// 64-bit quotients take a hundred cycles, 32-bit ones a fifth; the operands are not negative.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-    return (a | b) >> 32 ? a / b : (long long)(uint32_t(a) / uint32_t(b));
-}
 // Shares are counted in units: kTileUnits for a tile, `segment_units` more for a segment. A tile belongs to the CTA whose share holds its first unit.
 constexpr int kTileUnits = 4;
 struct Division {
-    long long each = 0, rest = 0, ctas = 0; // units per share, shares that have one more, shares
-    int extra = 0;
+    int each = 0, rest = 0, ctas = 0, extra = 0; // units per share, shares that have one more, shares, units of a segment
 
     // Where there is a CTA for every tile, each gets one. A share is never smaller than a tile, so that every CTA between a segment's first and
     // its last has a part of it.
-    __device__ Division(long long all, int segment_units) {
-        const long long tiles = all & ((1ll << kSegmentShift) - 1);
-        ctas = tiles < gridDim.x ? tiles : gridDim.x;
+    __device__ Division(const Work &all, int segment_units) {
+        ctas = min(all.tiles, int(gridDim.x));
         if (!ctas) return;
-        extra = tiles > gridDim.x ? segment_units : 0;
-        const long long total = units(all);
-        each = quotient(total, ctas), rest = total - each * ctas;
+        extra = all.tiles > int(gridDim.x) ? segment_units : 0;
+        const unsigned total = units(all);
+        each = int(total / unsigned(ctas)), rest = int(total) - each * ctas;
     }
-    __device__ long long units(long long work) const { return kTileUnits * (work & ((1ll << kSegmentShift) - 1)) + extra * (work >> kSegmentShift); }
-    __device__ long long share_of(long long cta) const { return each * min(cta, ctas) + min(min(cta, ctas), rest); } // its first unit
-    __device__ int cta_of(long long unit) const {
-        const long long larger = rest * (each + 1);
-        return int(unit < larger ? quotient(unit, each + 1) : rest + quotient(unit - larger, each));
+    __device__ int units(const Work &work) const { return kTileUnits * work.tiles + extra * work.segments; }
+    __device__ int share_of(int cta) const { return each * min(cta, ctas) + min(min(cta, ctas), rest); } // its first unit
+    __device__ int cta_of(int unit) const {
+        const int larger = rest * (each + 1);
+        return unit < larger ? int(unsigned(unit) / unsigned(each + 1)) : rest + int(unsigned(unit - larger) / unsigned(each));
     }
 };
 // Where a CTA's share begins: the sequence, and that sequence's first unit.
 struct Start {
-    long long all = 0, unit = 0;
-    int sequence = 0;
+    Work all;
+    int unit = 0, sequence = 0;
 };
-template <int Columns> __device__ __forceinline__ long long work_of_run(const AttentionArgs &a, int threads, int thread) {
+template <int Columns> __device__ __forceinline__ Work work_of_run(const AttentionArgs &a, int threads, int thread) {
     const int run = (a.sequences + threads - 1) / threads, from = min(a.sequences, thread * run), to = min(a.sequences, from + run);
-    long long own = 0;
-    for (int b = from; b < to; ++b) own += work_of<Columns>(a, b);
+    Work own;
+    for (int b = from; b < to; ++b) {
+        const Work w = work_of<Columns>(a, b);
+        own.tiles += w.tiles, own.segments += w.segments;
+    }
     return own;
 }
-// Whether this thread's run of sequences, with `base` in front of it, holds the start of the CTA's share.
+// Whether this thread's run of sequences, `own` with `base` in front of it, holds the start of the CTA's share.
 template <int Columns>
-__device__ __forceinline__ bool holds_start(const AttentionArgs &a, int segment_units, int threads, int thread, long long base, long long own, Start &start) {
+__device__ __forceinline__ bool holds_start(const AttentionArgs &a, int segment_units, int threads, int thread, const Work &base, const Work &own, Start &start) {
     const Division d(start.all, segment_units);
-    const long long begin = d.share_of(blockIdx.x);
-    if (blockIdx.x >= d.ctas || d.units(base) > begin || begin >= d.units(base + own)) return false;
+    const int begin = d.share_of(blockIdx.x);
+    if (int(blockIdx.x) >= d.ctas || d.units(base) > begin || begin >= d.units(base) + d.units(own)) return false;
     const int run = (a.sequences + threads - 1) / threads, to = min(a.sequences, thread * run + run);
     start.unit = d.units(base);
-    for (start.sequence = thread * run; start.sequence < to; ++start.sequence) {
-        const long long part = d.units(work_of<Columns>(a, start.sequence));
+    for (start.sequence = thread * run; start.sequence + 1 < to; ++start.sequence) {
+        const int part = d.units(work_of<Columns>(a, start.sequence));
         if (begin < start.unit + part) break;
         start.unit += part;
     }
@@ -152,10 +152,11 @@ __device__ __forceinline__ bool holds_start(const AttentionArgs &a, int segment_
 // By one warp, for a batch of up to kScanAlone sequences.
 template <int Columns> __device__ __forceinline__ Start start_alone(const AttentionArgs &a, int segment_units) {
     const int lane = threadIdx.x & 31;
-    const long long own = work_of_run<Columns>(a, 32, lane), through = scan_warp(own, lane);
+    const Work own = work_of_run<Columns>(a, 32, lane);
+    const Work through{scan_warp(own.tiles, lane), scan_warp(own.segments, lane)};
     Start start;
-    start.all = __shfl_sync(0xffffffffu, through, 31);
-    const bool here = holds_start<Columns>(a, segment_units, 32, lane, through - own, own, start);
+    start.all = {__shfl_sync(0xffffffffu, through.tiles, 31), __shfl_sync(0xffffffffu, through.segments, 31)};
+    const bool here = holds_start<Columns>(a, segment_units, 32, lane, {through.tiles - own.tiles, through.segments - own.segments}, own, start);
     if (const unsigned who = __ballot_sync(0xffffffffu, here)) {
         start.sequence = __shfl_sync(0xffffffffu, start.sequence, __ffs(who) - 1);
         start.unit = __shfl_sync(0xffffffffu, start.unit, __ffs(who) - 1);
@@ -163,20 +164,21 @@ template <int Columns> __device__ __forceinline__ Start start_alone(const Attent
     return start;
 }
 // By all threads of the CTA; `found` is for everyone behind the last barrier.
-template <int Columns, int Warps> __device__ __forceinline__ void start_together(const AttentionArgs &a, int segment_units, long long *sums, Start *found) {
+template <int Columns, int Warps> __device__ __forceinline__ void start_together(const AttentionArgs &a, int segment_units, Work *sums, Start *found) {
     const int warp = int(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const long long own = work_of_run<Columns>(a, 32 * Warps, int(threadIdx.x));
-    long long before = scan_warp(own, lane);
+    const Work own = work_of_run<Columns>(a, 32 * Warps, int(threadIdx.x));
+    Work before{scan_warp(own.tiles, lane), scan_warp(own.segments, lane)};
     Start start;
     if (lane == 31) sums[warp] = before;
     __syncthreads();
     for (int w = 0; w < Warps; ++w) {
-        if (w < warp) before += sums[w];
-        start.all += sums[w];
+        if (w < warp) before.tiles += sums[w].tiles, before.segments += sums[w].segments;
+        start.all.tiles += sums[w].tiles, start.all.segments += sums[w].segments;
     }
+    before.tiles -= own.tiles, before.segments -= own.segments;
     if (!threadIdx.x) *found = start; // shares that hold nothing keep this
     __syncthreads();
-    if (holds_start<Columns>(a, segment_units, 32 * Warps, int(threadIdx.x), before - own, own, start)) *found = start;
+    if (holds_start<Columns>(a, segment_units, 32 * Warps, int(threadIdx.x), before, own, start)) *found = start;
     __syncthreads();
 }
 
@@ -192,8 +194,8 @@ struct SegmentPart {
 template <int Columns, class Each>
 __device__ __forceinline__ int walk_share(const AttentionArgs &a, int segment_units, const Start &start, Each &&each) {
     const Division d(start.all, segment_units);
-    const long long begin = d.share_of(blockIdx.x), end = d.share_of((long long)blockIdx.x + 1);
-    long long at = start.unit;
+    const int begin = d.share_of(blockIdx.x), end = d.share_of(int(blockIdx.x) + 1);
+    int at = start.unit;
     SegmentPart p;
     p.ordinal = 0;
     for (p.sequence = start.sequence; begin < end && p.sequence < a.sequences && at < end; ++p.sequence) {
@@ -201,17 +203,17 @@ __device__ __forceinline__ int walk_share(const AttentionArgs &a, int segment_un
         const int count = query_tiles<Columns>(a, p.s);
         int segment = 0;
         if (begin > at) { // whole heads in front of the share
-            const long long head_units = kTileUnits * head_tiles<Columns>(a, p.s, count) + (long long)d.extra * count;
-            const long long heads = head_units ? min(quotient(begin - at, head_units), (long long)a.kv_heads) : 0;
-            segment = int(heads) * count, at += heads * head_units;
+            const int head_units = kTileUnits * head_tiles<Columns>(a, p.s, count) + d.extra * count;
+            const int heads = head_units ? min(int(unsigned(begin - at) / unsigned(head_units)), a.kv_heads) : 0;
+            segment = heads * count, at += heads * head_units;
         }
         // Heads outermost: their query tiles read the same keys, near one another in time.
         for (; segment < count * a.kv_heads && at < end; ++segment) {
-            p.head = segment / count, p.query_tile = segment - p.head * count, p.tiles = tiles_of<Columns>(a, p.s, p.query_tile);
-            const long long first_unit = at + d.extra;
-            at = first_unit + (long long)kTileUnits * p.tiles;
-            const auto tile_from = [&](long long unit) { // first tile that starts at or behind a unit
-                return unit <= first_unit ? 0 : unit >= at ? p.tiles : int((unit - first_unit + kTileUnits - 1) / kTileUnits);
+            p.head = count == 1 ? segment : segment / count, p.query_tile = segment - p.head * count, p.tiles = tiles_of<Columns>(a, p.s, p.query_tile);
+            const int first_unit = at + d.extra;
+            at = first_unit + kTileUnits * p.tiles;
+            const auto tile_from = [&](int unit) { // first tile that starts at or behind a unit
+                return unit <= first_unit ? 0 : unit >= at ? p.tiles : (unit - first_unit + kTileUnits - 1) / kTileUnits;
             };
             p.low = tile_from(begin), p.high = tile_from(end);
             if (p.low == p.high) continue;

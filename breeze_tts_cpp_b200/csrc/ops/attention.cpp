@@ -169,9 +169,10 @@ void validate_cached_attention(const CacheView &cache, const Attention &a) {
             refuse("prefix pages must be int32 [1, pages]");
         check_index(a.prefix_length, 1, "the prefix length is one int32");
     }
-    // Segments (a sequence, a cached head, a tile of at least eight query rows) are counted in 24 bits on the device.
-    const int64_t group = heads / cache.kv_heads, segments = (int64_t(a.queries.rows) * group / 8 + std::max(a.pages.rows, 1)) * cache.kv_heads;
-    if (segments >= int64_t(1) << 24) refuse("too many query rows");
+    // The device counts tiles of 128 keys, per sequence, cached head and tile of at least eight query rows, in 32 bits.
+    const int64_t group = heads / cache.kv_heads, segments = (int64_t(a.queries.rows) * group / 8 + a.pages.rows) * cache.kv_heads;
+    const int64_t longest = (int64_t(std::max(a.pages.cols, a.prefix_pages.cols)) * cache.page_size + 127) / 128;
+    if (segments * longest > int64_t(1) << 27) refuse("too many query rows for tables of this size");
     if (!std::isfinite(a.scale)) refuse("attention scale is not finite");
     if (cache.overlaps(a.output)) refuse("attention output overlaps the cache");
     for (const TensorView &v : {a.queries, a.pages, a.lengths, a.query_offsets, a.prefix_pages, a.prefix_length})
