@@ -8,7 +8,7 @@
 // a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Tiles alternate between
 // two teams of four softmax warps, a thread per query row, and each team has a softmax state, an output and an issuing warp of its own; the two
 // meet once per segment. A team takes its tile in two halves of 64 keys: while it works on one half, the product of the half before and the scores
-// of the next tile's run. Four warps turn bytes into fp16 operands: keys as they are, values transposed, so that both are K-major with the 128-byte
+// of the next tile's run. Eight warps turn bytes into fp16 operands: keys as they are, values transposed, so that both are K-major with the 128-byte
 // swizzle. Tables of a tile's scales go to the softmax warps through shared memory.
 //
 // Bound. A 128 x 128 x 128 tile costs the tensor pipe about 1300 cycles, its exponentials the special-function units 1024, conversions and softmax
@@ -19,7 +19,11 @@
 namespace tts::b200 {
 constexpr int kManyRows = 128;
 constexpr int kManySegmentUnits = 6; // a segment's queries, the meeting of the teams and the store next to a tile's kTileUnits
-constexpr int kSoftmaxWarps = 8, kConverters = 4, kManyWarps = kSoftmaxWarps + kConverters + 3, kManyThreads = 32 * kManyWarps;
+constexpr int kSoftmaxWarps = 8, kConverters = 8, kManyWarps = kSoftmaxWarps + kConverters + 4, kManyThreads = 32 * kManyWarps; // one warp idles
+// Registers a thread: 96 at launch (61440 in all); two groups of four warps each for the softmax and the conversions, one for the rest. The
+// shares add up to the launch's: 256 x 144 + 256 x 64 + 128 x 64.
+constexpr int kSoftmaxRegisters = 144, kOtherRegisters = 64;
+static_assert(32 * kSoftmaxWarps * kSoftmaxRegisters + (kManyThreads - 32 * kSoftmaxWarps) * kOtherRegisters == kManyThreads * 96);
 constexpr int kPartsAhead = 4;
 constexpr float kReferenceSlack = 8.f; // powers of two that a weight may exceed one by
 
@@ -52,6 +56,8 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
                  : "memory");
 }
 __device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return ptx::pack2(__uint_as_float(lo), __uint_as_float(hi)); }
+template <int Registers> __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Registers)); }
+template <int Registers> __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Registers)); }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -156,6 +162,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     };
     int first_tile = 0; // of the part, in the share
 
+    if (warp < kSoftmaxWarps) take_registers<kSoftmaxRegisters>();
+    else give_registers<kOtherRegisters>();
     if (warp == kProducer) { // ------------------------------------------------------------------ bytes and scales
         const int box = 1 << args.box_shift, boxes = kTileKeys >> args.box_shift;
         int slot = 0, item = 0, reuse = -1; // reuse: the slot's use before this one
@@ -213,7 +221,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         // No copy may be in flight when the CTA leaves, whatever the others did.
         int ignored = 0;
         for (int i = max(0, item - kSlots); i < item; ++i) ptx::mbar_wait(ptx::smem_u32(&raw_full[i % kSlots]), uint32_t(i / kSlots) & 1, &ignored);
-    } else if (warp >= kIssuer) { // -------------------------------------------------------------- products
+    } else if (warp == kIssuer || warp == kIssuer + 1) { // -------------------------------------------------------------- products
         constexpr uint32_t kScoreIdesc = idesc_f16(kRows, kTileKeys / 2), kOutIdesc = idesc_f16(kRows, HeadDim);
         const int team = warp - kIssuer;
         auto score = [&](int i, int half) { // S of half a tile, where the weights of the team's tile before stood
@@ -261,7 +269,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         __syncwarp();
         int ignored = 0;
         ptx::mbar_wait(ptx::smem_u32(&drained[team]), 0, &ignored);
-    } else if (warp >= kConverter) { // ----------------------------------------------------------- bytes to operands
+    } else if (warp >= kConverter && warp < kProducer) { // ----------------------------------------------------------- bytes to operands
         const int mine = warp - kConverter, thread = 32 * mine + lane;
         int slot = 0, use = 0;
         auto next_slot = [&] {
@@ -370,22 +378,25 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 {
                     const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::values + team * Shape::operand;
                     const float *scales = reinterpret_cast<const float *>(base_bytes + Shape::ring + slot * Shape::raw + kTileKeys * HeadDim);
-                    const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
                     // A lane takes four columns (a word) of eight keys, and stores eight keys of each column. Pairs of lanes take other groups of keys, so that
                     // eight lanes meet eight banks when they store.
                     constexpr int kWords = HeadDim / 4, kSets = 32 * kConverters / kWords, kTurns = kTileKeys / 8 / kSets; // kSets: threads that share a word
                     const int word = thread % kWords, set = thread / kWords;
-                    const int first = kSets == 4 ? ((word >> 1) + set) & 3 : (((word >> 1) & 3) + set) & 7; // group of keys, kSets apart from turn to turn
+                    const int first = (set & ~7) | ((((word >> 1) & 3) + set) & 7); // group of keys, kSets apart from turn to turn
+                    static_assert(kSets % 8 == 0);
                     uint32_t w[kTurns][8];
 #pragma unroll
                     for (int i = 0; i < kTurns; ++i)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
                             asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i][k]) : "r"(from + (8 * (kSets * i + first) + k) * HeadDim + 4 * word));
+                    if (thread < kTileKeys) {
+                        const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
+                        table_key[team][thread] = key_scale * score_scale;
+                        table_value[team][thread] = value_scale;
+                        table_shift[team][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
+                    }
                     arrive(raw_free[slot]);
-                    table_key[team][thread] = key_scale * score_scale;
-                    table_value[team][thread] = value_scale;
-                    table_shift[team][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
 #pragma unroll
                     for (int i = 0; i < kTurns; ++i) {
                         const int group = kSets * i + first;
@@ -406,7 +417,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             }
             return true;
         });
-    } else { // ----------------------------------------------------------------------------------- softmax
+    } else if (warp < kSoftmaxWarps) { // --------------------------------------------------------- softmax
         const int team = warp >> 2, row = 32 * (warp & 3) + lane;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16, at_scores = tmem + lanes + team * kTileKeys, at_out = tmem + lanes + kOut;
         for_parts([&](const SegmentPart &part) {
