@@ -6,7 +6,7 @@
 //
 // Layout. A segment is 128 query rows of one cached head (tokens times the group's heads; of a prefix: of all sequences), a tile 128 keys. Per tile
 // a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Tiles alternate between
-// two teams of four softmax warps, a thread per query row, and each team has a softmax state, an output and an issuing warp of its own; the two
+// two teams of four softmax warps, 32 rows a warp, and each team has a softmax state, an output and an issuing warp of its own; the two
 // meet once per segment. A team takes its tile in two halves of 64 keys: while it works on one half, the product of the half before and the scores
 // of the next tile's run. Eight warps turn bytes into fp16 operands: keys as they are, values transposed, so that both are K-major with the 128-byte
 // swizzle. Tables of a tile's scales go to the softmax warps through shared memory.
@@ -55,6 +55,12 @@ __device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
+// 16 lanes x 16 columns from a matrix fragment: lane l holds rows l / 4 (r[2j]) and l / 4 + 8 (r[2j + 1]), column 4j + l % 4.
+__device__ __forceinline__ void tmem_store_rows16(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return ptx::pack2(__uint_as_float(lo), __uint_as_float(hi)); }
 template <int Registers> __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Registers)); }
 template <int Registers> __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Registers)); }
@@ -90,7 +96,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     // Tile i of the share is team i % 2's, and its barriers' use i / 2. Of each half: scored: S is done (of both: the keys' buffer is free);
     // softmaxed: P is ready; weighted: O has it (of both: the values' buffer and the tables are free). keys/values: operands are ready.
     __shared__ uint64_t raw_full[kSlots], raw_free[kSlots], keys_ready[2], values_ready[2], scored[2][2], softmaxed[2][2], weighted[2][2];
-    __shared__ uint64_t queries_ready, largest_known, meet, outputs_free, drained[2]; // once per segment part, the last once
+    __shared__ uint64_t largest_known, meet, drained[2]; // once per segment part, the last once
+    // Warps that have laid down a part's queries, or read its outputs, over all parts. Counts and not phases: an issuer whose team has no tile in some
+    // parts may be several of them behind.
+    __shared__ int queries_ready, outputs_free;
     __shared__ __align__(16) float table_key[2][kTileKeys], table_shift[2][kTileKeys], table_value[2][kTileKeys];
     __shared__ float2 stats[2][kRows];
     __shared__ unsigned largest[2]; // of a part's queries, by the part's parity
@@ -120,15 +129,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             ptx::mbar_init(ptx::smem_u32(&drained[t]), 1);
             largest[t] = 0;
         }
-        ptx::mbar_init(ptx::smem_u32(&queries_ready), kConverters);
         ptx::mbar_init(ptx::smem_u32(&largest_known), kConverters);
         ptx::mbar_init(ptx::smem_u32(&meet), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&outputs_free), kSoftmaxWarps);
         for (int p = 0; p < kPartsAhead; ++p) {
             ptx::mbar_init(ptx::smem_u32(&part_full[p]), 1);
             ptx::mbar_init(ptx::smem_u32(&part_free[p]), kSoftmaxWarps + kConverters + 2);
         }
-        abort_flag = 0;
+        abort_flag = queries_ready = outputs_free = 0;
         ptx::fence_barrier_init();
     }
     if (warp == kIssuer) ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
@@ -145,6 +152,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         if (__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar), uint32_t(use) & 1, &abort_flag))) return true;
         if (!lane) *args.status = 1;
         return false;
+    };
+    auto wait_count = [&](int &count, int needed) {
+        bool reached = false;
+        const long long begun = clock64();
+        while (!(reached = *const_cast<volatile int *>(&count) >= needed) && !*const_cast<volatile int *>(&abort_flag))
+            if (clock64() - begun > ptx::kWaitLimitCycles) abort_flag = 1;
+        reached = __all_sync(0xffffffffu, reached);
+        __threadfence_block();
+        if (!reached && !lane) *args.status = 1;
+        return reached;
+    };
+    auto add_count = [&](int &count) {
+        __syncwarp();
+        if (!lane) {
+            __threadfence_block();
+            atomicAdd(&count, 1);
+        }
     };
     auto arrive = [&](uint64_t &bar) {
         __syncwarp();
@@ -241,9 +265,9 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         };
         for_parts([&](const SegmentPart &part) {
             const int end = first_tile + part.high - part.low, first = first_tile + ((first_tile ^ team) & 1);
-            if (!wait(queries_ready, part.ordinal)) return false;
+            if (!wait_count(queries_ready, kConverters * (part.ordinal + 1))) return false;
             if (first < end && (!score(first, 0) || !score(first, 1))) return false;
-            if (part.ordinal && !wait(outputs_free, part.ordinal - 1)) return false;
+            if (!wait_count(outputs_free, kSoftmaxWarps * part.ordinal)) return false;
             for (int i = first; i < end; i += 2) {
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
@@ -337,7 +361,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 }
             }
             ptx::fence_proxy_async_smem();
-            arrive(queries_ready);
+            add_count(queries_ready);
             if (thread == 0) largest[~part.ordinal & 1] = 0; // everyone has read the part before's
 
             const float score_scale = args.score_scale * scale_up;
@@ -418,58 +442,82 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             return true;
         });
     } else if (warp < kSoftmaxWarps) { // --------------------------------------------------------- softmax
-        const int team = warp >> 2, row = 32 * (warp & 3) + lane;
+        // Scores are read as matrix fragments: lane l has rows l / 4 + 8 r of the warp's 32 and of each eight columns the two at 2 (l % 4), so that a
+        // thread needs a quarter of the columns' scales. With a row per thread every scale went to every thread, and the shared memory's bandwidth, which
+        // the products' operands need, was what a tile waited for.
+        const int team = warp >> 2, row = 32 * (warp & 3) + lane, g = lane >> 2, t = lane & 3;
         const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16, at_scores = tmem + lanes + team * kTileKeys, at_out = tmem + lanes + kOut;
         for_parts([&](const SegmentPart &part) {
             const int count = part.high - part.low, end = first_tile + count, flat = part.query_tile * kRows + row;
             const bool live = row < part.columns;
-            const int limit = !live ? -1 : args.prefix ? part.s.length - 1 : part.s.length - part.s.count + flat / args.group;
-            const int least = __reduce_min_sync(0xffffffffu, live ? limit : INT_MAX);
-            float most = -INFINITY, sum = 0.f;
+            int limit[4], least = INT_MAX; // the last position that a row sees
+            float most[4], sum[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int its_row = 32 * (warp & 3) + 8 * r + g, token = (part.query_tile * kRows + its_row) / args.group;
+                limit[r] = its_row >= part.columns ? -1 : args.prefix ? part.s.length - 1 : part.s.length - part.s.count + token;
+                if (its_row < part.columns) least = min(least, limit[r]);
+                most[r] = -INFINITY, sum[r] = 0.f;
+            }
+            least = __reduce_min_sync(0xffffffffu, least);
             int last = -1;
             for (int i = first_tile + ((first_tile ^ team) & 1); i < end; i += 2) {
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) {
                     constexpr int kHalf = kTileKeys / 2;
-                    const int key = (part.low + i - first_tile) * kTileKeys + half * kHalf;
+                    const int key = (part.low + i - first_tile) * kTileKeys + half * kHalf + 2 * t;
                     const uint32_t at = at_scores + half * kHalf;
-                    const float *const of_key = table_key[team] + half * kHalf, *const of_shift = table_shift[team] + half * kHalf,
-                                      *const of_value = table_value[team] + half * kHalf;
-                    const bool masked = key + kHalf - 1 > least;
+                    const float *const of_key = table_key[team] + half * kHalf + 2 * t, *const of_shift = table_shift[team] + half * kHalf + 2 * t,
+                                      *const of_value = table_value[team] + half * kHalf + 2 * t;
+                    const bool masked = key - 2 * t + kHalf - 1 > least;
                     if (!wait(scored[team][half], i >> 1) || (!half && !wait(values_ready[team], i >> 1))) return false; // the tables come with the values
                     ptx::tcgen05_fence_after();
-                    // Scores come 32 columns at a time, the next ones on their way while these are worked on.
-                    float highest = -INFINITY;
+                    // 32 columns of 32 rows at a time. Having the next ones on their way meanwhile spills, and the other team's warp fills the gap.
+                    auto load = [&](int c, uint32_t(&s)[2][16]) {
+                        ptx::tmem_load_rows16<32>(at + c, s[0]);
+                        ptx::tmem_load_rows16<32>(at + c + (16u << 16), s[1]);
+                    };
+                    float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     auto find_highest = [&](auto masked_tile) {
                         constexpr bool kMasked = decltype(masked_tile)::value;
-                        uint32_t s[2][32];
-                        ptx::tmem_load32(at, s[0]);
-                        float parts[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < kHalf; c += 32) {
+                            uint32_t now[2][16];
+                            load(c, now);
                             ptx::tmem_load_wait();
-                            if (c + 32 < kHalf) ptx::tmem_load32(at + c + 32, s[(c / 32 + 1) & 1]);
-                            const uint32_t(&now)[32] = s[(c / 32) & 1];
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) {
-                                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(of_key + c + j);
-                                const ulonglong2 shift = *reinterpret_cast<const ulonglong2 *>(of_shift + c + j);
-                                float t[4];
-                                ptx::unpack2(ptx::fma2(pair(now[j], now[j + 1]), k.x, shift.x), t[0], t[1]);
-                                ptx::unpack2(ptx::fma2(pair(now[j + 2], now[j + 3]), k.y, shift.y), t[2], t[3]);
+                            for (int j = 0; j < 4; ++j) {
+                                const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), shift = *reinterpret_cast<const uint64_t *>(of_shift + c + 8 * j);
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) parts[e] = fmaxf(parts[e], kMasked && key + c + j + e > limit ? -INFINITY : t[e]);
+                                for (int r = 0; r < 4; ++r) {
+                                    float x, y;
+                                    ptx::unpack2(ptx::fma2(pair(now[r >> 1][4 * j + 2 * (r & 1)], now[r >> 1][4 * j + 2 * (r & 1) + 1]), k, shift), x, y);
+                                    if (kMasked && key + c + 8 * j > limit[r]) x = -INFINITY;
+                                    if (kMasked && key + c + 8 * j + 1 > limit[r]) y = -INFINITY;
+                                    highest[r] = fmaxf(highest[r], fmaxf(x, y));
+                                }
                             }
                         }
-                        highest = fmaxf(fmaxf(parts[0], parts[1]), fmaxf(parts[2], parts[3]));
                     };
                     if (masked) find_highest(std::true_type{});
                     else find_highest(std::false_type{});
-                    const bool raise = highest > most + kReferenceSlack; // also from no reference at all
+                    bool raise = false; // also from no reference at all
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 1));
+                        highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 2));
+                        raise |= highest[r] > most[r] + kReferenceSlack;
+                    }
                     if (__any_sync(0xffffffffu, raise)) {
-                        const float shrink = raise ? exp2_approx(most - highest) : 1.f;
-                        if (raise) most = highest;
-                        sum *= shrink;
+                        float shrink = 1.f; // of row `lane`
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const bool its = highest[r] > most[r] + kReferenceSlack;
+                            const float factor = its ? exp2_approx(most[r] - highest[r]) : 1.f, other = __shfl_sync(0xffffffffu, factor, 4 * (lane & 7));
+                            if (lane >> 3 == r) shrink = other;
+                            if (its) most[r] = highest[r];
+                            sum[r] *= factor;
+                        }
                         if (last >= 0 || half) { // this team's output so far, once the product before this half is in it
                             if (!wait(weighted[team][half ^ 1], (half ? i : last) >> 1)) return false;
                             ptx::tcgen05_fence_after();
@@ -484,48 +532,51 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                             }
                         }
                     }
-                    const float reference = most == -INFINITY ? 0.f : most;
-                    const uint64_t minus = ptx::pack2(-reference, -reference);
-                    uint64_t total = 0;
+                    uint64_t minus[4], total[4] = {};
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float reference = most[r] == -INFINITY ? 0.f : most[r];
+                        minus[r] = ptx::pack2(-reference, -reference);
+                    }
                     auto weigh = [&](auto masked_tile) {
                         constexpr bool kMasked = decltype(masked_tile)::value;
-                        uint32_t s[2][32];
-                        ptx::tmem_load32(at, s[0]);
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < kHalf; c += 32) {
+                            uint32_t now[2][16];
+                            load(c, now);
                             ptx::tmem_load_wait();
-                            if (c + 32 < kHalf) ptx::tmem_load32(at + c + 32, s[(c / 32 + 1) & 1]);
-                            const uint32_t(&now)[32] = s[(c / 32) & 1];
-                            uint32_t p[16];
+                            uint32_t p[2][8];
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4) {
-                                const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(of_key + c + j);
-                                const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(of_value + c + j);
-                                float x[4], w[4];
-                                ptx::unpack2(ptx::fma2(pair(now[j], now[j + 1]), k.x, minus), x[0], x[1]);
-                                ptx::unpack2(ptx::fma2(pair(now[j + 2], now[j + 3]), k.y, minus), x[2], x[3]);
+                            for (int j = 0; j < 4; ++j) {
+                                const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), v = *reinterpret_cast<const uint64_t *>(of_value + c + 8 * j);
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) x[e] = exp2_approx(kMasked && key + c + j + e > limit ? -INFINITY : x[e]);
-                                const uint64_t low = ptx::pack2(x[0], x[1]), high = ptx::pack2(x[2], x[3]);
-                                total = ptx::add2(total, ptx::add2(low, high));
-                                ptx::unpack2(ptx::mul2(low, v.x), w[0], w[1]);
-                                ptx::unpack2(ptx::mul2(high, v.y), w[2], w[3]);
-                                if (kMasked) // a hidden row's scale may be anything
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e) w[e] = key + c + j + e > limit ? 0.f : w[e];
-                                const __half2 a = __floats2half2_rn(w[0], w[1]), b = __floats2half2_rn(w[2], w[3]);
-                                p[j / 2] = *reinterpret_cast<const uint32_t *>(&a), p[j / 2 + 1] = *reinterpret_cast<const uint32_t *>(&b);
+                                for (int r = 0; r < 4; ++r) {
+                                    float x, y;
+                                    ptx::unpack2(ptx::fma2(pair(now[r >> 1][4 * j + 2 * (r & 1)], now[r >> 1][4 * j + 2 * (r & 1) + 1]), k, minus[r]), x, y);
+                                    const bool hide_x = kMasked && key + c + 8 * j > limit[r], hide_y = kMasked && key + c + 8 * j + 1 > limit[r];
+                                    const uint64_t both = ptx::pack2(exp2_approx(hide_x ? -INFINITY : x), exp2_approx(hide_y ? -INFINITY : y));
+                                    total[r] = ptx::add2(total[r], both);
+                                    ptx::unpack2(ptx::mul2(both, v), x, y);
+                                    if (hide_x) x = 0.f; // a hidden row's scale may be anything
+                                    if (hide_y) y = 0.f;
+                                    const __half2 w = __floats2half2_rn(x, y);
+                                    p[r >> 1][2 * j + (r & 1)] = *reinterpret_cast<const uint32_t *>(&w);
+                                }
                             }
-                            // Over scores that have been read: those on their way lie behind these columns.
-                            tmem_store16(at + c / 2, p);
+                            // Over scores that have been read: those still to come lie behind these columns.
+                            tmem_store_rows16(at + c / 2, p[0]);
+                            tmem_store_rows16(at + c / 2 + (16u << 16), p[1]);
                         }
                     };
                     if (masked) weigh(std::true_type{});
                     else weigh(std::false_type{});
                     tmem_store_wait();
-                    float a, b;
-                    ptx::unpack2(total, a, b);
-                    sum += a + b;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float x, y;
+                        ptx::unpack2(total[r], x, y);
+                        sum[r] += x + y; // of this lane's columns
+                    }
                     ptx::tcgen05_fence_before();
                     arrive(softmaxed[team][half]);
                 }
@@ -533,7 +584,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             }
             if (last >= 0) {
                 if (!wait(weighted[team][1], last >> 1)) return false;
-                stats[team][row] = make_float2(most, sum);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+                    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+                    if (!t) stats[team][32 * (warp & 3) + 8 * r + g] = make_float2(most[r], sum[r]);
+                }
             }
             arrive(meet);
             if (!wait(meet, part.ordinal)) return false;
@@ -588,7 +644,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 else if (part.first_cta >= 0) args.table[index] = make_int4(part.first_cta, int(blockIdx.x) - part.first_cta + 1, part.first_slot, row);
             }
             ptx::tcgen05_fence_before();
-            arrive(outputs_free);
+            add_count(outputs_free);
             first_tile = end;
             return true;
         });

@@ -114,6 +114,29 @@ def test_many_sequences(ctx_factory):
     check(batch.run(ctx_factory("int8")), *batch.want())
 
 
+def test_parts_that_only_one_team_has_tiles_of(ctx_factory):
+    """Over a thousand short segments of 128 query rows between longer ones, many to a multiprocessor and call after call without a pause."""
+    g = torch.Generator().manual_seed(5)
+    counts = torch.randint(20, 200, (40,), generator=g).tolist()
+    batch = Batch(23, [n + (1500 if b % 7 == 3 else 0) for b, n in enumerate(counts)], counts, heads=32, kv_heads=16, head_dim=64, page=64)
+    first = batch.run(ctx_factory("int8"))
+    out = batch.out.cuda()
+    q, pages, lengths = batch.q.cuda(), batch.pages.cuda(), torch.tensor(batch.lengths, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor(batch.offsets, dtype=torch.int32, device="cuda")
+    ctx = ctx_factory("int8")
+    for _ in range(200):
+        ctx.cached_attention(q, batch.cache, pages, lengths, out, query_offsets=offsets)
+    torch.cuda.synchronize()
+    assert ctx.status() == 0 and torch.equal(out, first)
+    some = [0, 7, 20]  # sequences, in 64 bits
+    for b in some:
+        rows = slice(batch.offsets[b], batch.offsets[b + 1])
+        want, bound = attention(batch.q[rows, :256], ops.CacheView(batch.cache.keys[:, :2].contiguous(), batch.cache.values[:, :2].contiguous(),
+                                batch.cache.key_scales[:, :2].contiguous(), batch.cache.value_scales[:, :2].contiguous(), ops.I8),
+                                batch.pages[b: b + 1], batch.lengths[b: b + 1], batch.out[rows, :256], None, [0, counts[b]])
+        check(first[rows, :256], want, bound)
+
+
 @pytest.mark.parametrize("prefix", [None, 20])
 def test_no_queries_at_all(ctx_factory, prefix):
     batch = Batch(22, [30, 0], [0, 0], spare_rows=2, prefix=prefix)
