@@ -94,13 +94,14 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     constexpr uint32_t kOut = 2 * kTileKeys; // tensor memory: two teams' scores, then their outputs
     extern __shared__ uint8_t raw_smem[];
     // Tile i of the share is team i % 2's, and its barriers' use i / 2. Of each half: scored: S is done (of both: the keys' buffer is free);
-    // softmaxed: P is ready; weighted: O has it (of both: the values' buffer and the tables are free). keys/values: operands are ready.
-    __shared__ uint64_t raw_full[kSlots], raw_free[kSlots], keys_ready[2], values_ready[2], scored[2][2], softmaxed[2][2], weighted[2][2];
+    // softmaxed: P is ready; weighted: O has it (of both: the values' buffer is free). keys/values: operands are ready. tables_ready
+    // has a use for every fourth tile: its tables are not written again before the team is done with them.
+    __shared__ uint64_t raw_full[kSlots], raw_free[kSlots], keys_ready[2], values_ready[2], scored[2][2], softmaxed[2][2], weighted[2][2], tables_ready[4];
     __shared__ uint64_t largest_known, meet, drained[2]; // once per segment part, the last once
     // Warps that have laid down a part's queries, or read its outputs, over all parts. Counts and not phases: an issuer whose team has no tile in some
     // parts may be several of them behind.
     __shared__ int queries_ready, outputs_free;
-    __shared__ __align__(16) float table_key[2][kTileKeys], table_shift[2][kTileKeys], table_value[2][kTileKeys];
+    __shared__ __align__(16) float table_key[4][kTileKeys], table_shift[4][kTileKeys], table_value[4][kTileKeys]; // of tile i: i % 4
     __shared__ float2 stats[2][kRows];
     __shared__ unsigned largest[2]; // of a part's queries, by the part's parity
     __shared__ Work sums[kManyWarps];
@@ -127,6 +128,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 ptx::mbar_init(ptx::smem_u32(&weighted[t][h]), 1);
             }
             ptx::mbar_init(ptx::smem_u32(&drained[t]), 1);
+            ptx::mbar_init(ptx::smem_u32(&tables_ready[2 * t]), kTileKeys / 32);
+            ptx::mbar_init(ptx::smem_u32(&tables_ready[2 * t + 1]), kTileKeys / 32);
             largest[t] = 0;
         }
         ptx::mbar_init(ptx::smem_u32(&largest_known), kConverters);
@@ -207,37 +210,52 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         nothing.ordinal = walk_share<kRows>(args, kManySegmentUnits, start, [&](const SegmentPart &part) {
             if (!publish(part)) return open = false;
             const int *pages = args.pages + size_t(part.sequence) * args.page_stride;
-            for (int tile = part.low; tile < part.high; ++tile) {
-                const int key = tile * kTileKeys, position = key + (lane << args.box_shift);
+            // Lane i's box of a tile: whether the cache has its page, and its first row there.
+            auto find = [&](int tile, bool &good, int &row) {
+                const int position = tile * kTileKeys + (lane << args.box_shift);
                 const bool wanted = lane < boxes && position < part.s.length;
                 const int page = wanted ? load_index(pages + (position >> args.page_shift)) : -1;
-                const bool good = unsigned(page) < unsigned(args.total_pages);
-                const uint32_t held = __ballot_sync(0xffffffffu, good);
-                const int row = (((page * args.kv_heads) + part.head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
-                for (int values = 0; values < 2; ++values, ++item) {
-                    if (reuse >= 0 && !wait(raw_free[slot], reuse)) return open = false;
-                    const uint32_t to = base + Shape::ring + slot * Shape::raw, bar = ptx::smem_u32(&raw_full[slot]);
-                    if (!lane) ptx::mbar_arrive_expect_tx(bar, __popc(held) * box * HeadDim);
-                    __syncwarp();
-                    if (good)
-                        copy_run(to + uint32_t(lane << args.box_shift) * HeadDim,
-                                 static_cast<const uint8_t *>(values ? args.cached_values : args.cached_keys) + size_t(row) * HeadDim, uint32_t(box) * HeadDim, bar);
-                    // A lane copies the scales of four keys and four values. Positions on a page that the cache does not have read as NaN.
-                    const int owner = (4 * lane) >> args.box_shift, its_row = __shfl_sync(0xffffffffu, row, owner) + ((4 * lane) & (box - 1));
-                    const uint32_t scales = to + kTileKeys * HeadDim + 16 * lane;
-                    if (!values) {
-                        ptx::mbar_arrive(bar);
-                    } else if (held >> owner & 1) {
-                        copy_async16(scales, args.key_scales + its_row);
-                        copy_async16(scales + kTileKeys * 4, args.value_scales + its_row);
-                        ptx::copy_async_arrive(bar);
-                    } else {
-                        st_shared16(scales, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
-                        st_shared16(scales + kTileKeys * 4, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
-                        ptx::mbar_arrive(bar);
-                    }
-                    if (++slot == kSlots) slot = 0, ++reuse;
+                good = unsigned(page) < unsigned(args.total_pages);
+                row = (((page * args.kv_heads) + part.head) << args.page_shift) + (position & ((1 << args.page_shift) - 1));
+            };
+            auto fetch = [&](bool values, bool good, int row) {
+                if (reuse >= 0 && !wait(raw_free[slot], reuse)) return open = false;
+                const uint32_t to = base + Shape::ring + slot * Shape::raw, bar = ptx::smem_u32(&raw_full[slot]), held = __ballot_sync(0xffffffffu, good);
+                if (!lane) ptx::mbar_arrive_expect_tx(bar, __popc(held) * box * HeadDim);
+                __syncwarp();
+                if (good)
+                    copy_run(to + uint32_t(lane << args.box_shift) * HeadDim,
+                             static_cast<const uint8_t *>(values ? args.cached_values : args.cached_keys) + size_t(row) * HeadDim, uint32_t(box) * HeadDim, bar);
+                // With the keys, a lane copies the scales of four keys and four values. Positions on a page that the cache does not have read as NaN.
+                const int owner = (4 * lane) >> args.box_shift, its_row = __shfl_sync(0xffffffffu, row, owner) + ((4 * lane) & (box - 1));
+                const uint32_t scales = to + kTileKeys * HeadDim + 16 * lane;
+                if (values) {
+                    ptx::mbar_arrive(bar);
+                } else if (held >> owner & 1) {
+                    copy_async16(scales, args.key_scales + its_row);
+                    copy_async16(scales + kTileKeys * 4, args.value_scales + its_row);
+                    ptx::copy_async_arrive(bar);
+                } else {
+                    st_shared16(scales, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
+                    st_shared16(scales + kTileKeys * 4, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu, 0x7fffffffu);
+                    ptx::mbar_arrive(bar);
                 }
+                ++item;
+                if (++slot == kSlots) slot = 0, ++reuse;
+                return true;
+            };
+            // A tile's keys come before the values of the tile in front of it: these wait for that team's product, those need not.
+            bool good, next_good = false;
+            int row, next_row = 0;
+            find(part.low, good, row);
+            if (!fetch(false, good, row)) return false;
+            for (int tile = part.low; tile < part.high; ++tile) {
+                if (tile + 1 < part.high) {
+                    find(tile + 1, next_good, next_row);
+                    if (!fetch(false, next_good, next_row)) return false;
+                }
+                if (!fetch(true, good, row)) return false;
+                good = next_good, row = next_row;
             }
             return true;
         });
@@ -365,18 +383,27 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             if (thread == 0) largest[~part.ordinal & 1] = 0; // everyone has read the part before's
 
             const float score_scale = args.score_scale * scale_up;
-            for (int tile = part.low; tile < part.high; ++tile, ++first_tile) {
-                const int team = first_tile & 1, before = (first_tile >> 1) - 1;
+            auto convert_keys = [&](int i) {
+                const int team = i & 1, before = (i >> 1) - 1;
                 if (!wait(raw_full[slot], use) || (before >= 0 && !wait(scored[team][1], before))) return false;
                 {
                     const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::keys + team * Shape::operand;
                     constexpr int kPieces = HeadDim / 16, kTurns = kTileKeys * kPieces / (32 * kConverters); // kPieces: lanes to a key row
                     uint32_t w[kTurns][4];
 #pragma unroll
-                    for (int i = 0; i < kTurns; ++i) // row HeadDim bytes long, so thread t's pieces lie 16 t bytes in and one turn apart
+                    for (int u = 0; u < kTurns; ++u) // row HeadDim bytes long, so thread t's pieces lie 16 t bytes in and one turn apart
                         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(w[i][0]), "=r"(w[i][1]), "=r"(w[i][2]), "=r"(w[i][3])
-                                     : "r"(from + 16 * (thread + 32 * kConverters * i)));
+                                     : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3])
+                                     : "r"(from + 16 * (thread + 32 * kConverters * u)));
+                    // The tile's scales, ahead of its values: the softmax of its first half needs no more than them and the scores.
+                    if (thread < kTileKeys) {
+                        const float *scales = reinterpret_cast<const float *>(base_bytes + Shape::ring + slot * Shape::raw + kTileKeys * HeadDim);
+                        const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
+                        table_key[i & 3][thread] = key_scale * score_scale;
+                        table_value[i & 3][thread] = value_scale;
+                        table_shift[i & 3][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
+                        arrive(tables_ready[i & 3]);
+                    }
                     arrive(raw_free[slot]);
                     const int c = thread % kPieces, row = thread / kPieces;
                     // The second panel's lanes store their chunks in the other order: eight lanes then meet eight banks. Rows of a turn are a
@@ -386,22 +413,25 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     const uint32_t panel = to + uint32_t(c >> 2) * (kTileKeys * 128), near = panel + panel_at(row, 2 * (c & 3) + odd),
                                    far = panel + panel_at(row, 2 * (c & 3) + 1 - odd);
 #pragma unroll
-                    for (int i = 0; i < kTurns; ++i) {
+                    for (int u = 0; u < kTurns; ++u) {
                         uint32_t h[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) widen_key<F>(odd ? w[i][e ^ 2] : w[i][e], h[2 * e], h[2 * e + 1]);
+                        for (int e = 0; e < 4; ++e) widen_key<F>(odd ? w[u][e ^ 2] : w[u][e], h[2 * e], h[2 * e + 1]);
                         constexpr uint32_t kApart = 32 * kConverters / kPieces * 128;
-                        st_shared16(near + i * kApart, h[0], h[1], h[2], h[3]);
-                        st_shared16(far + i * kApart, h[4], h[5], h[6], h[7]);
+                        st_shared16(near + u * kApart, h[0], h[1], h[2], h[3]);
+                        st_shared16(far + u * kApart, h[4], h[5], h[6], h[7]);
                     }
                 }
                 ptx::fence_proxy_async_smem();
                 arrive(keys_ready[team]);
                 next_slot();
+                return true;
+            };
+            auto convert_values = [&](int i) {
+                const int team = i & 1, before = (i >> 1) - 1;
                 if (!wait(raw_full[slot], use) || (before >= 0 && !wait(weighted[team][1], before))) return false;
                 {
                     const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::values + team * Shape::operand;
-                    const float *scales = reinterpret_cast<const float *>(base_bytes + Shape::ring + slot * Shape::raw + kTileKeys * HeadDim);
                     // A lane takes four columns (a word) of eight keys, and stores eight keys of each column. Pairs of lanes take other groups of keys, so that
                     // eight lanes meet eight banks when they store.
                     constexpr int kWords = HeadDim / 4, kSets = 32 * kConverters / kWords, kTurns = kTileKeys / 8 / kSets; // kSets: threads that share a word
@@ -410,26 +440,20 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     static_assert(kSets % 8 == 0);
                     uint32_t w[kTurns][8];
 #pragma unroll
-                    for (int i = 0; i < kTurns; ++i)
+                    for (int u = 0; u < kTurns; ++u)
 #pragma unroll
                         for (int k = 0; k < 8; ++k)
-                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[i][k]) : "r"(from + (8 * (kSets * i + first) + k) * HeadDim + 4 * word));
-                    if (thread < kTileKeys) {
-                        const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
-                        table_key[team][thread] = key_scale * score_scale;
-                        table_value[team][thread] = value_scale;
-                        table_shift[team][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
-                    }
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[u][k]) : "r"(from + (8 * (kSets * u + first) + k) * HeadDim + 4 * word));
                     arrive(raw_free[slot]);
 #pragma unroll
-                    for (int i = 0; i < kTurns; ++i) {
-                        const int group = kSets * i + first;
+                    for (int u = 0; u < kTurns; ++u) {
+                        const int group = kSets * u + first;
                         uint32_t h[4][4]; // [column][pair of keys]
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
 #pragma unroll
                             for (int c = 0; c < 2; ++c)
-                                widen<F>(biased<F>(__byte_perm(w[i][2 * k], w[i][2 * k + 1], c ? 0x7362u : 0x5140u)), h[2 * c][k], h[2 * c + 1][k]);
+                                widen<F>(biased<F>(__byte_perm(w[u][2 * k], w[u][2 * k + 1], c ? 0x7362u : 0x5140u)), h[2 * c][k], h[2 * c + 1][k]);
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
                             st_shared16(to + uint32_t(group >> 3) * (HeadDim * 128) + panel_at(4 * word + c, group & 7), h[c][0], h[c][1], h[c][2], h[c][3]);
@@ -438,7 +462,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 ptx::fence_proxy_async_smem();
                 arrive(values_ready[team]);
                 next_slot();
-            }
+                return true;
+            };
+            const int end = first_tile + part.high - part.low;
+            if (!convert_keys(first_tile)) return false;
+            for (; first_tile < end; ++first_tile)
+                if ((first_tile + 1 < end && !convert_keys(first_tile + 1)) || !convert_values(first_tile)) return false;
             return true;
         });
     } else if (warp < kSoftmaxWarps) { // --------------------------------------------------------- softmax
@@ -467,34 +496,33 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     constexpr int kHalf = kTileKeys / 2;
                     const int key = (part.low + i - first_tile) * kTileKeys + half * kHalf + 2 * t;
                     const uint32_t at = at_scores + half * kHalf;
-                    const float *const of_key = table_key[team] + half * kHalf + 2 * t, *const of_shift = table_shift[team] + half * kHalf + 2 * t,
-                                      *const of_value = table_value[team] + half * kHalf + 2 * t;
+                    const float *const of_key = table_key[i & 3] + half * kHalf + 2 * t, *const of_shift = table_shift[i & 3] + half * kHalf + 2 * t,
+                                      *const of_value = table_value[i & 3] + half * kHalf + 2 * t;
                     const bool masked = key - 2 * t + kHalf - 1 > least;
-                    if (!wait(scored[team][half], i >> 1) || (!half && !wait(values_ready[team], i >> 1))) return false; // the tables come with the values
+                    if (!wait(scored[team][half], i >> 1) || (!half && !wait(tables_ready[i & 3], i >> 2))) return false;
                     ptx::tcgen05_fence_after();
-                    // 32 columns of 32 rows at a time. Having the next ones on their way meanwhile spills, and the other team's warp fills the gap.
-                    auto load = [&](int c, uint32_t(&s)[2][16]) {
-                        ptx::tmem_load_rows16<32>(at + c, s[0]);
-                        ptx::tmem_load_rows16<32>(at + c + (16u << 16), s[1]);
-                    };
+                    // 16 rows by 32 columns at a time, the next ones on their way while these are worked on.
+                    const auto place = [&](int unit) { return at + uint32_t(unit >> 1) * 32 + (uint32_t(unit & 1) << 20); };
                     float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     auto find_highest = [&](auto masked_tile) {
                         constexpr bool kMasked = decltype(masked_tile)::value;
-#pragma unroll 1
-                        for (int c = 0; c < kHalf; c += 32) {
-                            uint32_t now[2][16];
-                            load(c, now);
+                        uint32_t s[2][16];
+                        ptx::tmem_load_rows16<32>(place(0), s[0]);
+#pragma unroll
+                        for (int unit = 0; unit < 4; ++unit) {
+                            const int c = (unit >> 1) * 32, b = unit & 1;
                             ptx::tmem_load_wait();
+                            if (unit < 3) ptx::tmem_load_rows16<32>(place(unit + 1), s[(unit + 1) & 1]);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), shift = *reinterpret_cast<const uint64_t *>(of_shift + c + 8 * j);
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) {
+                                for (int r = 0; r < 2; ++r) {
                                     float x, y;
-                                    ptx::unpack2(ptx::fma2(pair(now[r >> 1][4 * j + 2 * (r & 1)], now[r >> 1][4 * j + 2 * (r & 1) + 1]), k, shift), x, y);
-                                    if (kMasked && key + c + 8 * j > limit[r]) x = -INFINITY;
-                                    if (kMasked && key + c + 8 * j + 1 > limit[r]) y = -INFINITY;
-                                    highest[r] = fmaxf(highest[r], fmaxf(x, y));
+                                    ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, shift), x, y);
+                                    if (kMasked && key + c + 8 * j > limit[2 * b + r]) x = -INFINITY;
+                                    if (kMasked && key + c + 8 * j + 1 > limit[2 * b + r]) y = -INFINITY;
+                                    highest[2 * b + r] = fmaxf(highest[2 * b + r], fmaxf(x, y));
                                 }
                             }
                         }
@@ -503,12 +531,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     else find_highest(std::false_type{});
                     bool raise = false; // also from no reference at all
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 1));
-                        highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 2));
-                        raise |= highest[r] > most[r] + kReferenceSlack;
-                    }
+                    for (int r = 0; r < 4; ++r) raise |= highest[r] > most[r] + kReferenceSlack;
                     if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) { // over the row's four lanes
+                            highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 1));
+                            highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 2));
+                        }
                         float shrink = 1.f; // of row `lane`
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
@@ -540,32 +569,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     }
                     auto weigh = [&](auto masked_tile) {
                         constexpr bool kMasked = decltype(masked_tile)::value;
-#pragma unroll 1
-                        for (int c = 0; c < kHalf; c += 32) {
-                            uint32_t now[2][16];
-                            load(c, now);
+                        uint32_t s[2][16];
+                        ptx::tmem_load_rows16<32>(place(0), s[0]);
+#pragma unroll
+                        for (int unit = 0; unit < 4; ++unit) {
+                            const int c = (unit >> 1) * 32, b = unit & 1;
                             ptx::tmem_load_wait();
-                            uint32_t p[2][8];
+                            if (unit < 3) ptx::tmem_load_rows16<32>(place(unit + 1), s[(unit + 1) & 1]);
+                            uint32_t p[8];
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
                                 const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), v = *reinterpret_cast<const uint64_t *>(of_value + c + 8 * j);
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) {
+                                for (int r = 0; r < 2; ++r) {
+                                    const int mine = 2 * b + r;
                                     float x, y;
-                                    ptx::unpack2(ptx::fma2(pair(now[r >> 1][4 * j + 2 * (r & 1)], now[r >> 1][4 * j + 2 * (r & 1) + 1]), k, minus[r]), x, y);
-                                    const bool hide_x = kMasked && key + c + 8 * j > limit[r], hide_y = kMasked && key + c + 8 * j + 1 > limit[r];
+                                    ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, minus[mine]), x, y);
+                                    const bool hide_x = kMasked && key + c + 8 * j > limit[mine], hide_y = kMasked && key + c + 8 * j + 1 > limit[mine];
                                     const uint64_t both = ptx::pack2(exp2_approx(hide_x ? -INFINITY : x), exp2_approx(hide_y ? -INFINITY : y));
-                                    total[r] = ptx::add2(total[r], both);
+                                    total[mine] = ptx::add2(total[mine], both);
                                     ptx::unpack2(ptx::mul2(both, v), x, y);
                                     if (hide_x) x = 0.f; // a hidden row's scale may be anything
                                     if (hide_y) y = 0.f;
                                     const __half2 w = __floats2half2_rn(x, y);
-                                    p[r >> 1][2 * j + (r & 1)] = *reinterpret_cast<const uint32_t *>(&w);
+                                    p[2 * j + r] = *reinterpret_cast<const uint32_t *>(&w);
                                 }
                             }
-                            // Over scores that have been read: those still to come lie behind these columns.
-                            tmem_store_rows16(at + c / 2, p[0]);
-                            tmem_store_rows16(at + c / 2 + (16u << 16), p[1]);
+                            // Over scores that have been read: those still to come lie behind these columns, or in other rows.
+                            tmem_store_rows16(at + c / 2 + (uint32_t(b) << 20), p);
                         }
                     };
                     if (masked) weigh(std::true_type{});
