@@ -43,13 +43,14 @@ PassPlan plan_pass(int rows, int sequences, int group, bool prefix) {
     if (plan.many) plan.part_columns = int(std::min<int64_t>(kManyRows, all));
     return plan;
 }
-// A pass's workspace: the table, the partial sums, and with a shared prefix the rows that were done in one part.
+// A pass's workspace: the closed segments and the partial sums; with a shared prefix also the table of all rows and those done in one part.
 struct Carve {
-    size_t table, partials, complete, bytes;
+    size_t closed, table, partials, complete, bytes;
     Carve(int rows, int heads, int head_dim, bool prefix, int part_columns, int ctas) {
         const size_t row = size_t(head_dim + kPartialExtra) * 4;
-        table = 0;
-        partials = padded(size_t(rows) * heads * sizeof(int4));
+        closed = 0;
+        table = padded(size_t(ctas) * sizeof(ClosedSegment));
+        partials = table + (prefix ? padded(size_t(rows) * heads * sizeof(int4)) : 0);
         complete = partials + padded(size_t(ctas) * 2 * part_columns * row);
         bytes = complete + (prefix ? padded(size_t(rows) * heads * row) : 0);
     }
@@ -140,23 +141,25 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     args.status = status;
 
     CombineArgs combine{};
-    combine.sources = prefix ? 2 : 1, combine.rows = rows, combine.heads = heads, combine.output_stride = p.output.ld();
+    combine.rows = rows, combine.heads = heads, combine.group = args.group, combine.output_stride = p.output.ld();
     combine.row_count = p.query_offsets ? p.query_offsets + p.sequences : nullptr;
     combine.output = p.output.data, combine.output_scale = format;
     const CUtensorMap keys = cache_map(p.cache.keys, p.cache, 1 << args.box_shift), values = cache_map(p.cache.values, p.cache, 1 << args.box_shift);
     by_type(p.queries.type, p.cache.type, head_dim, [&](auto element, auto format, auto width) {
         using T = decltype(element);
         char *base = static_cast<char *>(workspace);
-        for (int pass = 0; pass < combine.sources; ++pass) {
+        int columns = 0; // rows of a split segment at most
+        for (int pass = 0; pass < (prefix ? 2 : 1); ++pass) {
             const PassPlan plan = plan_pass(rows, p.sequences, args.group, pass);
             const Carve carve(rows, heads, head_dim, prefix, plan.part_columns, ctas);
             args.part_columns = plan.part_columns;
-            args.table = reinterpret_cast<int4 *>(base + carve.table);
+            args.closed = reinterpret_cast<ClosedSegment *>(base + carve.closed);
+            args.table = prefix ? reinterpret_cast<int4 *>(base + carve.table) : nullptr;
             args.partials = reinterpret_cast<float *>(base + carve.partials);
             args.complete = prefix ? reinterpret_cast<float *>(base + carve.complete) : nullptr;
             base += carve.bytes;
             if (pass) {
-                args.prefix = true;
+                args.prefix = args.follows = true;
                 args.pages = p.prefix_pages, args.lengths = p.prefix_length, args.sequences = 1;
                 args.page_columns = args.page_stride = p.prefix_columns;
             }
@@ -164,11 +167,17 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
             const int most = !pass && !p.query_offsets ? args.group : INT_MAX;
             if (plan.many) launch_many<T, decltype(format)::value, decltype(width)::value>(args, ctas, stream);
             else launch_pass<T, decltype(format)::value, decltype(width)::value>(plan.narrow, most, args, keys, values, ctas, stream);
-            combine.source[pass] = {args.partials, args.complete, args.table, ctas, plan.part_columns};
+            combine.source[pass] = {args.partials, args.complete, args.closed, args.table, ctas, plan.part_columns};
+            columns = std::min(most, plan.part_columns);
         }
-        const long long warps = (long long)rows * heads;
-        launch_pdl("attention combine", combine_attention<T, decltype(width)::value>, dim3(unsigned((warps + kCombineThreads / 32 - 1) / (kCombineThreads / 32))),
-                   dim3(kCombineThreads), 0, stream, combine);
+        constexpr int kWarps = kCombineThreads / 32;
+        if (prefix)
+            launch_pdl("attention combine", combine_prefixed<T, decltype(width)::value>, dim3(unsigned(((long long)rows * heads + kWarps - 1) / kWarps)),
+                       dim3(kCombineThreads), 0, stream, combine);
+        else // two rows a warp where there are many: most CTAs find no segment, the others have little to read
+            launch_pdl("attention combine", combine_attention<T, decltype(width)::value>,
+                       dim3(unsigned(ctas), unsigned(columns > 16 ? (columns + 2 * kWarps - 1) / (2 * kWarps) : (columns + kWarps - 1) / kWarps)), dim3(kCombineThreads),
+                       0, stream, combine);
     });
 }
 } // namespace tts

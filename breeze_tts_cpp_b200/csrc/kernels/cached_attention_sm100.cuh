@@ -131,12 +131,13 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         ptx::prefetch_tensormap(&key_map);
         ptx::prefetch_tensormap(&value_map);
     }
+    // Dependents may start once what this pass reads is there: the second pass of a call takes that from the first.
+    if (!args.follows) pdl_wait_upstream();
     pdl_launch_dependents();
     __syncthreads();
 
     // Only the producers need to know where the CTA's share lies; for a long batch all threads find out.
     if (args.sequences > kScanAlone) {
-        pdl_wait_upstream();
         start_together<kColumns, kAttentionWarps>(args, kFewSegmentUnits, sums, &found);
     }
     // Every wait is bounded, and a warp whose wait gave up leaves as one; the others follow when theirs do.
@@ -167,14 +168,15 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         const bool leads = warp == kProducer;
         int stage = 0, issued = 0, team = 0;
         uint32_t phase = 0;
-        if (args.sequences <= kScanAlone) pdl_wait_upstream();
         const Start start = args.sequences > kScanAlone ? found : start_alone<kColumns>(args, kFewSegmentUnits);
         const int box = 1 << args.box_shift, boxes = kTileKeys >> args.box_shift;
         const uint32_t box_bytes = uint32_t(box) * 2 * HeadDim;
         bool open = true;
+        if (leads && !lane) note_closed(args, nullptr, kColumns);
         const int parts = walk_share<kColumns>(args, kFewSegmentUnits, start, [&](const SegmentPart &part) {
             const SequenceShape &s = part.s;
             const int low = part.low, high = part.high, head = part.head, columns = part.columns;
+            if (leads && !lane && part.first_cta >= 0) note_closed(args, &part, kColumns);
             const int *pages = args.pages + size_t(part.sequence) * args.page_stride;
             // Lane i's page of a tile: its box i. Always a load, of the last page where there is none, so that nothing waits for it here.
             auto page_at = [&](int tile) {
@@ -274,6 +276,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         // No copy may be in flight when the CTA leaves, whatever the workers did.
         int ignored = 0;
         for (int i = max(0, issued - stages); i < issued; ++i) ptx::mbar_wait(ptx::smem_u32(&full[i % kTeams][i % stages]), uint32_t((i / kTeams) / period) & 1, &ignored);
+        if (args.follows) pdl_wait_upstream();
         return;
     }
 
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                     store_row4<T>(args, static_cast<T *>(args.output) + at_row * args.output_stride + head * HeadDim + d, v,
                                            l == 0.f ? 0.f : args.output_scale / l);
                 }
-                if (!d) {
+                if (!d && args.table) {
                     if (!(flags & kNoteSplit)) args.table[index] = make_int4(0, 0, 0, 0);
                     else if (note.first_cta >= 0) args.table[index] = make_int4(note.first_cta, int(blockIdx.x) - note.first_cta + 1, note.first_slot, column);
                 }
@@ -563,56 +566,28 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     }
 }
 
-// Second launch: a warp per query row and head adds up what the first left in parts (own, and the shared prefix's), in the order of the
-// CTAs. Rows that are complete already cost it one read.
+// Last launch: a warp per query row and head adds up what was left in parts, in the order of the CTAs.
+constexpr int kCombineThreads = 128;
 struct CombineSource {
-    const float *partials, *complete; // complete == null: segments in one part are written already
+    const float *partials, *complete;
+    const ClosedSegment *closed;
     const int4 *table;
     int ctas, columns;
 };
 struct CombineArgs {
     CombineSource source[2];
-    int sources, rows, heads, output_stride;
-    bool aligned;
+    int rows, heads, group, output_stride;
     const int *row_count; // last of the query offsets, or null
     void *output;
     float output_scale;
 };
-constexpr int kCombineThreads = 128;
-template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThreads) combine_attention(const CombineArgs args) {
-    constexpr int kRow = HeadDim + kPartialExtra, kShare = HeadDim / 32;
-    pdl_launch_dependents();
-    pdl_wait_upstream();
-    const int lane = threadIdx.x & 31;
-    const long long index = (long long)blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5);
-    const int rows = args.row_count ? min(args.rows, load_index(args.row_count)) : args.rows;
-    if (index >= (long long)rows * args.heads) return;
+template <int HeadDim> struct RowSum {
+    static constexpr int kRow = HeadDim + kPartialExtra, kShare = HeadDim / 32;
     float highest = -INFINITY, l = 0.f, v[kShare] = {};
-    bool written = args.sources == 1;
-    int4 entries[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (i < args.sources)
-            asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(entries[i].x), "=r"(entries[i].y), "=r"(entries[i].z), "=r"(entries[i].w)
-                         : "l"(args.source[i].table + index)
-                         : "memory");
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if (i >= args.sources) break;
-        const CombineSource &s = args.source[i];
-        const int4 entry = entries[i];
-        const bool whole = entry.y <= 0;
-        if (whole && !s.complete) continue;
-        // Rows that no sequence covers have no entry: whatever stands there stays inside the workspace.
-        if (!whole && (entry.x < 0 || entry.y > s.ctas - entry.x || unsigned(entry.z) > 1u || unsigned(entry.w) >= unsigned(s.columns))) continue;
-        written = false;
-        const int parts = whole ? 1 : entry.y;
-        auto part_of = [&](int part) {
-            return whole ? s.complete + size_t(index) * kRow
-                         : s.partials + (size_t((entry.x + part) * 2 + (part ? 0 : entry.z)) * s.columns + entry.w) * kRow;
-        };
-        // 32 parts at a time: a lane reads the maximum and the sum of one, so that the rows' loads depend on nothing but the loop.
+
+    // 32 parts at a time: a lane reads the maximum and the sum of one, so that the rows' loads depend on nothing but the loop.
+    template <class PartOf> __device__ __forceinline__ void add(int parts, PartOf &&part_of) {
+        const int lane = threadIdx.x & 31;
         for (int first = 0; first < parts; first += 32) {
             const int count = min(32, parts - first);
             float most = -INFINITY, sum = 0.f;
@@ -650,10 +625,59 @@ template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThread
             }
         }
     }
-    if (written) return;
-    const float factor = l == 0.f ? 0.f : args.output_scale / l;
-    T *to = static_cast<T *>(args.output) + size_t(index / args.heads) * args.output_stride + size_t(index % args.heads) * HeadDim + kShare * lane;
+    template <class T> __device__ __forceinline__ void store(const CombineArgs &a, int row, int head) const {
+        const float factor = l == 0.f ? 0.f : a.output_scale / l;
+        T *to = static_cast<T *>(a.output) + size_t(row) * a.output_stride + size_t(head) * HeadDim + kShare * int(threadIdx.x & 31);
 #pragma unroll
-    for (int c = 0; c < kShare; ++c) to[c] = T(v[c] * factor);
+        for (int c = 0; c < kShare; ++c) to[c] = T(v[c] * factor);
+    }
+};
+// Without a prefix: only split segments are left to do, at most one for each CTA of the pass. A warp takes a few of a segment's rows.
+template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThreads) combine_attention(const CombineArgs args) {
+    pdl_launch_dependents();
+    pdl_wait_upstream();
+    const CombineSource &s = args.source[0];
+    const int *entry = reinterpret_cast<const int *>(s.closed + blockIdx.x);
+    int4 where, whose;
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(where.x), "=r"(where.y), "=r"(where.z), "=r"(where.w) : "l"(entry) : "memory");
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(whose.x), "=r"(whose.y), "=r"(whose.z), "=r"(whose.w) : "l"(entry + 4) : "memory");
+    if (!where.y) return;
+    for (int column = int(blockIdx.y) * (kCombineThreads / 32) + int(threadIdx.x >> 5); column < whose.z; column += int(gridDim.y) * (kCombineThreads / 32)) {
+        RowSum<HeadDim> sum;
+        sum.add(where.y, [&](int part) {
+            return s.partials + (size_t((where.x + part) * 2 + (part ? 0 : where.z)) * s.columns + column) * RowSum<HeadDim>::kRow;
+        });
+        const int flat = whose.x + column, token = flat / args.group;
+        sum.template store<T>(args, where.w + token, whose.y * args.group + flat - token * args.group);
+    }
+}
+// With a prefix: every row has a result of both passes, in one part or several.
+template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThreads) combine_prefixed(const CombineArgs args) {
+    pdl_launch_dependents();
+    pdl_wait_upstream();
+    const long long index = (long long)blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5);
+    const int rows = args.row_count ? min(args.rows, load_index(args.row_count)) : args.rows;
+    if (index >= (long long)rows * args.heads) return;
+    int4 entries[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(entries[i].x), "=r"(entries[i].y), "=r"(entries[i].z), "=r"(entries[i].w)
+                     : "l"(args.source[i].table + index)
+                     : "memory");
+    RowSum<HeadDim> sum;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const CombineSource &s = args.source[i];
+        const int4 entry = entries[i];
+        const bool whole = entry.y <= 0;
+        // Rows that no sequence covers have no entry: whatever stands there stays inside the workspace.
+        if (!whole && (entry.x < 0 || entry.y > s.ctas - entry.x || unsigned(entry.z) > 1u || unsigned(entry.w) >= unsigned(s.columns))) continue;
+        sum.add(whole ? 1 : entry.y, [&](int part) {
+            return whole ? s.complete + size_t(index) * RowSum<HeadDim>::kRow
+                         : s.partials + (size_t((entry.x + part) * 2 + (part ? 0 : entry.z)) * s.columns + entry.w) * RowSum<HeadDim>::kRow;
+        });
+    }
+    sum.template store<T>(args, int(index / args.heads), int(index % args.heads));
 }
 } // namespace tts::b200

@@ -143,11 +143,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     }
     if (warp == kIssuer) ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
     ptx::tcgen05_fence_before();
+    // Dependents may start once what this pass reads is there: the second pass of a call takes that from the first.
+    if (!args.follows) pdl_wait_upstream();
     pdl_launch_dependents();
     __syncthreads();
     ptx::tcgen05_fence_after();
     const uint32_t tmem = ptx::warp_uniform(tmem_slot);
-    pdl_wait_upstream();
     if (args.sequences > kScanAlone) start_together<kRows, kManyWarps>(args, kManySegmentUnits, sums, &found);
 
     // Every wait is bounded. A warp whose wait gave up goes to the end, where all meet; the others follow when theirs do.
@@ -207,8 +208,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         const Start start = args.sequences > kScanAlone ? found : start_alone<kRows>(args, kManySegmentUnits);
         bool open = true;
         SegmentPart nothing{};
+        if (!lane) note_closed(args, nullptr, kRows);
         nothing.ordinal = walk_share<kRows>(args, kManySegmentUnits, start, [&](const SegmentPart &part) {
             if (!publish(part)) return open = false;
+            if (!lane && part.first_cta >= 0) note_closed(args, &part, kRows);
             const int *pages = args.pages + size_t(part.sequence) * args.page_stride;
             // Lane i's box of a tile: whether the cache has its page, and its first row there.
             auto find = [&](int tile, bool &good, int &row) {
@@ -671,7 +674,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             }
             if (live && !team) {
                 if (kept) kept[HeadDim] = highest, kept[HeadDim + 1] = l;
-                if (!part.split) args.table[index] = make_int4(0, 0, 0, 0);
+                if (!args.table) {
+                } else if (!part.split) args.table[index] = make_int4(0, 0, 0, 0);
                 else if (part.first_cta >= 0) args.table[index] = make_int4(part.first_cta, int(blockIdx.x) - part.first_cta + 1, part.first_slot, row);
             }
             ptx::tcgen05_fence_before();
@@ -684,5 +688,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     __syncthreads();
     ptx::tcgen05_fence_after();
     if (warp == kIssuer) ptx::tmem_dealloc(tmem, 512);
+    if (args.follows) pdl_wait_upstream();
 }
 } // namespace tts::b200

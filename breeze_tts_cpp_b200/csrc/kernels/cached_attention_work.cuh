@@ -17,6 +17,11 @@ constexpr int kPartialExtra = 4; // maximum and sum behind a partial row, padded
 constexpr int kScanAlone = 256;  // up to here a warp adds the sequences' work up by itself
 constexpr size_t kAttentionSmem = 224 * 1024;
 
+// The split segment that a CTA closes: where its parts lie, and whose rows they are. count == 0: none.
+struct ClosedSegment {
+    int first_cta, count, first_slot, row, flat, head, columns, unused;
+};
+
 // One pass over one set of page tables: the sequences' own, or the shared prefix as one sequence of all query rows.
 struct AttentionArgs {
     const void *queries;
@@ -34,8 +39,12 @@ struct AttentionArgs {
     int stages, merge_columns, merge_buffers;
     int part_columns; // query rows that a partial sum has room for
     float *partials; // [ctas][2][part_columns][head_dim + kPartialExtra]
+    ClosedSegment *closed; // [ctas]
+    // With a shared prefix, whose rows take both passes' results: where each row's is, and the complete ones.
     int4 *table;     // [rows * heads]: first CTA, parts, slot of the first part, column; parts == 0: complete
-    float *complete; // [rows * heads][head_dim + kPartialExtra], or null: complete segments go to the output
+    float *complete; // [rows * heads][head_dim + kPartialExtra]
+    // The second pass of a call reads nothing that the first writes, so it does not wait for it (which has waited for what both read) before its end.
+    bool follows;
     int *status;
 };
 
@@ -190,6 +199,13 @@ struct SegmentPart {
     int slot;                  // where a partial sum goes: 0 for a share's first part, 1 for a later one
     bool split, final;
 };
+// What a CTA says about the segment that it closes, for the launch that adds up the parts; `part` null: that it closes none.
+__device__ __forceinline__ void note_closed(const AttentionArgs &a, const SegmentPart *part, int columns_per_tile) {
+    ClosedSegment c{};
+    if (part)
+        c = {part->first_cta, int(blockIdx.x) - part->first_cta + 1, part->first_slot, part->s.row, part->query_tile * columns_per_tile, part->head, part->columns, 0};
+    a.closed[blockIdx.x] = c;
+}
 // Calls `each` for every part of this CTA's share, in order, until it returns false. Returns the number of parts.
 template <int Columns, class Each>
 __device__ __forceinline__ int walk_share(const AttentionArgs &a, int segment_units, const Start &start, Each &&each) {
