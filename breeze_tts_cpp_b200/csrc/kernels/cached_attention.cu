@@ -62,9 +62,9 @@ template <class T, Type F, int HeadDim> void launch_many(const AttentionArgs &ar
 template <class T, Type F, int HeadDim, int Tiles>
 void launch_pass(AttentionArgs args, int most_columns, const CUtensorMap &keys, const CUtensorMap &values, int ctas, cudaStream_t stream) {
     using Shape = AttentionShape<HeadDim, Tiles>;
-    // What the workers leave for the mergers, twice where that is small, and as many stages as the rest of the shared memory holds.
+    // What the workers leave for the mergers, several times where that is small, and as many stages as the rest of the shared memory holds.
     args.merge_columns = std::min(Shape::columns, most_columns);
-    args.merge_buffers = args.merge_columns <= 4 ? 2 : 1;
+    args.merge_buffers = args.merge_columns <= 2 ? kMergeBuffers : args.merge_columns <= 4 ? 2 : 1;
     const size_t merge = size_t(args.merge_buffers) * Shape::merge(args.merge_columns);
     args.stages = int(std::min<size_t>(kMaxRing, (kAttentionSmem - 1024 - merge) / Shape::stage));
     launch_pdl("cached attention", cached_attention<T, F, HeadDim, Tiles>, dim3(unsigned(ctas)), dim3(kAttentionThreads),

@@ -27,9 +27,9 @@
 #include "kernels/sm100_ptx.cuh"
 
 namespace tts::b200 {
-constexpr int kTeam = 4, kTeams = 2, kWorkers = kTeam * kTeams, kProducers = 2, kMergers = 2, kMaxRing = 12;
+constexpr int kTeam = 4, kTeams = 2, kWorkers = kTeam * kTeams, kProducers = 2, kMergers = 2, kMaxRing = 12, kMergeBuffers = 4;
 constexpr int kAttentionWarps = kWorkers + kProducers + kMergers, kAttentionThreads = 32 * kAttentionWarps; // three per scheduler: 168 registers a thread
-constexpr int kFewSegmentUnits = 2; // a segment's queries, flush and merge next to a tile's kTileUnits
+constexpr int kFewSegmentUnits = 6; // a segment's queries, flush and merge next to a tile's kTileUnits (64 sequences of up to 4096: 2 units 65.2 us, 4 60.9, 6 59.9)
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     using Shape = AttentionShape<HeadDim, Tiles>;
     constexpr int kColumns = Shape::columns, kSteps = HeadDim / 16, kProducer = kWorkers, kMerger = kProducer + kProducers;
     extern __shared__ uint8_t raw_smem[];
-    __shared__ uint64_t full[kTeams][kMaxRing], empty[kMaxRing], merge_full[2]; // full: of each team
-    __shared__ TileNote notes[kMaxRing], merge_notes[2];
+    __shared__ uint64_t full[kTeams][kMaxRing], empty[kMaxRing], merge_full[kMergeBuffers]; // full: of each team
+    __shared__ TileNote notes[kMaxRing], merge_notes[kMergeBuffers];
     __shared__ Work sums[kAttentionWarps];
     __shared__ Start found;
     __shared__ int abort_flag;
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
             for (int team = 0; team < kTeams; ++team) ptx::mbar_init(ptx::smem_u32(&full[team][s]), 33); // the leading producer's, and a lane's scales each
             ptx::mbar_init(ptx::smem_u32(&empty[s]), kTeam);
         }
-        for (int b = 0; b < 2; ++b) ptx::mbar_init(ptx::smem_u32(&merge_full[b]), kWorkers);
+        for (int b = 0; b < kMergeBuffers; ++b) ptx::mbar_init(ptx::smem_u32(&merge_full[b]), kWorkers);
         abort_flag = merged = 0;
         ptx::fence_barrier_init();
         ptx::prefetch_tensormap(&key_map);
@@ -362,26 +362,35 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                     const uint4 v = *reinterpret_cast<const uint4 *>(bytes + Shape::queries + (8 * n + g) * Shape::query_row + (kShare * t + 8 * c) * 2);
                     *reinterpret_cast<uint4 *>(share + 8 * c) = live ? v : make_uint4(0, 0, 0, 0);
                 }
-                unsigned largest = 0;
+                const uint32_t *words = reinterpret_cast<const uint32_t *>(share);
+                int exponent = 0; // BF16 rows are divided by the power of two of their largest element; FP16 ones are in range as they are
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                    unsigned largest = 0;
 #pragma unroll
-                for (int c = 0; c < kShare; ++c) largest = max(largest, __float_as_uint(float(share[c])) & 0x7fffffffu);
-                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-                const int exponent = largest && largest < 0x7f800000u ? max(int(largest >> 23), 1) - 127 : 0;
+                    for (int c = 0; c < kShare / 2; ++c) largest = max(largest, max(words[c] << 16 & 0x7fffffffu, words[c] & 0x7fff0000u));
+                    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                    largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                    exponent = largest && largest < 0x7f800000u ? max(int(largest >> 23), 1) - 127 : 0;
+                }
                 const float down = __int_as_float(exponent < 127 ? (127 - exponent) << 23 : 0x00400000); // 2^-exponent
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
-                        const __half2 v = __floats2half2_rn(float(share[4 * k + 2 * c]) * down, float(share[4 * k + 2 * c + 1]) * down);
-                        q[n][k][c] = *reinterpret_cast<const uint32_t *>(&v);
+                        const uint32_t w = words[2 * k + c];
+                        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                            const __half2 v = __floats2half2_rn(__uint_as_float(w << 16) * down, __uint_as_float(w & 0xffff0000u) * down);
+                            q[n][k][c] = *reinterpret_cast<const uint32_t *>(&v);
+                        } else {
+                            q[n][k][c] = w;
+                        }
                     }
                 // The scores of this lane belong to columns 2t and 2t + 1, whose rows lanes 8t and 8t + 4 hold.
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int of = __shfl_sync(0xffffffffu, exponent, 8 * t + 4 * c), seen = 8 * n + 2 * t + c;
-                    factor[n][c] = ldexpf(args.score_scale, of);
-                    limit[n][c] = seen < columns ? (args.prefix ? note.limit : note.limit + (note.flat + seen) / args.group) : -1;
+                    factor[n][c] = args.score_scale * __int_as_float((127 + of) << 23);
+                    limit[n][c] = seen >= columns ? -1 : args.prefix || note.count == 1 ? note.limit : note.limit + (note.flat + seen) / args.group;
                     if (seen < columns) least = min(least, limit[n][c]);
                     most[n][c] = -INFINITY;
                     sum[n][c] = 0.f;

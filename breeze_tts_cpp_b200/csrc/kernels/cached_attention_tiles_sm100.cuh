@@ -18,7 +18,7 @@
 
 namespace tts::b200 {
 constexpr int kManyRows = 128;
-constexpr int kManySegmentUnits = 6; // a segment's queries, the meeting of the teams and the store next to a tile's kTileUnits
+constexpr int kManySegmentUnits = 12; // filling and draining the pipeline, the meeting of the teams and the store, next to a tile's kTileUnits
 constexpr int kSoftmaxWarps = 8, kConverters = 8, kManyWarps = kSoftmaxWarps + kConverters + 4, kManyThreads = 32 * kManyWarps; // one warp idles
 // Registers a thread: 96 at launch (61440 in all); two groups of four warps each for the softmax and the conversions, one for the rest. The
 // shares add up to the launch's: 256 x 144 + 256 x 64 + 128 x 64.
