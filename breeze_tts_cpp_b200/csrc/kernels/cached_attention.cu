@@ -129,6 +129,7 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     args.query_stride = p.queries.ld(), args.output_stride = p.output.ld();
     args.rows = rows, args.heads = heads, args.kv_heads = p.cache.kv_heads, args.group = heads / p.cache.kv_heads;
     args.aligned = aligned16(p.queries) && aligned16(p.output);
+    args.sectors = args.aligned && reinterpret_cast<uintptr_t>(p.output.data) % 32 == 0 && p.output.ld() % 16 == 0;
     args.pages = p.pages, args.lengths = p.lengths, args.query_offsets = p.query_offsets;
     args.sequences = p.sequences, args.page_columns = p.page_columns, args.page_stride = p.page_stride;
     args.page_shift = shift_of(p.cache.page_size), args.total_pages = p.cache.pages, args.offset_count = p.sequences;

@@ -5,11 +5,11 @@
 // when a tile's maximum passes it by 2^8, so that the accumulated output is rescaled hardly ever.
 //
 // Layout. A segment is 128 query rows of one cached head (tokens times the group's heads; of a prefix: of all sequences), a tile 128 keys. Per tile
-// a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Tiles alternate between
-// two teams of four softmax warps, 32 rows a warp, and each team has a softmax state, an output and an issuing warp of its own; the two
-// meet once per segment. A team takes its tile in two halves of 64 keys: while it works on one half, the product of the half before and the scores
-// of the next tile's run. Eight warps turn bytes into fp16 operands: keys as they are, values transposed, so that both are K-major with the 128-byte
-// swizzle. Tables of a tile's scales go to the softmax warps through shared memory.
+// a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Two teams of four
+// softmax warps, 32 rows a warp, take one half of a tile's keys each, and each team has a softmax state, an output and an issuing warp of its own;
+// they meet once per segment. A team has the scores of two tiles, so that the products of one run while it works on the other. Eight warps turn
+// bytes into fp16 operands: keys as they are, values transposed, so that both are K-major with the 128-byte swizzle. Tables of a tile's scales go
+// to the softmax warps through shared memory.
 //
 // Bound. A 128 x 128 x 128 tile costs the tensor pipe about 1300 cycles, its exponentials the special-function units 1024, conversions and softmax
 // about 1600 issue cycles, so all of them have to overlap.
@@ -70,18 +70,29 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 }
 // 16-byte chunk `chunk` of row `row` in a K-major operand panel (rows of 64 halves, 128-byte swizzle).
 __device__ __forceinline__ uint32_t panel_at(int row, int chunk) { return uint32_t(row * 128 + ((chunk ^ (row & 7)) << 4)); }
-template <class T> __device__ __forceinline__ void store_row8(const AttentionArgs &a, T *to, const float (&v)[8], float factor) {
+// 32 bytes at once: a thread has a row, so narrower stores would write parts of sectors.
+__device__ __forceinline__ void store_sector(void *to, const float (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])),
+                 "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])),
+                 "r"(__float_as_uint(v[7]))
+                 : "memory");
+}
+template <class T> __device__ __forceinline__ void store_row16(const AttentionArgs &a, T *to, const float (&v)[16], float factor) {
     union {
-        uint4 words;
-        T e[8];
+        float words[8];
+        uint4 fours[2];
+        T e[16];
     } out;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out.e[i] = T(v[i] * factor);
-    if (a.aligned) {
-        *reinterpret_cast<uint4 *>(to) = out.words;
+    for (int i = 0; i < 16; ++i) out.e[i] = T(v[i] * factor);
+    if (a.sectors) {
+        store_sector(to, out.words);
+    } else if (a.aligned) {
+        reinterpret_cast<uint4 *>(to)[0] = out.fours[0];
+        reinterpret_cast<uint4 *>(to)[1] = out.fours[1];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) to[i] = out.e[i];
+        for (int i = 0; i < 16; ++i) to[i] = out.e[i];
     }
 }
 } // namespace many
@@ -93,14 +104,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     constexpr int kRows = kManyRows, kSlots = Shape::slots, kConverter = kSoftmaxWarps, kProducer = kConverter + kConverters, kIssuer = kProducer + 1; // an issuer per team
     constexpr uint32_t kOut = 2 * kTileKeys; // tensor memory: two teams' scores, then their outputs
     extern __shared__ uint8_t raw_smem[];
-    // Tile i of the share is team i % 2's, and its barriers' use i / 2. Of each half: scored: S is done (of both: the keys' buffer is free);
-    // softmaxed: P is ready; weighted: O has it (of both: the values' buffer is free). keys/values: operands are ready. tables_ready
-    // has a use for every fourth tile: its tables are not written again before the team is done with them.
+    // Tile i of the share has buffers and barriers i % 2, and these their use i / 2. Of each team: scored: S is done (of both: the keys' buffer is
+    // free); softmaxed: P is ready; weighted: O has it (of both: the values' buffer is free). keys/values: operands are ready. tables_ready
+    // has a use for every fourth tile: its tables are not written again before the teams are done with them.
     __shared__ uint64_t raw_full[kSlots], raw_free[kSlots], keys_ready[2], values_ready[2], scored[2][2], softmaxed[2][2], weighted[2][2], tables_ready[4];
-    __shared__ uint64_t largest_known, meet, drained[2]; // once per segment part, the last once
-    // Warps that have laid down a part's queries, or read its outputs, over all parts. Counts and not phases: an issuer whose team has no tile in some
-    // parts may be several of them behind.
-    __shared__ int queries_ready, outputs_free;
+    __shared__ uint64_t queries_ready, largest_known, meet, outputs_free, drained[2]; // once per segment part, the last once
     __shared__ __align__(16) float table_key[4][kTileKeys], table_shift[4][kTileKeys], table_value[4][kTileKeys]; // of tile i: i % 4
     __shared__ float2 stats[2][kRows];
     __shared__ unsigned largest[2]; // of a part's queries, by the part's parity
@@ -132,13 +140,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             ptx::mbar_init(ptx::smem_u32(&tables_ready[2 * t + 1]), kTileKeys / 32);
             largest[t] = 0;
         }
+        ptx::mbar_init(ptx::smem_u32(&queries_ready), kConverters);
+        ptx::mbar_init(ptx::smem_u32(&outputs_free), kSoftmaxWarps);
         ptx::mbar_init(ptx::smem_u32(&largest_known), kConverters);
         ptx::mbar_init(ptx::smem_u32(&meet), kSoftmaxWarps);
         for (int p = 0; p < kPartsAhead; ++p) {
             ptx::mbar_init(ptx::smem_u32(&part_full[p]), 1);
             ptx::mbar_init(ptx::smem_u32(&part_free[p]), kSoftmaxWarps + kConverters + 2);
         }
-        abort_flag = queries_ready = outputs_free = 0;
+        abort_flag = 0;
         ptx::fence_barrier_init();
     }
     if (warp == kIssuer) ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
@@ -156,23 +166,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         if (__all_sync(0xffffffffu, ptx::mbar_wait(ptx::smem_u32(&bar), uint32_t(use) & 1, &abort_flag))) return true;
         if (!lane) *args.status = 1;
         return false;
-    };
-    auto wait_count = [&](int &count, int needed) {
-        bool reached = false;
-        const long long begun = clock64();
-        while (!(reached = *const_cast<volatile int *>(&count) >= needed) && !*const_cast<volatile int *>(&abort_flag))
-            if (clock64() - begun > ptx::kWaitLimitCycles) abort_flag = 1;
-        reached = __all_sync(0xffffffffu, reached);
-        __threadfence_block();
-        if (!reached && !lane) *args.status = 1;
-        return reached;
-    };
-    auto add_count = [&](int &count) {
-        __syncwarp();
-        if (!lane) {
-            __threadfence_block();
-            atomicAdd(&count, 1);
-        }
     };
     auto arrive = [&](uint64_t &bar) {
         __syncwarp();
@@ -269,42 +262,42 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     } else if (warp == kIssuer || warp == kIssuer + 1) { // -------------------------------------------------------------- products
         constexpr uint32_t kScoreIdesc = idesc_f16(kRows, kTileKeys / 2), kOutIdesc = idesc_f16(kRows, HeadDim);
         const int team = warp - kIssuer;
-        auto score = [&](int i, int half) { // S of half a tile, where the weights of the team's tile before stood
-            if ((!half && !wait(keys_ready[team], i >> 1)) || (i >= 2 && !wait(weighted[team][half], (i >> 1) - 1))) return false;
+        constexpr int kHalf = kTileKeys / 2;
+        auto score = [&](int i) { // S of the team's half of a tile, where the weights of the tile before the last stood
+            const int buffer = i & 1;
+            if (!wait(keys_ready[buffer], i >> 1) || (i >= 2 && !wait(weighted[team][buffer], (i >> 1) - 1))) return false;
             ptx::tcgen05_fence_after();
             if (ptx::elect_one()) {
-                const uint32_t q = ptx::smem_desc_lo_k128(base), k = ptx::smem_desc_lo_k128(base + Shape::keys + team * Shape::operand + half * (kTileKeys / 2 * 128));
+                const uint32_t q = ptx::smem_desc_lo_k128(base), k = ptx::smem_desc_lo_k128(base + Shape::keys + buffer * Shape::operand + team * (kHalf * 128));
 #pragma unroll
                 for (int s = 0; s < HeadDim / 16; ++s) {
                     const uint32_t at = uint32_t(s >> 2) * (kRows * 128 >> 4) + uint32_t(s & 3) * 2;
-                    mma_smem(tmem + team * kTileKeys + half * (kTileKeys / 2), q + at, k + at, kScoreIdesc, s > 0);
+                    mma_smem(tmem + team * kTileKeys + buffer * kHalf, q + at, k + at, kScoreIdesc, s > 0);
                 }
-                ptx::tcgen05_commit(ptx::smem_u32(&scored[team][half]));
+                ptx::tcgen05_commit(ptx::smem_u32(&scored[team][buffer]));
             }
             __syncwarp();
             return true;
         };
         for_parts([&](const SegmentPart &part) {
-            const int end = first_tile + part.high - part.low, first = first_tile + ((first_tile ^ team) & 1);
-            if (!wait_count(queries_ready, kConverters * (part.ordinal + 1))) return false;
-            if (first < end && (!score(first, 0) || !score(first, 1))) return false;
-            if (!wait_count(outputs_free, kSoftmaxWarps * part.ordinal)) return false;
-            for (int i = first; i < end; i += 2) {
+            const int first = first_tile, end = first + part.high - part.low;
+            if (!wait(queries_ready, part.ordinal)) return false;
+            if (!score(first) || (first + 1 < end && !score(first + 1))) return false;
+            if (part.ordinal && !wait(outputs_free, part.ordinal - 1)) return false;
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    if ((!half && !wait(values_ready[team], i >> 1)) || !wait(softmaxed[team][half], i >> 1)) return false;
-                    ptx::tcgen05_fence_after();
-                    if (ptx::elect_one()) {
-                        const uint32_t v = ptx::smem_desc_lo_k128(base + Shape::values + team * Shape::operand + half * (HeadDim * 128));
+            for (int i = first; i < end; ++i) {
+                const int buffer = i & 1;
+                if (!wait(values_ready[buffer], i >> 1) || !wait(softmaxed[team][buffer], i >> 1)) return false;
+                ptx::tcgen05_fence_after();
+                if (ptx::elect_one()) {
+                    const uint32_t v = ptx::smem_desc_lo_k128(base + Shape::values + buffer * Shape::operand + team * (HeadDim * 128));
 #pragma unroll
-                        for (int s = 0; s < kTileKeys / 32; ++s)
-                            mma_tmem(tmem + kOut + team * HeadDim, tmem + team * kTileKeys + half * (kTileKeys / 2) + 8 * s, v + uint32_t(s) * 2, kOutIdesc,
-                                     s > 0 || half || i > first);
-                        ptx::tcgen05_commit(ptx::smem_u32(&weighted[team][half]));
-                    }
-                    __syncwarp();
-                    if (i + 2 < end && !score(i + 2, half)) return false;
+                    for (int s = 0; s < kHalf / 16; ++s)
+                        mma_tmem(tmem + kOut + team * HeadDim, tmem + team * kTileKeys + buffer * kHalf + 8 * s, v + uint32_t(s) * 2, kOutIdesc, s > 0 || i > first);
+                    ptx::tcgen05_commit(ptx::smem_u32(&weighted[team][buffer]));
                 }
+                __syncwarp();
+                if (i + 2 < end && !score(i + 2)) return false;
             }
             first_tile = end;
             return true;
@@ -324,7 +317,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             // Queries, once the products of the part before have read theirs. Rows past the segment are zero. BF16 rows are divided by the power of
             // two of their largest element of all, which brings them into fp16's range; what that costs the small ones is small next to the others.
             for (int i = max(0, first_tile - 2); i < first_tile; ++i)
-                if (!wait(scored[i & 1][1], i >> 1)) return false;
+                if (!wait(scored[0][i & 1], i >> 1) || !wait(scored[1][i & 1], i >> 1)) return false;
             constexpr int kChunks = HeadDim / 8, kTurns = kRows * kChunks / (32 * kConverters); // kChunks: threads to a row
             const int flat = part.query_tile * kRows, chunk = thread % kChunks;
             const auto place = [&](int i) { // where this thread's piece of turn i goes; rows of a turn are a multiple of eight apart
@@ -382,15 +375,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 }
             }
             ptx::fence_proxy_async_smem();
-            add_count(queries_ready);
+            arrive(queries_ready);
             if (thread == 0) largest[~part.ordinal & 1] = 0; // everyone has read the part before's
 
             const float score_scale = args.score_scale * scale_up;
             auto convert_keys = [&](int i) {
-                const int team = i & 1, before = (i >> 1) - 1;
-                if (!wait(raw_full[slot], use) || (before >= 0 && !wait(scored[team][1], before))) return false;
+                const int buffer = i & 1, before = (i >> 1) - 1;
+                if (!wait(raw_full[slot], use) || (before >= 0 && (!wait(scored[0][buffer], before) || !wait(scored[1][buffer], before)))) return false;
                 {
-                    const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::keys + team * Shape::operand;
+                    const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::keys + buffer * Shape::operand;
                     constexpr int kPieces = HeadDim / 16, kTurns = kTileKeys * kPieces / (32 * kConverters); // kPieces: lanes to a key row
                     uint32_t w[kTurns][4];
 #pragma unroll
@@ -426,15 +419,15 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     }
                 }
                 ptx::fence_proxy_async_smem();
-                arrive(keys_ready[team]);
+                arrive(keys_ready[buffer]);
                 next_slot();
                 return true;
             };
             auto convert_values = [&](int i) {
-                const int team = i & 1, before = (i >> 1) - 1;
-                if (!wait(raw_full[slot], use) || (before >= 0 && !wait(weighted[team][1], before))) return false;
+                const int buffer = i & 1, before = (i >> 1) - 1;
+                if (!wait(raw_full[slot], use) || (before >= 0 && (!wait(weighted[0][buffer], before) || !wait(weighted[1][buffer], before)))) return false;
                 {
-                    const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::values + team * Shape::operand;
+                    const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::values + buffer * Shape::operand;
                     // A lane takes four columns (a word) of eight keys, and stores eight keys of each column. Pairs of lanes take other groups of keys, so that
                     // eight lanes meet eight banks when they store.
                     constexpr int kWords = HeadDim / 4, kSets = 32 * kConverters / kWords, kTurns = kTileKeys / 8 / kSets; // kSets: threads that share a word
@@ -463,7 +456,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     }
                 }
                 ptx::fence_proxy_async_smem();
-                arrive(values_ready[team]);
+                arrive(values_ready[buffer]);
                 next_slot();
                 return true;
             };
@@ -492,17 +485,16 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 most[r] = -INFINITY, sum[r] = 0.f;
             }
             least = __reduce_min_sync(0xffffffffu, least);
-            int last = -1;
-            for (int i = first_tile + ((first_tile ^ team) & 1); i < end; i += 2) {
 #pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
+            for (int i = first_tile; i < end; ++i) {
+                {
                     constexpr int kHalf = kTileKeys / 2;
-                    const int key = (part.low + i - first_tile) * kTileKeys + half * kHalf + 2 * t;
-                    const uint32_t at = at_scores + half * kHalf;
-                    const float *const of_key = table_key[i & 3] + half * kHalf + 2 * t, *const of_shift = table_shift[i & 3] + half * kHalf + 2 * t,
-                                      *const of_value = table_value[i & 3] + half * kHalf + 2 * t;
+                    const int buffer = i & 1, key = (part.low + i - first_tile) * kTileKeys + team * kHalf + 2 * t;
+                    const uint32_t at = at_scores + buffer * kHalf;
+                    const float *const of_key = table_key[i & 3] + team * kHalf + 2 * t, *const of_shift = table_shift[i & 3] + team * kHalf + 2 * t,
+                                      *const of_value = table_value[i & 3] + team * kHalf + 2 * t;
                     const bool masked = key - 2 * t + kHalf - 1 > least;
-                    if (!wait(scored[team][half], i >> 1) || (!half && !wait(tables_ready[i & 3], i >> 2))) return false;
+                    if (!wait(scored[team][buffer], i >> 1) || !wait(tables_ready[i & 3], i >> 2)) return false;
                     ptx::tcgen05_fence_after();
                     // 16 rows by 32 columns at a time, the next ones on their way while these are worked on.
                     const auto place = [&](int unit) { return at + uint32_t(unit >> 1) * 32 + (uint32_t(unit & 1) << 20); };
@@ -550,8 +542,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                             if (its) most[r] = highest[r];
                             sum[r] *= factor;
                         }
-                        if (last >= 0 || half) { // this team's output so far, once the product before this half is in it
-                            if (!wait(weighted[team][half ^ 1], (half ? i : last) >> 1)) return false;
+                        if (i > first_tile) { // this team's output so far, once the product before this one is in it
+                            if (!wait(weighted[team][buffer ^ 1], (i - 1) >> 1)) return false;
                             ptx::tcgen05_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < HeadDim; c += 16) {
@@ -612,35 +604,23 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                         sum[r] += x + y; // of this lane's columns
                     }
                     ptx::tcgen05_fence_before();
-                    arrive(softmaxed[team][half]);
+                    arrive(softmaxed[team][buffer]);
                 }
-                last = i;
             }
-            if (last >= 0) {
-                if (!wait(weighted[team][1], last >> 1)) return false;
+            if (!wait(weighted[team][(end - 1) & 1], (end - 1) >> 1)) return false;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-                    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                    if (!t) stats[team][32 * (warp & 3) + 8 * r + g] = make_float2(most[r], sum[r]);
-                }
+            for (int r = 0; r < 4; ++r) {
+                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+                sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+                if (!t) stats[team][32 * (warp & 3) + 8 * r + g] = make_float2(most[r], sum[r]);
             }
             arrive(meet);
             if (!wait(meet, part.ordinal)) return false;
             ptx::tcgen05_fence_after();
-            // Both teams' outputs; each team stores one half of the columns. A part of one tile has one team's only.
-            const bool has[2] = {count > 1 || !(first_tile & 1), count > 1 || (first_tile & 1)};
-            float highest = -INFINITY, l = 0.f, factor[2] = {0.f, 0.f};
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (has[t]) highest = fmaxf(highest, stats[t][row].x);
-            const float reference = highest == -INFINITY ? 0.f : highest;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (has[t]) {
-                    factor[t] = exp2_approx(stats[t][row].x - reference);
-                    l += factor[t] * stats[t][row].y;
-                }
+            // Both teams' outputs; each team stores one half of the columns.
+            const float2 mine[2] = {stats[0][row], stats[1][row]};
+            const float highest = fmaxf(mine[0].x, mine[1].x), reference = highest == -INFINITY ? 0.f : highest;
+            const float factor[2] = {exp2_approx(mine[0].x - reference), exp2_approx(mine[1].x - reference)}, l = factor[0] * mine[0].y + factor[1] * mine[1].y;
             const int head = part.head * args.group + flat % args.group;
             const size_t at_row = size_t(part.s.row) + flat / args.group, index = at_row * args.heads + head;
             float *kept = part.split      ? args.partials + (size_t(blockIdx.x * 2 + part.slot) * args.part_columns + row) * (HeadDim + kPartialExtra)
@@ -650,26 +630,18 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
 #pragma unroll 1
             for (int c = team * (HeadDim / 2); c < (team + 1) * (HeadDim / 2); c += 16) {
                 uint32_t o[2][16];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (has[t]) ptx::tmem_load16(at_out + t * HeadDim + c, o[t]);
-                    else
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) o[t][j] = 0;
-                }
+                ptx::tmem_load16(at_out + c, o[0]);
+                ptx::tmem_load16(at_out + HeadDim + c, o[1]);
                 ptx::tmem_load_wait();
                 if (!live) continue;
+                float v[16];
 #pragma unroll
-                for (int j = 0; j < 16; j += 8) {
-                    float v[8];
+                for (int e = 0; e < 16; ++e) v[e] = factor[0] * __uint_as_float(o[0][e]) + factor[1] * __uint_as_float(o[1][e]);
+                if (kept) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = factor[0] * __uint_as_float(o[0][j + e]) + factor[1] * __uint_as_float(o[1][j + e]);
-                    if (kept) {
-                        *reinterpret_cast<float4 *>(kept + c + j) = make_float4(v[0], v[1], v[2], v[3]);
-                        *reinterpret_cast<float4 *>(kept + c + j + 4) = make_float4(v[4], v[5], v[6], v[7]);
-                    } else {
-                        store_row8(args, static_cast<T *>(args.output) + at_row * args.output_stride + size_t(head) * HeadDim + c + j, v, scale);
-                    }
+                    for (int e = 0; e < 16; e += 8) store_sector(kept + c + e, *reinterpret_cast<const float(*)[8]>(v + e));
+                } else {
+                    store_row16(args, static_cast<T *>(args.output) + at_row * args.output_stride + size_t(head) * HeadDim + c, v, scale);
                 }
             }
             if (live && !team) {
@@ -679,7 +651,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 else if (part.first_cta >= 0) args.table[index] = make_int4(part.first_cta, int(blockIdx.x) - part.first_cta + 1, part.first_slot, row);
             }
             ptx::tcgen05_fence_before();
-            add_count(outputs_free);
+            arrive(outputs_free);
             first_tile = end;
             return true;
         });

@@ -13,7 +13,7 @@
 
 namespace tts::b200 {
 constexpr int kTileKeys = 128;
-constexpr int kPartialExtra = 4; // maximum and sum behind a partial row, padded to 16 bytes
+constexpr int kPartialExtra = 8; // maximum and sum behind a partial row, padded to a sector of 32 bytes
 constexpr int kScanAlone = 256;  // up to here a warp adds the sequences' work up by itself
 constexpr size_t kAttentionSmem = 224 * 1024;
 
@@ -27,7 +27,7 @@ struct AttentionArgs {
     const void *queries;
     void *output;
     int query_stride, output_stride, rows, heads, group, kv_heads;
-    bool aligned;
+    bool aligned, sectors; // rows of 16-bit elements start on 16 bytes; output rows on 32
     const int *pages, *lengths, *query_offsets;
     int sequences, page_columns, page_stride, page_shift, total_pages, box_shift;
     int offset_count; // entries of query_offsets behind the first; the last one counts the rows
