@@ -594,16 +594,29 @@ template <int HeadDim> struct RowSum {
     static constexpr int kRow = HeadDim + kPartialExtra, kShare = HeadDim / 32;
     float highest = -INFINITY, l = 0.f, v[kShare] = {};
 
-    // 32 parts at a time: a lane reads the maximum and the sum of one, so that the rows' loads depend on nothing but the loop.
+    static __device__ __forceinline__ void read(const float *from, float (&x)[kShare]) {
+        if constexpr (kShare == 4) {
+            const float4 w = *reinterpret_cast<const float4 *>(from);
+            x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+        } else {
+            const float2 w = *reinterpret_cast<const float2 *>(from);
+            x[0] = w.x, x[1] = w.y;
+        }
+    }
+    // 32 parts at a time: a lane reads the maximum and the sum of one, and the first parts' rows are on their way meanwhile.
     template <class PartOf> __device__ __forceinline__ void add(int parts, PartOf &&part_of) {
+        constexpr int kAhead = 8;
         const int lane = threadIdx.x & 31;
         for (int first = 0; first < parts; first += 32) {
             const int count = min(32, parts - first);
-            float most = -INFINITY, sum = 0.f;
+            float most = -INFINITY, sum = 0.f, ahead[kAhead][kShare];
             if (lane < count) {
                 const float2 stats = *reinterpret_cast<const float2 *>(part_of(first + lane) + HeadDim);
                 most = stats.x, sum = stats.y;
             }
+#pragma unroll
+            for (int part = 0; part < kAhead; ++part)
+                if (part < count) read(part_of(first + part) + kShare * lane, ahead[part]);
             float raised = most;
 #pragma unroll
             for (int d = 16; d; d >>= 1) raised = fmaxf(raised, __shfl_xor_sync(0xffffffffu, raised, d));
@@ -617,18 +630,18 @@ template <int HeadDim> struct RowSum {
 #pragma unroll
             for (int c = 0; c < kShare; ++c) v[c] *= shrink;
             highest = raised;
+#pragma unroll
+            for (int part = 0; part < kAhead; ++part) {
+                if (part >= count) break;
+                const float f = __shfl_sync(0xffffffffu, factor, part);
+#pragma unroll
+                for (int c = 0; c < kShare; ++c) v[c] += ahead[part][c] * f;
+            }
 #pragma unroll 8
-            for (int part = 0; part < count; ++part) {
-                const float *from = part_of(first + part) + kShare * lane;
+            for (int part = kAhead; part < count; ++part) {
                 const float f = __shfl_sync(0xffffffffu, factor, part);
                 float x[kShare];
-                if constexpr (kShare == 4) {
-                    const float4 w = *reinterpret_cast<const float4 *>(from);
-                    x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-                } else {
-                    const float2 w = *reinterpret_cast<const float2 *>(from);
-                    x[0] = w.x, x[1] = w.y;
-                }
+                read(part_of(first + part) + kShare * lane, x);
 #pragma unroll
                 for (int c = 0; c < kShare; ++c) v[c] += x[c] * f;
             }
