@@ -221,3 +221,91 @@ def test_refusals(ctx_factory):
     with pytest.raises(_lib.B200QError, match="workspace of"):
         small.cached_attention(q, batch.cache, pages, lengths, out)
     small.close()
+
+
+def many(counts=(70, 40), **other):
+    """More than sixteen query rows of a cached head: the tensor memory's kernel."""
+    lengths = [n + 100 for n in counts]
+    return Batch(30, lengths, list(counts), **{"heads": 4, "kv_heads": 2, "page": 16, **other})
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_many_rows_with_missing_pages_and_rows_that_are_no_numbers(ctx_factory, fmt, head_dim):
+    batch = many(fmt=FORMATS[fmt], head_dim=head_dim)
+    batch.pages[0, 6] = 10**6  # positions 96 to 111 of 170: seen by all
+    batch.pages[1, 8] = -3  # positions 128 to 139: by the last twelve queries
+    page = batch.pages[1, 7].item()
+    batch.cache.value_scales[page, 1, 10] = float("nan")  # position 122: by the last eighteen, of one cached head
+    batch.cache.key_scales[page, 0, 11] = float("nan")
+    got, (want, bound) = batch.run(ctx_factory("int8")), batch.want()
+    check(got, want, bound)
+    assert torch.isnan(want[:70]).all() and not torch.isnan(want[70:90]).any() and torch.isnan(want[-1]).all()
+
+
+@pytest.mark.parametrize("spread", [8.0, 20.0])
+def test_many_rows_with_scales_far_apart(ctx_factory, spread):
+    batch = many(fmt=ops.I8)
+    g = torch.Generator().manual_seed(9)
+    batch.cache.value_scales.mul_(torch.exp(torch.randn(batch.cache.value_scales.shape, generator=g) * spread / 2).cuda())
+    check(batch.run(ctx_factory("int8")), *batch.want())
+
+
+@pytest.mark.parametrize("power", [-90, 100])
+def test_many_rows_of_any_magnitude(ctx_factory, power):
+    batch = many()
+    batch.q = (batch.q.double() * 2.0**power).bfloat16()
+    scale = 2.0**-power * 0.05
+    check(batch.run(ctx_factory("int8"), scale=scale), *batch.want(scale))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_strided(ctx_factory, dtype):
+    batch = many(head_dim=64, dtype=DTYPES[dtype])
+    want, bound = batch.want(0.3)
+    rows = batch.q.shape[0]
+    for shift in (0, 3, 8):  # 16-byte alignment for the last, 32 for the first only
+        packed = torch.full((rows, 4 * 64 + 40), 9.0, dtype=batch.q.dtype, device="cuda")
+        held = torch.full((rows, 4 * 64 + 24), 9.0, dtype=batch.q.dtype, device="cuda")
+        q, out = packed[:, shift: shift + 256], held[:, shift: shift + 256]
+        q.copy_(batch.q)
+        check(batch.run(ctx_factory("int8"), out=out, q=q, scale=0.3), want, bound)
+        assert (held[:, :shift] == 9).all() and (held[:, shift + 256:] == 9).all()
+
+
+def test_references_that_rise_late(ctx_factory):
+    """Scores that grow by far more than the weights' range from tile to tile: the outputs so far are rescaled, again and again."""
+    for batch in (many((130,), page=64, head_dim=128), Batch(31, [700], None, heads=2, kv_heads=1, page=64, head_dim=128),
+                  many((40, 30), page=64, head_dim=64, prefix=600)):
+        shape = batch.cache.key_scales.shape
+        tables = [t for t in ([batch.pages] if batch.prefix_pages is None else [batch.prefix_pages[None], batch.pages])]
+        for table in tables:
+            for row in table.tolist():
+                for i, p in enumerate(row):
+                    if 0 <= p < shape[0]:
+                        batch.cache.key_scales[p] *= 1.6 ** i
+        check(batch.run(ctx_factory("int8")), *batch.want())
+
+
+def test_strided_page_tables(ctx_factory):
+    batch = Batch(32, [130, 31, 77, 0], None, page=32)
+    wide = torch.full((4, 3 * batch.pages.shape[1] + 1), 7 * 10**5, dtype=torch.int32)
+    part = wide[:, 2: 2 + batch.pages.shape[1]]
+    part.copy_(batch.pages)
+    on_device = wide.cuda()[:, 2: 2 + batch.pages.shape[1]]
+    out = batch.out.cuda()
+    ctx = ctx_factory("int8")
+    ctx.cached_attention(batch.q.cuda(), batch.cache, on_device, torch.tensor(batch.lengths, dtype=torch.int32, device="cuda"), out)
+    check(out, *batch.want())
+
+
+def test_offsets_that_are_none(ctx_factory):
+    """Offsets that fall, or lie outside of the rows, name rows inside of them or none: nothing else is written, nothing waits for good."""
+    batch = Batch(33, [60, 60, 60], [2, 2, 2], spare_rows=4)
+    lengths = torch.tensor(batch.lengths, dtype=torch.int32, device="cuda")
+    ctx, held = ctx_factory("int8"), torch.full((14, batch.q.shape[1]), 5.0, dtype=batch.q.dtype, device="cuda")
+    for offsets in ([0, 4, 2, 6], [0, 2, 4, 99], [-3, 2, 4, 6], [6, 4, 2, 0], [2**31 - 1, -(2**31), 5, 5]):
+        ctx.cached_attention(batch.q.cuda(), batch.cache, batch.pages.cuda(), lengths, held[2:12],
+                             query_offsets=torch.tensor(offsets, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        assert ctx.status() == 0 and (held[:2] == 5).all() and (held[12:] == 5).all()
