@@ -224,7 +224,7 @@ def test_refusals(ctx_factory):
 
 
 def many(counts=(70, 40), **other):
-    """More than sixteen query rows of a cached head: the tensor memory's kernel."""
+    """More than 32 query rows of a cached head: the tensor memory's kernel."""
     lengths = [n + 100 for n in counts]
     return Batch(30, lengths, list(counts), **{"heads": 4, "kv_heads": 2, "page": 16, **other})
 
