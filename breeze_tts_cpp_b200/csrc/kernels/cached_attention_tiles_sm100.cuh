@@ -5,8 +5,8 @@
 // when a tile's maximum passes it by 2^8, so that the accumulated output is rescaled hardly ever.
 //
 // Layout. A segment is 128 query rows of one cached head (tokens times the group's heads; of a prefix: of all sequences), a tile 128 keys. Per tile
-// a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Two teams of four
-// softmax warps, 32 rows a warp, take one half of a tile's keys each, and each team has a softmax state, an output and an issuing warp of its own;
+// a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Two teams of eight
+// softmax warps, 16 rows a warp, take one half of a tile's keys each, and each team has a softmax state, an output and an issuing warp of its own;
 // they meet once per segment. A team has the scores of two tiles, so that the products of one run while it works on the other. Eight warps turn
 // bytes into fp16 operands: keys as they are, values transposed, so that both are K-major with the 128-byte swizzle. Tables of a tile's scales go
 // to the softmax warps through shared memory.
@@ -19,11 +19,7 @@
 namespace tts::b200 {
 constexpr int kManyRows = 128;
 constexpr int kManySegmentUnits = 12; // filling and draining the pipeline, the meeting of the teams and the store, next to a tile's kTileUnits
-constexpr int kSoftmaxWarps = 8, kConverters = 8, kManyWarps = kSoftmaxWarps + kConverters + 4, kManyThreads = 32 * kManyWarps; // one warp idles
-// Registers a thread: 96 at launch (61440 in all); two groups of four warps each for the softmax and the conversions, one for the rest. The
-// shares add up to the launch's: 256 x 144 + 256 x 64 + 128 x 64.
-constexpr int kSoftmaxRegisters = 144, kOtherRegisters = 64;
-static_assert(32 * kSoftmaxWarps * kSoftmaxRegisters + (kManyThreads - 32 * kSoftmaxWarps) * kOtherRegisters == kManyThreads * 96);
+constexpr int kSoftmaxWarps = 16, kConverters = 8, kManyWarps = kSoftmaxWarps + kConverters + 3, kManyThreads = 32 * kManyWarps; // 72 registers a thread
 constexpr int kPartsAhead = 4;
 constexpr float kReferenceSlack = 8.f; // powers of two that a weight may exceed one by
 
@@ -49,8 +45,9 @@ __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint32_t b_lo, 
                  "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(ptx::kDescHiK128)
                  : "memory");
 }
-__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+// The fragment of tmem_load_rows16<32> back to where it came from.
+__device__ __forceinline__ void tmem_store_scores16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
                  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
@@ -62,8 +59,6 @@ __device__ __forceinline__ void tmem_store_rows16(uint32_t taddr, const uint32_t
                  : "memory");
 }
 __device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) { return ptx::pack2(__uint_as_float(lo), __uint_as_float(hi)); }
-template <int Registers> __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Registers)); }
-template <int Registers> __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Registers)); }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -183,8 +178,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     };
     int first_tile = 0; // of the part, in the share
 
-    if (warp < kSoftmaxWarps) take_registers<kSoftmaxRegisters>();
-    else give_registers<kOtherRegisters>();
     if (warp == kProducer) { // ------------------------------------------------------------------ bytes and scales
         const int box = 1 << args.box_shift, boxes = kTileKeys >> args.box_shift;
         int slot = 0, item = 0, reuse = -1; // reuse: the slot's use before this one
@@ -467,19 +460,21 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             return true;
         });
     } else if (warp < kSoftmaxWarps) { // --------------------------------------------------------- softmax
-        // Scores are read as matrix fragments: lane l has rows l / 4 + 8 r of the warp's 32 and of each eight columns the two at 2 (l % 4), so that a
+        // Scores are read as matrix fragments: lane l has rows l / 4 and l / 4 + 8 of the warp's 16 and of each eight columns the two at 2 (l % 4), so that a
         // thread needs a quarter of the columns' scales. With a row per thread every scale went to every thread, and the shared memory's bandwidth, which
         // the products' operands need, was what a tile waited for.
-        const int team = warp >> 2, row = 32 * (warp & 3) + lane, g = lane >> 2, t = lane & 3;
-        const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16, at_scores = tmem + lanes + team * kTileKeys, at_out = tmem + lanes + kOut;
+        const int team = warp >> 3, block = warp >> 2 & 1, row = 32 * (warp & 3) + lane, g = lane >> 2, t = lane & 3;
+        const int first_row = 32 * (warp & 3) + 16 * block + g; // this lane's rows: this one, and eight further on
+        const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16, block_lanes = lanes + (uint32_t(block) << 20), at_out = tmem + lanes + kOut;
+        const uint32_t at_scores = tmem + block_lanes + team * kTileKeys, own_out = tmem + block_lanes + kOut + team * HeadDim;
         for_parts([&](const SegmentPart &part) {
             const int count = part.high - part.low, end = first_tile + count, flat = part.query_tile * kRows + row;
             const bool live = row < part.columns;
-            int limit[4], least = INT_MAX; // the last position that a row sees
-            float most[4], sum[4];
+            int limit[2], least = INT_MAX; // the last position that a row sees
+            float most[2], sum[2];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int its_row = 32 * (warp & 3) + 8 * r + g, token = (part.query_tile * kRows + its_row) / args.group;
+            for (int r = 0; r < 2; ++r) {
+                const int its_row = first_row + 8 * r, token = (part.query_tile * kRows + its_row) / args.group;
                 limit[r] = its_row >= part.columns ? -1 : args.prefix ? part.s.length - 1 : part.s.length - part.s.count + token;
                 if (its_row < part.columns) least = min(least, limit[r]);
                 most[r] = -INFINITY, sum[r] = 0.f;
@@ -487,137 +482,126 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             least = __reduce_min_sync(0xffffffffu, least);
 #pragma unroll 1
             for (int i = first_tile; i < end; ++i) {
-                {
-                    constexpr int kHalf = kTileKeys / 2;
-                    const int buffer = i & 1, key = (part.low + i - first_tile) * kTileKeys + team * kHalf + 2 * t;
-                    const uint32_t at = at_scores + buffer * kHalf;
-                    const float *const of_key = table_key[i & 3] + team * kHalf + 2 * t, *const of_shift = table_shift[i & 3] + team * kHalf + 2 * t,
-                                      *const of_value = table_value[i & 3] + team * kHalf + 2 * t;
-                    const bool masked = key - 2 * t + kHalf - 1 > least;
-                    if (!wait(scored[team][buffer], i >> 1) || !wait(tables_ready[i & 3], i >> 2)) return false;
-                    ptx::tcgen05_fence_after();
-                    // 16 rows by 32 columns at a time, the next ones on their way while these are worked on.
-                    const auto place = [&](int unit) { return at + uint32_t(unit >> 1) * 32 + (uint32_t(unit & 1) << 20); };
-                    float highest[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto find_highest = [&](auto masked_tile) {
-                        constexpr bool kMasked = decltype(masked_tile)::value;
-                        uint32_t s[2][16];
-                        ptx::tmem_load_rows16<32>(place(0), s[0]);
+                constexpr int kHalf = kTileKeys / 2;
+                const int buffer = i & 1, key = (part.low + i - first_tile) * kTileKeys + team * kHalf + 2 * t;
+                const uint32_t at = at_scores + buffer * kHalf;
+                const float *const of_key = table_key[i & 3] + team * kHalf + 2 * t, *const of_shift = table_shift[i & 3] + team * kHalf + 2 * t,
+                                  *const of_value = table_value[i & 3] + team * kHalf + 2 * t;
+                const bool masked = key - 2 * t + kHalf - 1 > least;
+                if (!wait(scored[team][buffer], i >> 1) || !wait(tables_ready[i & 3], i >> 2)) return false;
+                ptx::tcgen05_fence_after();
+                // 32 columns at a time, the next ones on their way while these are worked on.
+                float highest[2] = {-INFINITY, -INFINITY};
+                auto find_highest = [&](auto masked_tile) {
+                    constexpr bool kMasked = decltype(masked_tile)::value;
+                    uint32_t s[2][16];
+                    ptx::tmem_load_rows16<32>(at, s[0]);
 #pragma unroll
-                        for (int unit = 0; unit < 4; ++unit) {
-                            const int c = (unit >> 1) * 32, b = unit & 1;
-                            ptx::tmem_load_wait();
-                            if (unit < 3) ptx::tmem_load_rows16<32>(place(unit + 1), s[(unit + 1) & 1]);
+                    for (int unit = 0; unit < kHalf / 32; ++unit) {
+                        const int c = unit * 32;
+                        ptx::tmem_load_wait();
+                        if (unit + 1 < kHalf / 32) ptx::tmem_load_rows16<32>(at + c + 32, s[(unit + 1) & 1]);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), shift = *reinterpret_cast<const uint64_t *>(of_shift + c + 8 * j);
+                        for (int j = 0; j < 4; ++j) {
+                            const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), shift = *reinterpret_cast<const uint64_t *>(of_shift + c + 8 * j);
 #pragma unroll
-                                for (int r = 0; r < 2; ++r) {
-                                    float x, y;
-                                    ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, shift), x, y);
-                                    if (kMasked && key + c + 8 * j > limit[2 * b + r]) x = -INFINITY;
-                                    if (kMasked && key + c + 8 * j + 1 > limit[2 * b + r]) y = -INFINITY;
-                                    highest[2 * b + r] = fmaxf(highest[2 * b + r], fmaxf(x, y));
-                                }
+                            for (int r = 0; r < 2; ++r) {
+                                float x, y;
+                                ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, shift), x, y);
+                                if (kMasked && key + c + 8 * j > limit[r]) x = -INFINITY;
+                                if (kMasked && key + c + 8 * j + 1 > limit[r]) y = -INFINITY;
+                                highest[r] = fmaxf(highest[r], fmaxf(x, y));
                             }
                         }
-                    };
-                    if (masked) find_highest(std::true_type{});
-                    else find_highest(std::false_type{});
-                    bool raise = false; // also from no reference at all
+                    }
+                };
+                if (masked) find_highest(std::true_type{});
+                else find_highest(std::false_type{});
+                // The reference rises where a row's maximum passes it, and from none at all.
+                if (__any_sync(0xffffffffu, highest[0] > most[0] + kReferenceSlack || highest[1] > most[1] + kReferenceSlack)) {
+                    float shrink[2];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) raise |= highest[r] > most[r] + kReferenceSlack;
-                    if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) { // over the row's four lanes
-                            highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 1));
-                            highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 2));
-                        }
-                        float shrink = 1.f; // of row `lane`
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const bool its = highest[r] > most[r] + kReferenceSlack;
-                            const float factor = its ? exp2_approx(most[r] - highest[r]) : 1.f, other = __shfl_sync(0xffffffffu, factor, 4 * (lane & 7));
-                            if (lane >> 3 == r) shrink = other;
-                            if (its) most[r] = highest[r];
-                            sum[r] *= factor;
-                        }
-                        if (i > first_tile) { // this team's output so far, once the product before this one is in it
-                            if (!wait(weighted[team][buffer ^ 1], (i - 1) >> 1)) return false;
-                            ptx::tcgen05_fence_after();
+                    for (int r = 0; r < 2; ++r) {
+                        highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 1)); // over the row's four lanes
+                        highest[r] = fmaxf(highest[r], __shfl_xor_sync(0xffffffffu, highest[r], 2));
+                        const bool its = highest[r] > most[r] + kReferenceSlack;
+                        shrink[r] = its ? exp2_approx(most[r] - highest[r]) : 1.f;
+                        if (its) most[r] = highest[r];
+                        sum[r] *= shrink[r];
+                    }
+                    if (i > first_tile) { // this team's output so far, once the product before this one is in it
+                        if (!wait(weighted[team][buffer ^ 1], (i - 1) >> 1)) return false;
+                        ptx::tcgen05_fence_after();
 #pragma unroll 1
-                            for (int c = 0; c < HeadDim; c += 16) {
-                                uint32_t o[16];
-                                ptx::tmem_load16(at_out + team * HeadDim + c, o);
-                                ptx::tmem_load_wait();
-#pragma unroll
-                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink);
-                                tmem_store16(at_out + team * HeadDim + c, o);
-                            }
-                        }
-                    }
-                    uint64_t minus[4], total[4] = {};
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float reference = most[r] == -INFINITY ? 0.f : most[r];
-                        minus[r] = ptx::pack2(-reference, -reference);
-                    }
-                    auto weigh = [&](auto masked_tile) {
-                        constexpr bool kMasked = decltype(masked_tile)::value;
-                        uint32_t s[2][16];
-                        ptx::tmem_load_rows16<32>(place(0), s[0]);
-#pragma unroll
-                        for (int unit = 0; unit < 4; ++unit) {
-                            const int c = (unit >> 1) * 32, b = unit & 1;
+                        for (int c = 0; c < HeadDim; c += 32) {
+                            uint32_t o[16];
+                            ptx::tmem_load_rows16<32>(own_out + c, o);
                             ptx::tmem_load_wait();
-                            if (unit < 3) ptx::tmem_load_rows16<32>(place(unit + 1), s[(unit + 1) & 1]);
-                            uint32_t p[8];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), v = *reinterpret_cast<const uint64_t *>(of_value + c + 8 * j);
-#pragma unroll
-                                for (int r = 0; r < 2; ++r) {
-                                    const int mine = 2 * b + r;
-                                    float x, y;
-                                    ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, minus[mine]), x, y);
-                                    const bool hide_x = kMasked && key + c + 8 * j > limit[mine], hide_y = kMasked && key + c + 8 * j + 1 > limit[mine];
-                                    const uint64_t both = ptx::pack2(exp2_approx(hide_x ? -INFINITY : x), exp2_approx(hide_y ? -INFINITY : y));
-                                    total[mine] = ptx::add2(total[mine], both);
-                                    ptx::unpack2(ptx::mul2(both, v), x, y);
-                                    if (hide_x) x = 0.f; // a hidden row's scale may be anything
-                                    if (hide_y) y = 0.f;
-                                    const __half2 w = __floats2half2_rn(x, y);
-                                    p[2 * j + r] = *reinterpret_cast<const uint32_t *>(&w);
-                                }
-                            }
-                            // Over scores that have been read: those still to come lie behind these columns, or in other rows.
-                            tmem_store_rows16(at + c / 2 + (uint32_t(b) << 20), p);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * shrink[j >> 1 & 1]);
+                            tmem_store_scores16(own_out + c, o);
                         }
-                    };
-                    if (masked) weigh(std::true_type{});
-                    else weigh(std::false_type{});
-                    tmem_store_wait();
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float x, y;
-                        ptx::unpack2(total[r], x, y);
-                        sum[r] += x + y; // of this lane's columns
                     }
-                    ptx::tcgen05_fence_before();
-                    arrive(softmaxed[team][buffer]);
                 }
+                uint64_t minus[2], total[2] = {};
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float reference = most[r] == -INFINITY ? 0.f : most[r];
+                    minus[r] = ptx::pack2(-reference, -reference);
+                }
+                auto weigh = [&](auto masked_tile) {
+                    constexpr bool kMasked = decltype(masked_tile)::value;
+                    uint32_t s[2][16];
+                    ptx::tmem_load_rows16<32>(at, s[0]);
+#pragma unroll
+                    for (int unit = 0; unit < kHalf / 32; ++unit) {
+                        const int c = unit * 32;
+                        ptx::tmem_load_wait();
+                        if (unit + 1 < kHalf / 32) ptx::tmem_load_rows16<32>(at + c + 32, s[(unit + 1) & 1]);
+                        uint32_t p[8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint64_t k = *reinterpret_cast<const uint64_t *>(of_key + c + 8 * j), v = *reinterpret_cast<const uint64_t *>(of_value + c + 8 * j);
+#pragma unroll
+                            for (int r = 0; r < 2; ++r) {
+                                float x, y;
+                                ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, minus[r]), x, y);
+                                const bool hide_x = kMasked && key + c + 8 * j > limit[r], hide_y = kMasked && key + c + 8 * j + 1 > limit[r];
+                                const uint64_t both = ptx::pack2(exp2_approx(hide_x ? -INFINITY : x), exp2_approx(hide_y ? -INFINITY : y));
+                                total[r] = ptx::add2(total[r], both);
+                                ptx::unpack2(ptx::mul2(both, v), x, y);
+                                if (hide_x) x = 0.f; // a hidden row's scale may be anything
+                                if (hide_y) y = 0.f;
+                                const __half2 w = __floats2half2_rn(x, y);
+                                p[2 * j + r] = *reinterpret_cast<const uint32_t *>(&w);
+                            }
+                        }
+                        tmem_store_rows16(at + c / 2, p); // over scores that have been read: those still to come lie behind these columns
+                    }
+                };
+                if (masked) weigh(std::true_type{});
+                else weigh(std::false_type{});
+                tmem_store_wait();
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    float x, y;
+                    ptx::unpack2(total[r], x, y);
+                    sum[r] += x + y; // of this lane's columns
+                }
+                ptx::tcgen05_fence_before();
+                arrive(softmaxed[team][buffer]);
             }
             if (!wait(weighted[team][(end - 1) & 1], (end - 1) >> 1)) return false;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < 2; ++r) {
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
                 sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-                if (!t) stats[team][32 * (warp & 3) + 8 * r + g] = make_float2(most[r], sum[r]);
+                if (!t) stats[team][first_row + 8 * r] = make_float2(most[r], sum[r]);
             }
             arrive(meet);
             if (!wait(meet, part.ordinal)) return false;
             ptx::tcgen05_fence_after();
-            // Both teams' outputs; each team stores one half of the columns.
+            // Both teams' outputs, a thread to a row now; the four warps of its rows store a quarter of the columns each.
             const float2 mine[2] = {stats[0][row], stats[1][row]};
             const float highest = fmaxf(mine[0].x, mine[1].x), reference = highest == -INFINITY ? 0.f : highest;
             const float factor[2] = {exp2_approx(mine[0].x - reference), exp2_approx(mine[1].x - reference)}, l = factor[0] * mine[0].y + factor[1] * mine[1].y;
@@ -628,7 +612,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                                           : nullptr;
             const float scale = l == 0.f ? 0.f : args.output_scale / l;
 #pragma unroll 1
-            for (int c = team * (HeadDim / 2); c < (team + 1) * (HeadDim / 2); c += 16) {
+            for (int c = (warp >> 2) * (HeadDim / 4); c < ((warp >> 2) + 1) * (HeadDim / 4); c += 16) {
                 uint32_t o[2][16];
                 ptx::tmem_load16(at_out + c, o[0]);
                 ptx::tmem_load16(at_out + HeadDim + c, o[1]);
@@ -644,7 +628,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     store_row16(args, static_cast<T *>(args.output) + at_row * args.output_stride + size_t(head) * HeadDim + c, v, scale);
                 }
             }
-            if (live && !team) {
+            if (live && warp < 4) {
                 if (kept) kept[HeadDim] = highest, kept[HeadDim + 1] = l;
                 if (!args.table) {
                 } else if (!part.split) args.table[index] = make_int4(0, 0, 0, 0);
