@@ -131,6 +131,7 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     args.queries = p.queries.data, args.output = p.output.data;
     args.query_stride = p.queries.ld(), args.output_stride = p.output.ld();
     args.rows = rows, args.heads = heads, args.kv_heads = p.cache.kv_heads, args.group = heads / p.cache.kv_heads;
+    args.group_inverse = 1.f / float(args.group);
     args.aligned = aligned16(p.queries) && aligned16(p.output);
     args.sectors = args.aligned && reinterpret_cast<uintptr_t>(p.output.data) % 32 == 0 && p.output.ld() % 16 == 0;
     args.pages = p.pages, args.lengths = p.lengths, args.query_offsets = p.query_offsets;

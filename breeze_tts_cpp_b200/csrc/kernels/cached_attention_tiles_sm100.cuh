@@ -312,16 +312,17 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             for (int i = max(0, first_tile - 2); i < first_tile; ++i)
                 if (!wait(scored[0][i & 1], i >> 1) || !wait(scored[1][i & 1], i >> 1)) return false;
             constexpr int kChunks = HeadDim / 8, kTurns = kRows * kChunks / (32 * kConverters); // kChunks: threads to a row
-            const int flat = part.query_tile * kRows, chunk = thread % kChunks;
+            const int flat = part.query_tile * kRows, chunk = thread % kChunks, whole = flat / args.group, over = flat - whole * args.group;
             const auto place = [&](int i) { // where this thread's piece of turn i goes; rows of a turn are a multiple of eight apart
                 return base + uint32_t(chunk >> 3) * (kRows * 128) + panel_at(thread / kChunks, chunk & 7) + uint32_t(i) * (32 * kConverters / kChunks * 128);
             };
             static_assert(32 * kConverters / kChunks % 8 == 0);
 #pragma unroll 1
             for (int i = 0; i < kTurns; ++i) { // all rows in flight at once, as they are
-                const int row = thread / kChunks + 32 * kConverters / kChunks * i, token = (flat + row) / args.group;
-                const T *at = static_cast<const T *>(args.queries) + size_t(part.s.row + token) * args.query_stride +
-                              (part.head * args.group + flat + row - token * args.group) * HeadDim + 8 * chunk;
+                const int row = thread / kChunks + 32 * kConverters / kChunks * i;
+                const int tokens = int((float(over + row) + .5f) * args.group_inverse); // exact: the half is far more than the product is off by
+                const T *at = static_cast<const T *>(args.queries) + size_t(part.s.row + whole + tokens) * args.query_stride +
+                              (part.head * args.group + over + row - tokens * args.group) * HeadDim + 8 * chunk;
                 if (row >= part.columns) {
                     st_shared16(place(i), 0, 0, 0, 0);
                 } else if (args.aligned) {
@@ -333,6 +334,53 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     st_shared16(place(i), v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
                 }
             }
+            auto convert_keys = [&](int i) {
+                const int buffer = i & 1, before = (i >> 1) - 1;
+                if (!wait(raw_full[slot], use) || (before >= 0 && (!wait(scored[0][buffer], before) || !wait(scored[1][buffer], before)))) return false;
+                {
+                    const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::keys + buffer * Shape::operand;
+                    constexpr int kPieces = HeadDim / 16, kTurns = kTileKeys * kPieces / (32 * kConverters); // kPieces: lanes to a key row
+                    uint32_t w[kTurns][4];
+#pragma unroll
+                    for (int u = 0; u < kTurns; ++u) // row HeadDim bytes long, so thread t's pieces lie 16 t bytes in and one turn apart
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3])
+                                     : "r"(from + 16 * (thread + 32 * kConverters * u)));
+                    const int c = thread % kPieces, row = thread / kPieces;
+                    // The second panel's lanes store their chunks in the other order: eight lanes then meet eight banks. Rows of a turn are a
+                    // multiple of eight apart, so the swizzle is the same in all of them.
+                    static_assert(32 * kConverters / kPieces % 8 == 0);
+                    const int odd = (c >> 2) & 1;
+                    const uint32_t panel = to + uint32_t(c >> 2) * (kTileKeys * 128), near = panel + panel_at(row, 2 * (c & 3) + odd),
+                                   far = panel + panel_at(row, 2 * (c & 3) + 1 - odd);
+#pragma unroll
+                    for (int u = 0; u < kTurns; ++u) {
+                        uint32_t h[8];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) widen_key<F>(odd ? w[u][e ^ 2] : w[u][e], h[2 * e], h[2 * e + 1]);
+                        constexpr uint32_t kApart = 32 * kConverters / kPieces * 128;
+                        st_shared16(near + u * kApart, h[0], h[1], h[2], h[3]);
+                        st_shared16(far + u * kApart, h[4], h[5], h[6], h[7]);
+                    }
+                }
+                ptx::fence_proxy_async_smem();
+                arrive(keys_ready[buffer]);
+                return true;
+            };
+            auto note_scales = [&](int i, float score_scale) { // of the keys that were converted last, and of their values
+                if (thread < kTileKeys) {
+                    const float *scales = reinterpret_cast<const float *>(base_bytes + Shape::ring + slot * Shape::raw + kTileKeys * HeadDim);
+                    const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
+                    table_key[i & 3][thread] = key_scale * score_scale;
+                    table_value[i & 3][thread] = value_scale;
+                    table_shift[i & 3][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
+                    arrive(tables_ready[i & 3]);
+                }
+                arrive(raw_free[slot]);
+                next_slot();
+            };
+            // The first tile's keys while the queries are on their way.
+            if (!convert_keys(first_tile)) return false;
             ptx::copy_async_wait_all();
             float scale_up = 1.f;
             if constexpr (std::is_same<T, __nv_bfloat16>::value) {
@@ -372,50 +420,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             if (thread == 0) largest[~part.ordinal & 1] = 0; // everyone has read the part before's
 
             const float score_scale = args.score_scale * scale_up;
-            auto convert_keys = [&](int i) {
-                const int buffer = i & 1, before = (i >> 1) - 1;
-                if (!wait(raw_full[slot], use) || (before >= 0 && (!wait(scored[0][buffer], before) || !wait(scored[1][buffer], before)))) return false;
-                {
-                    const uint32_t from = base + Shape::ring + slot * Shape::raw, to = base + Shape::keys + buffer * Shape::operand;
-                    constexpr int kPieces = HeadDim / 16, kTurns = kTileKeys * kPieces / (32 * kConverters); // kPieces: lanes to a key row
-                    uint32_t w[kTurns][4];
-#pragma unroll
-                    for (int u = 0; u < kTurns; ++u) // row HeadDim bytes long, so thread t's pieces lie 16 t bytes in and one turn apart
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3])
-                                     : "r"(from + 16 * (thread + 32 * kConverters * u)));
-                    // The tile's scales, ahead of its values: the softmax of its first half needs no more than them and the scores.
-                    if (thread < kTileKeys) {
-                        const float *scales = reinterpret_cast<const float *>(base_bytes + Shape::ring + slot * Shape::raw + kTileKeys * HeadDim);
-                        const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
-                        table_key[i & 3][thread] = key_scale * score_scale;
-                        table_value[i & 3][thread] = value_scale;
-                        table_shift[i & 3][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
-                        arrive(tables_ready[i & 3]);
-                    }
-                    arrive(raw_free[slot]);
-                    const int c = thread % kPieces, row = thread / kPieces;
-                    // The second panel's lanes store their chunks in the other order: eight lanes then meet eight banks. Rows of a turn are a
-                    // multiple of eight apart, so the swizzle is the same in all of them.
-                    static_assert(32 * kConverters / kPieces % 8 == 0);
-                    const int odd = (c >> 2) & 1;
-                    const uint32_t panel = to + uint32_t(c >> 2) * (kTileKeys * 128), near = panel + panel_at(row, 2 * (c & 3) + odd),
-                                   far = panel + panel_at(row, 2 * (c & 3) + 1 - odd);
-#pragma unroll
-                    for (int u = 0; u < kTurns; ++u) {
-                        uint32_t h[8];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) widen_key<F>(odd ? w[u][e ^ 2] : w[u][e], h[2 * e], h[2 * e + 1]);
-                        constexpr uint32_t kApart = 32 * kConverters / kPieces * 128;
-                        st_shared16(near + u * kApart, h[0], h[1], h[2], h[3]);
-                        st_shared16(far + u * kApart, h[4], h[5], h[6], h[7]);
-                    }
-                }
-                ptx::fence_proxy_async_smem();
-                arrive(keys_ready[buffer]);
-                next_slot();
-                return true;
-            };
+            note_scales(first_tile, score_scale);
             auto convert_values = [&](int i) {
                 const int buffer = i & 1, before = (i >> 1) - 1;
                 if (!wait(raw_full[slot], use) || (before >= 0 && (!wait(weighted[0][buffer], before) || !wait(weighted[1][buffer], before)))) return false;
@@ -454,9 +459,13 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 return true;
             };
             const int end = first_tile + part.high - part.low;
-            if (!convert_keys(first_tile)) return false;
-            for (; first_tile < end; ++first_tile)
-                if ((first_tile + 1 < end && !convert_keys(first_tile + 1)) || !convert_values(first_tile)) return false;
+            for (; first_tile < end; ++first_tile) {
+                if (first_tile + 1 < end) {
+                    if (!convert_keys(first_tile + 1)) return false;
+                    note_scales(first_tile + 1, score_scale);
+                }
+                if (!convert_values(first_tile)) return false;
+            }
             return true;
         });
     } else if (warp < kSoftmaxWarps) { // --------------------------------------------------------- softmax
@@ -591,6 +600,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 ptx::tcgen05_fence_before();
                 arrive(softmaxed[team][buffer]);
             }
+            const int head = part.head * args.group + flat - flat / args.group * args.group;
+            const size_t at_row = size_t(part.s.row) + flat / args.group, index = at_row * args.heads + head;
+            float *kept = part.split      ? args.partials + (size_t(blockIdx.x * 2 + part.slot) * args.part_columns + row) * (HeadDim + kPartialExtra)
+                          : args.complete ? args.complete + index * (HeadDim + kPartialExtra)
+                                          : nullptr;
             if (!wait(weighted[team][(end - 1) & 1], (end - 1) >> 1)) return false;
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
@@ -605,11 +619,6 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             const float2 mine[2] = {stats[0][row], stats[1][row]};
             const float highest = fmaxf(mine[0].x, mine[1].x), reference = highest == -INFINITY ? 0.f : highest;
             const float factor[2] = {exp2_approx(mine[0].x - reference), exp2_approx(mine[1].x - reference)}, l = factor[0] * mine[0].y + factor[1] * mine[1].y;
-            const int head = part.head * args.group + flat % args.group;
-            const size_t at_row = size_t(part.s.row) + flat / args.group, index = at_row * args.heads + head;
-            float *kept = part.split      ? args.partials + (size_t(blockIdx.x * 2 + part.slot) * args.part_columns + row) * (HeadDim + kPartialExtra)
-                          : args.complete ? args.complete + index * (HeadDim + kPartialExtra)
-                                          : nullptr;
             const float scale = l == 0.f ? 0.f : args.output_scale / l;
 #pragma unroll 1
             for (int c = (warp >> 2) * (HeadDim / 4); c < ((warp >> 2) + 1) * (HeadDim / 4); c += 16) {

@@ -34,6 +34,7 @@ struct AttentionArgs {
     bool prefix;
     const void *cached_keys, *cached_values;
     const float *key_scales, *value_scales;
+    float group_inverse;
     float score_scale; // softmax scale, log2 e and the key format's factor
     float output_scale;
     int stages, merge_columns, merge_buffers;
