@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         const uint32_t box_bytes = uint32_t(box) * 2 * HeadDim;
         bool open = true;
         if (leads && !lane) note_closed(args, nullptr, kColumns);
-        const int parts = walk_share<kColumns>(args, kFewSegmentUnits, start, [&](const SegmentPart &part) {
+        const int parts = walk_share<kColumns>(args, start, [&](const SegmentPart &part) {
             const SequenceShape &s = part.s;
             const int low = part.low, high = part.high, head = part.head, columns = part.columns;
             if (leads && !lane && part.first_cta >= 0) note_closed(args, &part, kColumns);

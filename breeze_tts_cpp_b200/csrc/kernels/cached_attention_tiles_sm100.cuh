@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
         bool open = true;
         SegmentPart nothing{};
         if (!lane) note_closed(args, nullptr, kRows);
-        nothing.ordinal = walk_share<kRows>(args, kManySegmentUnits, start, [&](const SegmentPart &part) {
+        nothing.ordinal = walk_share<kRows>(args, start, [&](const SegmentPart &part) {
             if (!publish(part)) return open = false;
             if (!lane && part.first_cta >= 0) note_closed(args, &part, kRows);
             const int *pages = args.pages + size_t(part.sequence) * args.page_stride;
