@@ -663,7 +663,8 @@ template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThread
     int4 where, whose;
     asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(where.x), "=r"(where.y), "=r"(where.z), "=r"(where.w) : "l"(entry) : "memory");
     asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(whose.x), "=r"(whose.y), "=r"(whose.z), "=r"(whose.w) : "l"(entry + 4) : "memory");
-    if (!where.y) return;
+    // Offsets that fall can make the counts run over: what is read stays inside the workspace.
+    if (where.y <= 0 || where.x < 0 || where.y > s.ctas - where.x) return;
     for (int column = int(blockIdx.y) * (kCombineThreads / 32) + int(threadIdx.x >> 5); column < whose.z; column += int(gridDim.y) * (kCombineThreads / 32)) {
         RowSum<HeadDim> sum;
         sum.add(where.y, [&](int part) {

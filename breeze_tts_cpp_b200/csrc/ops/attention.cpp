@@ -9,9 +9,12 @@
 namespace tts::ops {
 namespace {
 [[noreturn]] void refuse(const char *what) { throw std::invalid_argument(what); }
-bool dense16(const TensorView &v) { return v.data && (v.type == Type::F16 || v.type == Type::BF16); }
+bool aligned(const void *p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+bool dense16(const TensorView &v) { return v.data && (v.type == Type::F16 || v.type == Type::BF16) && aligned(v.data, 2); }
+// Positions are ints, and so is the end of the tile of 128 keys that the last one lies in.
+bool too_long(int page_columns, int page_size) { return size_t(page_columns) * page_size > size_t(std::numeric_limits<int>::max()) - 127; }
 void check_index(const TensorView &v, size_t count, const char *what) {
-    if (!v.data || v.type != Type::I32 || v.rows != 1 || size_t(v.cols) != count || reinterpret_cast<uintptr_t>(v.data) % 4) refuse(what);
+    if (!v.data || v.type != Type::I32 || v.rows != 1 || size_t(v.cols) != count || !aligned(v.data, 4)) refuse(what);
 }
 // Column slices of one buffer (a packed QKV row) interleave: their spans overlap, their elements need not.
 bool collide(const TensorView &a, const TensorView &b) {
@@ -25,7 +28,7 @@ bool same_rows(const TensorView &a, const TensorView &b) {
     return a.data == b.data && a.rows == b.rows && a.cols == b.cols && (a.rows <= 1 || a.ld() == b.ld());
 }
 void check_plan(const RotaryView &plan, int head_dim, int device) {
-    if (!plan.turns || plan.device != device) refuse("rotary plan is missing or on another device");
+    if (!plan.turns || !aligned(plan.turns, 8) || plan.device != device) refuse("rotary plan is missing, misaligned or on another device");
     if (plan.dims < 16 || plan.dims > head_dim || plan.dims % 16) refuse("rotary columns must be a multiple of 16 within the head");
     if (!std::isfinite(plan.scale)) refuse("rotary scale is not finite");
 }
@@ -100,7 +103,7 @@ void validate_cache_write(const CacheView &cache, TensorView keys, TensorView va
         refuse("positions without a rotary plan");
     }
     for (const TensorView *norm : {&query_norm, &key_norm})
-        if (norm->data && (norm->type != keys.type || norm->numel() != size_t(cache.head_dim) || norm->rows != 1)) refuse("head norm weight shape/type mismatch");
+        if (norm->data && (norm->type != keys.type || norm->numel() != size_t(cache.head_dim) || norm->rows != 1 || !aligned(norm->data, 2))) refuse("head norm weight shape/type mismatch");
     if ((query_norm.data || key_norm.data) && !(epsilon >= 0.f && std::isfinite(epsilon))) refuse("invalid norm epsilon");
     if (queries.data || query_output.data) {
         if (!dense16(queries) || !dense16(query_output) || queries.type != keys.type || query_output.type != keys.type ||
@@ -156,8 +159,8 @@ void validate_cached_attention(const CacheView &cache, const Attention &a) {
     const int heads = a.queries.cols / cache.head_dim;
     if (!heads || a.queries.cols % cache.head_dim || heads % cache.kv_heads) refuse("query heads must be a multiple of the cache's heads");
     if (size_t(a.queries.rows) * heads > size_t(std::numeric_limits<int>::max())) refuse("too many query rows");
-    if (!a.pages.data || a.pages.type != Type::I32 || a.pages.rows < 1 || a.pages.cols < 1 ||
-        size_t(a.pages.cols) * cache.page_size > size_t(std::numeric_limits<int>::max()))
+    if (!a.pages.data || a.pages.type != Type::I32 || a.pages.rows < 1 || a.pages.cols < 1 || !aligned(a.pages.data, 4) ||
+        too_long(a.pages.cols, cache.page_size))
         refuse("attention pages must be int32 [sequences, pages]");
     check_index(a.lengths, size_t(a.pages.rows), "attention lengths must be int32, one per sequence");
     if (a.query_offsets.data) check_index(a.query_offsets, size_t(a.pages.rows) + 1, "query offsets must be int32, one more than sequences");
@@ -165,14 +168,14 @@ void validate_cached_attention(const CacheView &cache, const Attention &a) {
     if (!a.prefix_pages.data != !a.prefix_length.data) refuse("a prefix needs its pages and its length");
     if (a.prefix_pages.data) {
         check_index(a.prefix_pages, size_t(a.prefix_pages.cols), "prefix pages must be int32 [1, pages]");
-        if (a.prefix_pages.cols < 1 || size_t(a.prefix_pages.cols) * cache.page_size > size_t(std::numeric_limits<int>::max()))
+        if (a.prefix_pages.cols < 1 || too_long(a.prefix_pages.cols, cache.page_size))
             refuse("prefix pages must be int32 [1, pages]");
         check_index(a.prefix_length, 1, "the prefix length is one int32");
     }
     // The device counts tiles of 128 keys, per sequence, cached head and tile of at least eight query rows, in 32 bits.
     const int64_t group = heads / cache.kv_heads, segments = (int64_t(a.queries.rows) * group / 8 + a.pages.rows) * cache.kv_heads;
     const int64_t longest = (int64_t(std::max(a.pages.cols, a.prefix_pages.cols)) * cache.page_size + 127) / 128;
-    if (segments * longest > int64_t(1) << 27) refuse("too many query rows for tables of this size");
+    if (double(segments) * double(longest) > double(1 << 27)) refuse("too many query rows for tables of this size");
     if (!std::isfinite(a.scale)) refuse("attention scale is not finite");
     if (cache.overlaps(a.output)) refuse("attention output overlaps the cache");
     for (const TensorView &v : {a.queries, a.pages, a.lengths, a.query_offsets, a.prefix_pages, a.prefix_length})
@@ -186,6 +189,7 @@ void cached_attention(const CacheView &cache, const Attention &a) {
     const size_t needed = cached_attention_workspace(a.queries.rows, a.pages.rows, heads, cache.kv_heads, cache.head_dim, prefix, gpu.multiprocessors);
     if (!gpu.gemm_workspace.data() || gpu.gemm_workspace.size() < needed)
         throw std::invalid_argument("attention needs a context workspace of " + std::to_string(needed) + " bytes");
+    if (!aligned(gpu.gemm_workspace.data(), 32)) throw std::invalid_argument("attention needs a context workspace on a 32-byte boundary");
     AttentionProblem p;
     p.queries = a.queries, p.output = a.output, p.cache = cache;
     p.pages = a.pages.ptr<int>(), p.sequences = a.pages.rows, p.page_columns = a.pages.cols, p.page_stride = a.pages.ld();

@@ -138,6 +138,27 @@ def test_attention_refusals():
     assert "too many query rows" in attention(cache(at=1 << 36), **large)
 
 
+def test_addresses_that_no_element_has():
+    """Elements lie on multiples of their size; a vector load or store would fault elsewhere."""
+    assert "shape/type" in write(k=tensor(1, 3, 128)) and "shape/type" in write(q=tensor(20001, 3, 256), q_out=tensor(30000, 3, 256))
+    assert "norm weight" in write(k_norm=tensor(401, 1, 64)) and "slots" in write(slots=tensor(8194, 1, 3, I32))
+    assert "misaligned" in write(rotary=RotaryPlan(MEMORY + (1 << 29) + 4, 64, 0, 1.0, 0), positions=tensor(9000, 1, 3, I32))
+    assert "shape/type" in attention(queries=tensor(1, 3, 256)) and "shape/type" in attention(output=tensor((1 << 20) + 1, 3, 256))
+    assert "pages" in attention(pages=tensor((1 << 21) + 2, 3, 5, I32)) and "lengths" in attention(lengths=tensor((1 << 22) + 1, 1, 3, I32))
+
+
+def test_tables_whose_last_tile_ends_past_an_int():
+    """Positions are counted to the end of a tile of 128 keys in 32 bits."""
+    one = dict(queries=tensor(0, 1, 128), output=tensor(1 << 20, 1, 128), lengths=tensor(1 << 22, 1, 1, I32))
+    small = cache(kv_heads=1, at=1 << 36)
+    most = (2**31 - 128) // 16
+    assert attention(small, pages=tensor(1 << 30, 1, most, I32), **one) == ""
+    assert "attention pages" in attention(small, pages=tensor(1 << 30, 1, most + 1, I32), **one)
+    prefix = dict(pages=tensor(1 << 21, 1, 5, I32), prefix_length=tensor(1 << 24, 1, 1, I32))
+    assert attention(small, prefix_pages=tensor(1 << 30, 1, most, I32), **prefix, **one) == ""
+    assert "prefix pages" in attention(small, prefix_pages=tensor(1 << 30, 1, most + 1, I32), **prefix, **one)
+
+
 def test_null_structs_are_errors():
     assert "null cache" in refused("b200q_cache_read", None, tensor(0, 1, 3, I32), tensor(0, 3, 128), NONE)
     assert "null attention" in refused("b200q_cached_attention", cache(), None)
