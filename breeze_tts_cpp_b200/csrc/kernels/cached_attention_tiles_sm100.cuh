@@ -103,10 +103,12 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     // free); softmaxed: P is ready; weighted: O has it (of both: the values' buffer is free). keys/values: operands are ready. tables_ready
     // has a use for every fourth tile: its tables are not written again before the teams are done with them.
     __shared__ uint64_t raw_full[kSlots], raw_free[kSlots], keys_ready[2], values_ready[2], scored[2][2], softmaxed[2][2], weighted[2][2], tables_ready[4];
-    __shared__ uint64_t queries_ready, largest_known, meet, outputs_free, drained[2]; // once per segment part, the last once
+    __shared__ uint64_t queries_ready, meet, outputs_free, drained[2]; // once per segment part, the last once
     __shared__ __align__(16) float table_key[4][kTileKeys], table_shift[4][kTileKeys], table_value[4][kTileKeys]; // of tile i: i % 4
     __shared__ float2 stats[2][kRows];
-    __shared__ unsigned largest[2]; // of a part's queries, by the part's parity
+    // What a BF16 row's scores are multiplied by, by the part's ordinal: three parts on, the softmax warps have begun the first one's tiles.
+    __shared__ float row_scale[4][kRows];
+    constexpr bool kScaledRows = std::is_same<T, __nv_bfloat16>::value;
     __shared__ Work sums[kManyWarps];
     __shared__ Start found;
     __shared__ SegmentPart parts[kPartsAhead];
@@ -131,13 +133,11 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 ptx::mbar_init(ptx::smem_u32(&weighted[t][h]), 1);
             }
             ptx::mbar_init(ptx::smem_u32(&drained[t]), 1);
-            ptx::mbar_init(ptx::smem_u32(&tables_ready[2 * t]), kTileKeys / 32);
-            ptx::mbar_init(ptx::smem_u32(&tables_ready[2 * t + 1]), kTileKeys / 32);
-            largest[t] = 0;
+            ptx::mbar_init(ptx::smem_u32(&tables_ready[2 * t]), kConverters);
+            ptx::mbar_init(ptx::smem_u32(&tables_ready[2 * t + 1]), kConverters);
         }
         ptx::mbar_init(ptx::smem_u32(&queries_ready), kConverters);
         ptx::mbar_init(ptx::smem_u32(&outputs_free), kSoftmaxWarps);
-        ptx::mbar_init(ptx::smem_u32(&largest_known), kConverters);
         ptx::mbar_init(ptx::smem_u32(&meet), kSoftmaxWarps);
         for (int p = 0; p < kPartsAhead; ++p) {
             ptx::mbar_init(ptx::smem_u32(&part_full[p]), 1);
@@ -307,8 +307,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             if (++slot == kSlots) slot = 0, ++use;
         };
         for_parts([&](const SegmentPart &part) {
-            // Queries, once the products of the part before have read theirs. Rows past the segment are zero. BF16 rows are divided by the power of
-            // two of their largest element of all, which brings them into fp16's range; what that costs the small ones is small next to the others.
+            // Queries, once the products of the part before have read theirs. Rows past the segment are zero. A BF16 row is divided by the power of two
+            // of its largest element, which brings it into fp16's range whatever the rows beside it hold.
             for (int i = max(0, first_tile - 2); i < first_tile; ++i)
                 if (!wait(scored[0][i & 1], i >> 1) || !wait(scored[1][i & 1], i >> 1)) return false;
             constexpr int kChunks = HeadDim / 8, kTurns = kRows * kChunks / (32 * kConverters); // kChunks: threads to a row
@@ -367,46 +367,34 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 arrive(keys_ready[buffer]);
                 return true;
             };
-            auto note_scales = [&](int i, float score_scale) { // of the keys that were converted last, and of their values
+            auto note_scales = [&](int i) { // of the keys that were converted last, and of their values
                 if (thread < kTileKeys) {
                     const float *scales = reinterpret_cast<const float *>(base_bytes + Shape::ring + slot * Shape::raw + kTileKeys * HeadDim);
                     const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
-                    table_key[i & 3][thread] = key_scale * score_scale;
+                    table_key[i & 3][thread] = key_scale * args.score_scale;
                     table_value[i & 3][thread] = value_scale;
                     table_shift[i & 3][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
-                    arrive(tables_ready[i & 3]);
                 }
+                arrive(tables_ready[i & 3]);
                 arrive(raw_free[slot]);
                 next_slot();
             };
             // The first tile's keys while the queries are on their way.
             if (!convert_keys(first_tile)) return false;
             ptx::copy_async_wait_all();
-            float scale_up = 1.f;
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                auto load = [&](int i, uint32_t(&w)[4]) {
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place(i)) : "memory");
-                };
-                unsigned most = 0;
+            if constexpr (kScaledRows) {
 #pragma unroll 4
-                for (int i = 0; i < kTurns; ++i) {
+                for (int i = 0; i < kTurns; ++i) { // kChunks lanes hold a row
                     uint32_t w[4];
-                    load(i, w);
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(place(i)) : "memory");
+                    unsigned most = 0;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) most = max(most, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
-                }
-                most = __reduce_max_sync(0xffffffffu, most);
-                if (!lane) atomicMax(&largest[part.ordinal & 1], most);
-                arrive(largest_known);
-                if (!wait(largest_known, part.ordinal)) return false;
-                most = *const_cast<volatile unsigned *>(&largest[part.ordinal & 1]);
-                const int exponent = most && most < 0x7f800000u ? max(int(most >> 23), 1) - 127 : 0;
-                const float down = __int_as_float(exponent < 127 ? (127 - exponent) << 23 : 0x00400000); // 2^-exponent
-                scale_up = __int_as_float(exponent > -127 ? (127 + exponent) << 23 : 0x00400000);
-#pragma unroll 4
-                for (int i = 0; i < kTurns; ++i) {
-                    uint32_t w[4];
-                    load(i, w);
+#pragma unroll
+                    for (int d = 1; d < kChunks; d <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+                    const int exponent = most && most < 0x7f800000u ? max(int(most >> 23), 1) - 127 : 0;
+                    const float down = __int_as_float(exponent < 127 ? (127 - exponent) << 23 : 0x00400000); // 2^-exponent
+                    if (!chunk) row_scale[part.ordinal & 3][thread / kChunks + 32 * kConverters / kChunks * i] = __int_as_float(exponent > -127 ? (127 + exponent) << 23 : 0x00400000);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const __half2 v = __floats2half2_rn(__uint_as_float(w[e] << 16) * down, __uint_as_float(w[e] & 0xffff0000u) * down);
@@ -417,10 +405,8 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             }
             ptx::fence_proxy_async_smem();
             arrive(queries_ready);
-            if (thread == 0) largest[~part.ordinal & 1] = 0; // everyone has read the part before's
 
-            const float score_scale = args.score_scale * scale_up;
-            note_scales(first_tile, score_scale);
+            note_scales(first_tile);
             auto convert_values = [&](int i) {
                 const int buffer = i & 1, before = (i >> 1) - 1;
                 if (!wait(raw_full[slot], use) || (before >= 0 && (!wait(weighted[0][buffer], before) || !wait(weighted[1][buffer], before)))) return false;
@@ -462,7 +448,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             for (; first_tile < end; ++first_tile) {
                 if (first_tile + 1 < end) {
                     if (!convert_keys(first_tile + 1)) return false;
-                    note_scales(first_tile + 1, score_scale);
+                    note_scales(first_tile + 1);
                 }
                 if (!convert_values(first_tile)) return false;
             }
@@ -481,6 +467,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
             const bool live = row < part.columns;
             int limit[2], least = INT_MAX; // the last position that a row sees
             float most[2], sum[2];
+            uint64_t up[2] = {};
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int its_row = first_row + 8 * r, token = (part.query_tile * kRows + its_row) / args.group;
@@ -500,6 +487,10 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 if (!wait(scored[team][buffer], i >> 1) || !wait(tables_ready[i & 3], i >> 2)) return false;
                 ptx::tcgen05_fence_after();
                 // 32 columns at a time, the next ones on their way while these are worked on.
+                if (kScaledRows && i == first_tile) {
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) up[r] = ptx::pack2(row_scale[part.ordinal & 3][first_row + 8 * r], row_scale[part.ordinal & 3][first_row + 8 * r]);
+                }
                 float highest[2] = {-INFINITY, -INFINITY};
                 auto find_highest = [&](auto masked_tile) {
                     constexpr bool kMasked = decltype(masked_tile)::value;
@@ -516,7 +507,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 float x, y;
-                                ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, shift), x, y);
+                                ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), kScaledRows ? ptx::mul2(k, up[r]) : k, shift), x, y);
                                 if (kMasked && key + c + 8 * j > limit[r]) x = -INFINITY;
                                 if (kMasked && key + c + 8 * j + 1 > limit[r]) y = -INFINITY;
                                 highest[r] = fmaxf(highest[r], fmaxf(x, y));
@@ -574,7 +565,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 float x, y;
-                                ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), k, minus[r]), x, y);
+                                ptx::unpack2(ptx::fma2(pair(s[unit & 1][4 * j + 2 * r], s[unit & 1][4 * j + 2 * r + 1]), kScaledRows ? ptx::mul2(k, up[r]) : k, minus[r]), x, y);
                                 const bool hide_x = kMasked && key + c + 8 * j > limit[r], hide_y = kMasked && key + c + 8 * j + 1 > limit[r];
                                 const uint64_t both = ptx::pack2(exp2_approx(hide_x ? -INFINITY : x), exp2_approx(hide_y ? -INFINITY : y));
                                 total[r] = ptx::add2(total[r], both);

@@ -259,6 +259,20 @@ def test_many_rows_of_any_magnitude(ctx_factory, power):
     check(batch.run(ctx_factory("int8"), scale=scale), *batch.want(scale))
 
 
+def test_many_rows_beside_a_row_that_is_huge_or_infinite(ctx_factory):
+    """BF16 rows enter fp16 each by a power of two of its own: a row 2^28 above the others, or one with an infinity, costs those nothing. (Nothing is
+    asked of these rows: scores of 2^30 are known to within 2^6 in fp32, so exp of them to within a factor of 2^64.)"""
+    batch = many()
+    batch.q = batch.q.clone()
+    batch.q[5] = (batch.q[5].double() * 2.0**28).bfloat16()
+    batch.q[9, 3] = float("inf")
+    batch.q[81, 70] = float("-inf")
+    batch.q[90] = (batch.q[90].double() * 2.0**28).bfloat16()
+    got, (want, bound) = batch.run(ctx_factory("int8")), batch.want()
+    others = [r for r in range(110) if r not in (5, 9, 81, 90)]
+    check(got[others], want[others], bound[others])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_many_rows_strided(ctx_factory, dtype):
     batch = many(head_dim=64, dtype=DTYPES[dtype])
