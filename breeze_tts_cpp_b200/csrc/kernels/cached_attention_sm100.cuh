@@ -36,6 +36,9 @@ constexpr int kTeam = 4, kTeams = 2, kWorkers = kTeam * kTeams, kProducers = 2, 
 constexpr int kAttentionWarps = kWorkers + kProducers + kMergers, kAttentionThreads = 32 * kAttentionWarps; // three per scheduler: 168 registers a thread
 constexpr int kFewSegmentUnits = 6; // a segment's queries, flush and merge next to a tile's kTileUnits (64 sequences of up to 4096: 2 units 65.2 us, 4 60.9, 6 59.9)
 
+// log2 of the least value scale that the reference follows. Behind smaller ones, zero among them, p_j grows to 2^96, of which fp32 holds a sum of 2^23
+// (with many rows' slack); what their values add lies below 2^-96 of the format's range.
+constexpr float kLeastScale = -96.f;
 __device__ __forceinline__ float exp2_approx(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -468,7 +471,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
                 for (int n = 0; n < Tiles; ++n) mma_f16(scores[n][m], a[0], a[1], a[2], a[3], q[n][k][0], q[n][k][1]);
             }
 #pragma unroll
-            for (int r = 0; r < 2; ++r) shift[m][r] = fmaxf(log2_approx(fabsf(value_scale[m][r])), -126.f);
+            for (int r = 0; r < 2; ++r) shift[m][r] = fmaxf(log2_approx(fabsf(value_scale[m][r])), kLeastScale);
         }
         const int position = first_key + row + g;
         const bool masked = first_key + kTileKeys - 1 > least;

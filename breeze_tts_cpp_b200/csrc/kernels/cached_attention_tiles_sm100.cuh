@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                     const float key_scale = scales[thread], value_scale = scales[kTileKeys + thread];
                     table_key[i & 3][thread] = key_scale * args.score_scale;
                     table_value[i & 3][thread] = value_scale;
-                    table_shift[i & 3][thread] = fmaxf(log2_approx(fabsf(value_scale)), -126.f);
+                    table_shift[i & 3][thread] = fmaxf(log2_approx(fabsf(value_scale)), kLeastScale);
                 }
                 arrive(tables_ready[i & 3]);
                 arrive(raw_free[slot]);

@@ -301,6 +301,21 @@ def test_references_that_rise_late(ctx_factory):
         check(batch.run(ctx_factory("int8")), *batch.want())
 
 
+@pytest.mark.parametrize("prefix", [None, 900])
+@pytest.mark.parametrize("counts", [None, [40, 33, 1]])
+def test_values_whose_scale_is_zero(ctx_factory, counts, prefix):
+    """A cache filled by its owner may hold zero scales, runs of tiles of them: they weigh in the sum, wherever the shares end."""
+    batch = Batch(34, [1500, 900, 300], counts, heads=2, kv_heads=1, page=64, prefix=prefix)
+    for b, runs in ((0, [(0, 12)]), (1, [(0, 15)]), (2, [(1, 3)])):
+        for first, last in runs:
+            batch.cache.value_scales[batch.pages[b, first:last].clamp(max=batch.cache.value_scales.shape[0] - 1).long()] = 0.0
+    if prefix:
+        batch.cache.value_scales[batch.prefix_pages[3:9].long()] = 0.0
+    context = ops.Context("int8", workspace_bytes=64 << 20)
+    check(batch.run(context), *batch.want())
+    context.close()
+
+
 def test_strided_page_tables(ctx_factory):
     batch = Batch(32, [130, 31, 77, 0], None, page=32)
     wide = torch.full((4, 3 * batch.pages.shape[1] + 1), 7 * 10**5, dtype=torch.int32)
