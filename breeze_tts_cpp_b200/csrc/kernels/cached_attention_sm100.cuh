@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
     __shared__ Work sums[kAttentionWarps];
     __shared__ Start found;
     __shared__ int abort_flag;
-    __shared__ int merged; // parts that the mergers are done with, times kMergers
+    __shared__ int merged[kMergers]; // parts that each merger is done with, written by that one only
     const uint32_t ring = (ptx::smem_u32(raw_smem) + 1023u) & ~1023u;
     uint8_t *const ring_bytes = raw_smem + (ring - ptx::smem_u32(raw_smem));
     const int stages = args.stages, merge_floats = int(Shape::merge(args.merge_columns) / 4);
@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
             ptx::mbar_init(ptx::smem_u32(&empty[s]), kTeam);
         }
         for (int b = 0; b < kMergeBuffers; ++b) ptx::mbar_init(ptx::smem_u32(&merge_full[b]), kWorkers);
-        abort_flag = merged = 0;
+        abort_flag = 0;
+        for (int m = 0; m < kMergers; ++m) merged[m] = 0;
         ptx::fence_barrier_init();
         ptx::prefetch_tensormap(&key_map);
         ptx::prefetch_tensormap(&value_map);
@@ -155,10 +156,18 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         return false;
     };
 
+    // Until every merger is done with that many parts. A sum of theirs would not do: the one with less to do (with none at all, at one column of 128)
+    // runs ahead by as many parts as there are buffers, and would stand in for the other.
     auto wait_merged = [&](int parts) {
+        auto least = [&] {
+            int done = INT_MAX;
+#pragma unroll
+            for (int m = 0; m < kMergers; ++m) done = min(done, const_cast<volatile int *>(merged)[m]);
+            return done;
+        };
         bool reached = false;
         const long long start = clock64();
-        while (!(reached = *const_cast<volatile int *>(&merged) >= parts) && !*const_cast<volatile int *>(&abort_flag))
+        while (!(reached = least() >= parts) && !*const_cast<volatile int *>(&abort_flag))
             if (clock64() - start > ptx::kWaitLimitCycles) abort_flag = 1;
         reached = __all_sync(0xffffffffu, reached);
         __threadfence_block();
@@ -335,7 +344,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
             __syncwarp();
             if (!lane) {
                 __threadfence_block();
-                atomicAdd(&merged, 1);
+                const_cast<volatile int *>(merged)[warp - kMerger] = ordinal + 1;
             }
             if (flags & kNoteFinal) return;
         }
@@ -545,8 +554,8 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         if (flags & kNoteFlush) { // this warp's share of the segment's part; the mergers add the shares up
             const int ordinal = note.ordinal, buffer = ordinal % args.merge_buffers;
             const int columns = min(kColumns, note.count * args.group - note.flat);
-            // A count and not a barrier's phase: a group has no tile in some parts, and could be two phases off.
-            if (ordinal >= args.merge_buffers && !wait_merged(kMergers * (ordinal - args.merge_buffers + 1))) return;
+            // Counts and not a barrier's phase: a group has no tile in some parts, and could be two phases off.
+            if (ordinal >= args.merge_buffers && !wait_merged(ordinal - args.merge_buffers + 1)) return;
             const int share = (team - note.first_team + kTeams) % kTeams * kTeam + warp % kTeam;
             float *const shares = merge + buffer * merge_floats + share * args.merge_columns * Shape::row;
 #pragma unroll
