@@ -46,6 +46,7 @@ bool tensor_of(PyObject *object, b200q_tensor &out, int code = -1) {
     const size_t dims = sizes.size();
     if ((dims != 1 && dims != 2) || strides[dims - 1] != 1) return false;
     const int64_t rows = dims == 2 ? sizes[0] : 1, cols = sizes[dims - 1];
+    if (rows > 1 && strides[0] < cols) return false; // expanded rows: a stride of 0 says dense
     const int64_t stride = dims == 2 && rows > 1 && strides[0] != cols ? strides[0] : 0;
     if (code < 0) code = type_code(t.scalar_type());
     if (code < 0 || rows > INT32_MAX || cols > INT32_MAX || stride < 0 || stride > INT32_MAX) return false;

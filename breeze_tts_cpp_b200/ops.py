@@ -48,6 +48,8 @@ def _tensor(t: torch.Tensor | None, type_code: int | None = None) -> Tensor:
         t = t.unsqueeze(0)
     if t.dim() != 2 or t.stride(1) != 1:
         raise ValueError("operands must be 2-D with a dense inner axis")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:  # a stride of 0 would be taken for dense rows
+        raise ValueError("operands' rows must not overlap: expanded tensors have to be made contiguous")
     code = type_code if type_code is not None else _TORCH_TYPES[t.dtype]
     stride = t.stride(0) if t.shape[0] > 1 and t.stride(0) != t.shape[1] else 0
     return Tensor(t.data_ptr(), t.shape[0], t.shape[1], stride, code, t.device.index)
