@@ -52,6 +52,8 @@ def _tensor(t: torch.Tensor | None, type_code: int | None = None) -> Tensor:
         raise ValueError("operands' rows must not overlap: expanded tensors have to be made contiguous")
     code = type_code if type_code is not None else _TORCH_TYPES[t.dtype]
     stride = t.stride(0) if t.shape[0] > 1 and t.stride(0) != t.shape[1] else 0
+    if max(*t.shape, stride) > 2**31 - 1:  # ctypes would keep the low 32 bits
+        raise ValueError("operands have at most 2^31 - 1 rows and columns, and as many elements between two rows")
     return Tensor(t.data_ptr(), t.shape[0], t.shape[1], stride, code, t.device.index)
 
 

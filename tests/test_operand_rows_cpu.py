@@ -21,3 +21,11 @@ def test_windows_are_refused():
     with FakeTensorMode():
         with pytest.raises(ValueError, match="overlap"):
             ops._tensor(torch.empty(64, dtype=torch.int32, device="cuda").unfold(0, 16, 4))
+
+
+@pytest.mark.parametrize("shape,columns", [((2, 2**32 + 128), 128), ((3, 2**31), 16), ((2**32 + 3, 16), 16), ((1, 2**32 + 16), 2**32 + 16)])
+def test_sizes_past_32_bits_are_refused(shape, columns):
+    """Their low 32 bits may be sizes that the call takes."""
+    with FakeTensorMode():
+        with pytest.raises(ValueError, match="2\\^31"):
+            ops._tensor(torch.empty(shape, dtype=torch.bfloat16, device="cuda")[:, :columns])
