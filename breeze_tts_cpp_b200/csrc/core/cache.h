@@ -22,8 +22,11 @@ struct CacheView {
         if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
             throw std::invalid_argument("cache pages hold 16 to 1024 tokens, a power of two");
         if (pages < 1 || kv_heads < 1) throw std::invalid_argument("empty cache");
-        // Rows are a tensor map's coordinate, slots an int32 index.
-        if (rows() > size_t(std::numeric_limits<int>::max())) throw std::invalid_argument("cache has more than 2^31 - 1 rows");
+        // Rows are a tensor map's coordinate, slots an int32 index, and so are the columns of a 16-bit row of all heads. The product of all three
+        // sizes may pass 64 bits.
+        constexpr size_t most = size_t(std::numeric_limits<int>::max());
+        if (size_t(pages) * kv_heads > most / page_size) throw std::invalid_argument("cache has more than 2^31 - 1 rows");
+        if (size_t(kv_heads) > most / head_dim) throw std::invalid_argument("cache heads have more than 2^31 - 1 columns in all");
         const void *parts[] = {keys, values, key_scales, value_scales};
         const size_t sizes[] = {rows() * head_dim, rows() * head_dim, rows() * 4, rows() * 4};
         for (int i = 0; i < 4; ++i) {

@@ -1,0 +1,33 @@
+"""Cache operators at the far ends of their sizes, without a GPU: what passes 32 or 64 bits is refused."""
+import pytest
+
+from breeze_tts_cpp_b200._lib import I32, Cache, Tensor
+from tests.test_cache_cpu import MEMORY, NONE, refused, tensor
+
+
+def cache(pages, kv_heads, page=16, head_dim=64):
+    """Storage 2^44 bytes apart: no overlap, whatever the sizes."""
+    return Cache(*(MEMORY + (i << 44) for i in range(1, 5)), pages, kv_heads, page, head_dim, 4, 0)
+
+
+def empty(rows, cols=0):
+    return Tensor(MEMORY, rows, cols, 0, 0, 0)
+
+
+@pytest.mark.parametrize("pages,kv_heads,page", [
+    (1 << 27, 1 << 27, 1024), (1 << 30, 1 << 30, 16), (1 << 28, 1 << 30, 64), (2**31 - 1, 2**31 - 1, 1024), (1 << 28, 1, 16), (1, 1 << 28, 16)])
+def test_caches_with_too_many_rows(pages, kv_heads, page):
+    """The first three products are 2^64, of which 64 bits keep nothing."""
+    for name, arguments in (("b200q_cache_write", (empty(3), empty(3), tensor(8192, 1, 3, I32), NONE, None, NONE, NONE, NONE, NONE, 1e-6)),
+                            ("b200q_cache_read", (tensor(8192, 1, 3, I32), empty(3), NONE))):
+        assert "2^31 - 1 rows" in refused(name, cache(pages, kv_heads, page), *arguments)
+
+
+@pytest.mark.parametrize("kv_heads,head_dim", [(1 << 26, 64), (1 << 25, 64), (1 << 25, 128), ((1 << 26) + 1, 64), (1 << 24, 128)])
+def test_caches_with_too_many_columns(kv_heads, head_dim):
+    """Columns of all heads are counted in 32 bits: the first and third of these left 0 of them, and the fourth 64."""
+    width = kv_heads * head_dim % 2**32
+    width = width if width < 2**31 else 0
+    write = (empty(3, width), empty(3, width), tensor(8192, 1, 3, I32), NONE, None, NONE, NONE, NONE, NONE, 1e-6)
+    assert "2^31 - 1 columns" in refused("b200q_cache_write", cache(1, kv_heads, 16, head_dim), *write)
+    assert "2^31 - 1 columns" in refused("b200q_cache_read", cache(1, kv_heads, 16, head_dim), tensor(8192, 1, 3, I32), empty(3, width), NONE)
