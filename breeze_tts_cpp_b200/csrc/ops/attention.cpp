@@ -32,6 +32,9 @@ void check_plan(const RotaryView &plan, int head_dim, int device) {
     if (plan.dims < 16 || plan.dims > head_dim || plan.dims % 16) refuse("rotary columns must be a multiple of 16 within the head");
     if (!std::isfinite(plan.scale)) refuse("rotary scale is not finite");
 }
+TensorView turns_of(const RotaryView &plan) {
+    return plan.turns ? TensorView(const_cast<double *>(plan.turns), 1, plan.dims / 2, Type::F64, 0, plan.device) : TensorView();
+}
 void check_devices(int device, std::initializer_list<TensorView> operands) {
     for (const TensorView &v : operands)
         if (v.data && v.device != device) refuse("operands are on different devices");
@@ -82,6 +85,7 @@ void validate_rotary(TensorView input, TensorView positions, RotaryView plan, in
     check_plan(plan, head_dim, input.device);
     if (!same_rows(input, output) && collide(output, input)) refuse("rotary output overlaps its input");
     if (output.overlaps(positions)) refuse("rotary output overlaps its positions");
+    if (output.overlaps(turns_of(plan))) refuse("rotary output overlaps its plan");
 }
 void rotary(TensorView input, TensorView positions, RotaryView plan, int head_dim, TensorView output) {
     validate_rotary(input, positions, plan, head_dim, output);
@@ -105,18 +109,19 @@ void validate_cache_write(const CacheView &cache, TensorView keys, TensorView va
     for (const TensorView *norm : {&query_norm, &key_norm})
         if (norm->data && (norm->type != keys.type || norm->numel() != size_t(cache.head_dim) || norm->rows != 1 || !aligned(norm->data, 2))) refuse("head norm weight shape/type mismatch");
     if ((query_norm.data || key_norm.data) && !(epsilon >= 0.f && std::isfinite(epsilon))) refuse("invalid norm epsilon");
+    const TensorView turns = turns_of(plan);
     if (queries.data || query_output.data) {
         if (!dense16(queries) || !dense16(query_output) || queries.type != keys.type || query_output.type != keys.type ||
             queries.rows != keys.rows || query_output.rows != keys.rows || queries.cols != query_output.cols || !queries.cols ||
             queries.cols % cache.head_dim)
             refuse("query input/output shape/type mismatch");
         if (!same_rows(queries, query_output) && collide(query_output, queries)) refuse("query output overlaps its input");
-        for (const TensorView &source : {keys, values, slots, positions, query_norm, key_norm})
+        for (const TensorView &source : {keys, values, slots, positions, turns, query_norm, key_norm})
             if (collide(query_output, source)) refuse("query output overlaps another operand");
     } else if (query_norm.data) {
         refuse("a query norm without queries");
     }
-    for (const TensorView &v : {keys, values, slots, positions, queries, query_output, query_norm, key_norm})
+    for (const TensorView &v : {keys, values, slots, positions, turns, queries, query_output, query_norm, key_norm})
         if (cache.overlaps(v)) refuse("an operand overlaps the cache");
 }
 void cache_write(const CacheView &cache, TensorView keys, TensorView values, TensorView slots, TensorView positions, RotaryView plan,

@@ -1,4 +1,4 @@
-"""Cache operators at the far ends of their sizes, without a GPU: what passes 32 or 64 bits is refused."""
+"""What the cache operators refuse, beyond test_cache_cpu.py, without a GPU: sizes past 32 or 64 bits, outputs over the rotary plan."""
 import pytest
 
 from breeze_tts_cpp_b200._lib import I32, Cache, Tensor
@@ -31,3 +31,16 @@ def test_caches_with_too_many_columns(kv_heads, head_dim):
     write = (empty(3, width), empty(3, width), tensor(8192, 1, 3, I32), NONE, None, NONE, NONE, NONE, NONE, 1e-6)
     assert "2^31 - 1 columns" in refused("b200q_cache_write", cache(1, kv_heads, 16, head_dim), *write)
     assert "2^31 - 1 columns" in refused("b200q_cache_read", cache(1, kv_heads, 16, head_dim), tensor(8192, 1, 3, I32), empty(3, width), NONE)
+
+
+def test_outputs_over_the_plan_are_refused():
+    """Rows that are written while others still take their angles from there."""
+    from tests.test_cache_cpu import cache as small, plan, write
+    rotary, positions, at = plan(), tensor(9000, 1, 3, I32), 1 << 29
+    x, out = tensor(0, 3, 128), tensor(at - 512, 3, 128)  # rows of 256 bytes: the third begins at the plan
+    assert "overlaps its plan" in refused("b200q_rotary", x, positions, rotary, 64, out)
+    assert "overlaps its plan" in refused("b200q_rotary", x, positions, rotary, 64, tensor(at + 254, 3, 128))
+    assert refused("b200q_rotary", x, positions, rotary, 64, tensor(at + 256, 3, 128)) == ""  # 32 pairs of 8 bytes end there
+    assert refused("b200q_rotary", x, positions, rotary, 64, tensor(at - 768, 3, 128)) == ""
+    assert "overlaps another operand" in write(rotary=rotary, positions=positions, q=tensor(20000, 3, 128), q_out=out)
+    assert "overlaps the cache" in write(small(at=at - 4096), rotary=rotary, positions=positions)
