@@ -5,6 +5,8 @@
 #include <cuda_runtime_api.h>
 
 namespace tts {
+// Query heads that share a cached one, at most: a query row's token is found by an fp32 product, which from 2^23 of them on may be one off.
+constexpr int kMostGroup = 1 << 20;
 struct AttentionProblem {
     TensorView queries, output; // [rows, heads * head_dim]
     CacheView cache;

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
 #pragma unroll 1
             for (int i = 0; i < kTurns; ++i) { // all rows in flight at once, as they are
                 const int row = thread / kChunks + 32 * kConverters / kChunks * i;
-                const int tokens = int((float(over + row) + .5f) * args.group_inverse); // exact: the half is far more than the product is off by
+                const int tokens = int((float(over + row) + .5f) * args.group_inverse); // exact up to kMostGroup: the half is far more than the product is off by
                 const T *at = static_cast<const T *>(args.queries) + size_t(part.s.row + whole + tokens) * args.query_stride +
                               (part.head * args.group + over + row - tokens * args.group) * HeadDim + 8 * chunk;
                 if (row >= part.columns) {

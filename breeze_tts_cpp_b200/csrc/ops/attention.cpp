@@ -163,6 +163,7 @@ void validate_cached_attention(const CacheView &cache, const Attention &a) {
         refuse("attention queries/output shape/type mismatch");
     const int heads = a.queries.cols / cache.head_dim;
     if (!heads || a.queries.cols % cache.head_dim || heads % cache.kv_heads) refuse("query heads must be a multiple of the cache's heads");
+    if (heads / cache.kv_heads > kMostGroup) refuse("more than 2^20 query heads to a cached one");
     if (size_t(a.queries.rows) * heads > size_t(std::numeric_limits<int>::max())) refuse("too many query rows");
     if (!a.pages.data || a.pages.type != Type::I32 || a.pages.rows < 1 || a.pages.cols < 1 || !aligned(a.pages.data, 4) ||
         too_long(a.pages.cols, cache.page_size))

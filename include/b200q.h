@@ -215,8 +215,8 @@ int b200q_cache_write(b200q_context *, const b200q_cache *cache, const b200q_ten
 int b200q_cache_read(b200q_context *, const b200q_cache *cache, const b200q_tensor *slots, const b200q_tensor *keys, const b200q_tensor *values,
                      char *error, size_t error_capacity);
 
-/* Attention over the cache. queries and output are [rows, heads * head_dim], BF16 or F16; heads is a multiple of the cache's kv_heads,
- * query head h reads cached head h / (heads / kv_heads). pages [sequences, columns] (rows may be strided) gives each sequence's pages, lengths its cached
+/* Attention over the cache. queries and output are [rows, heads * head_dim], BF16 or F16; heads is a multiple of the cache's kv_heads (at
+ * most 2^20 times as many), query head h reads cached head h / (heads / kv_heads). pages [sequences, columns] (rows may be strided) gives each sequence's pages, lengths its cached
  * tokens, those of its query rows included (clamped to 0 .. columns * page_size). query_offsets ([1, sequences + 1], rising from 0) says which rows are a
  * sequence's; without it there is one row per sequence. Row i of n sees positions 0 .. length - n + i; a row that sees nothing is zero; rows behind the
  * last offset are left as they are. With prefix_pages ([1, columns]) and prefix_length ([1, 1]), all rows also see all of that prefix, which is read once for

@@ -44,3 +44,12 @@ def test_outputs_over_the_plan_are_refused():
     assert refused("b200q_rotary", x, positions, rotary, 64, tensor(at - 768, 3, 128)) == ""
     assert "overlaps another operand" in write(rotary=rotary, positions=positions, q=tensor(20000, 3, 128), q_out=out)
     assert "overlaps the cache" in write(small(at=at - 4096), rotary=rotary, positions=positions)
+
+
+def test_groups_of_too_many_heads_are_refused():
+    """Which token a query row belongs to is found by an fp32 product; from 2^23 heads to a cached one on it may name the next."""
+    from tests.test_cache_cpu import attention, cache as small
+    for heads, refusal in ((1 << 20, ""), ((1 << 20) + 1, "2^20 query heads"), (1 << 24, "2^20 query heads")):
+        one = dict(queries=tensor(0, 1, heads * 64), output=tensor(1 << 36, 1, heads * 64), pages=tensor(1 << 37, 1, 5, I32), lengths=tensor(1 << 38, 1, 1, I32))
+        got = attention(small(kv_heads=1, at=1 << 39), **one)
+        assert got == "" if not refusal else refusal in got
