@@ -119,8 +119,8 @@ size_t attention_workspace_bytes(int rows, int sequences, int heads, int kv_head
     return bytes;
 }
 
-void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t workspace_bytes, int *status, int multiprocessors,
-                             cudaStream_t stream) {
+void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t workspace_bytes, int *status, int *pass_word,
+                             int multiprocessors, cudaStream_t stream) {
     const int rows = p.queries.rows, head_dim = p.cache.head_dim, heads = p.queries.cols / head_dim, ctas = multiprocessors;
     const bool prefix = p.prefix_pages != nullptr;
     if (!rows) return;
@@ -144,11 +144,12 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     args.score_scale = p.scale * 1.4426950408889634f;
     args.output_scale = format;
     args.status = status;
+    args.pass_word = prefix ? pass_word : nullptr;
 
     CombineArgs combine{};
     combine.rows = rows, combine.heads = heads, combine.group = args.group, combine.output_stride = p.output.ld();
     combine.row_count = p.query_offsets ? p.query_offsets + p.sequences : nullptr;
-    combine.output = p.output.data, combine.output_scale = format;
+    combine.output = p.output.data, combine.output_scale = format, combine.pass_word = args.pass_word;
     const CUtensorMap keys = cache_map(p.cache.keys, p.cache, 1 << args.box_shift), values = cache_map(p.cache.values, p.cache, 1 << args.box_shift);
     by_type(p.queries.type, p.cache.type, head_dim, [&](auto element, auto format, auto width) {
         using T = decltype(element);

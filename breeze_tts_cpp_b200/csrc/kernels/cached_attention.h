@@ -20,7 +20,8 @@ struct AttentionProblem {
 };
 // Bytes of workspace behind the context's header that a launch uses.
 size_t attention_workspace_bytes(int rows, int sequences, int heads, int kv_heads, int head_dim, bool prefix, int multiprocessors);
-void launch_cached_attention(const AttentionProblem &, void *workspace, size_t workspace_bytes, int *status, int multiprocessors,
+// `status` and `pass_word`: in the workspace's header (quant_linear_workspace.h).
+void launch_cached_attention(const AttentionProblem &, void *workspace, size_t workspace_bytes, int *status, int *pass_word, int multiprocessors,
                              cudaStream_t stream);
 // Part of quant_linear_initialize: the instances' dynamic shared memory, on the current device.
 void raise_attention_limits();

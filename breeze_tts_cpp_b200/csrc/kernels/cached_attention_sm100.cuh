@@ -140,10 +140,7 @@ __global__ void __launch_bounds__(kAttentionThreads, 1)
         ptx::prefetch_tensormap(&key_map);
         ptx::prefetch_tensormap(&value_map);
     }
-    // Dependents may start once what this pass reads is there: the second pass of a call takes that from the first.
-    if (!args.follows) pdl_wait_upstream();
-    pdl_launch_dependents();
-    __syncthreads();
+    begin_pass(args);
 
     // Only the producers need to know where the CTA's share lies; for a long batch all threads find out.
     if (args.sequences > kScanAlone) {
@@ -604,6 +601,7 @@ struct CombineArgs {
     CombineSource source[2];
     int rows, heads, group, output_stride;
     const int *row_count; // last of the query offsets, or null
+    int *pass_word;
     void *output;
     float output_scale;
 };
@@ -695,6 +693,7 @@ template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThread
 template <class T, int HeadDim> __global__ void __launch_bounds__(kCombineThreads) combine_prefixed(const CombineArgs args) {
     pdl_launch_dependents();
     pdl_wait_upstream();
+    if (!blockIdx.x && !threadIdx.x) *args.pass_word = 0; // both passes are over
     const long long index = (long long)blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5);
     const int rows = args.row_count ? min(args.rows, load_index(args.row_count)) : args.rows;
     if (index >= (long long)rows * args.heads) return;

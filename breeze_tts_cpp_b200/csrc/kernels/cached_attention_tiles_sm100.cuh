@@ -154,10 +154,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
     }
     if (warp == kIssuer) ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
     ptx::tcgen05_fence_before();
-    // Dependents may start once what this pass reads is there: the second pass of a call takes that from the first.
-    if (!args.follows) pdl_wait_upstream();
-    pdl_launch_dependents();
-    __syncthreads();
+    begin_pass(args);
     ptx::tcgen05_fence_after();
     const uint32_t tmem = ptx::warp_uniform(tmem_slot);
     if (args.sequences > kScanAlone) start_together<kRows, kManyWarps>(args, kManySegmentUnits, sums, &found);

@@ -8,6 +8,9 @@
 //     __restrict__ reads them by load_upstream16 and its kin (quant_codec.cuh): the compiler may move a plain load in front of the wait.
 // Because every kernel waits for its predecessor to finish before it finishes itself, ordering
 // stays transitive along the whole chain. Outside such a launch both instructions do nothing.
+// One kernel reads and writes before it waits: the second pass of an attention with a shared prefix (begin_pass, cached_attention_work.cuh). It needs
+// what the first pass has waited for and nothing that the first pass writes, and waits before its end like the others. What a kernel's wait promises it
+// gets by a word that the first pass releases behind its own wait, before dependents may start, and that the second acquires; without it, it waits.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdexcept>

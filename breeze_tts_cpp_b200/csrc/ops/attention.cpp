@@ -204,6 +204,6 @@ void cached_attention(const CacheView &cache, const Attention &a) {
     p.scale = a.scale != 0.f ? a.scale : 1.f / std::sqrt(float(cache.head_dim));
     launch_cached_attention(p, static_cast<char *>(gpu.gemm_workspace.data()) + quant_linear_header_bytes(),
                             gpu.gemm_workspace.size() - quant_linear_header_bytes(), quant_linear_status_word(gpu.gemm_workspace.data()),
-                            gpu.multiprocessors, gpu.stream);
+                            attention_pass_word(gpu.gemm_workspace.data()), gpu.multiprocessors, gpu.stream);
 }
 } // namespace tts::ops

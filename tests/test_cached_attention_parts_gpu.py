@@ -46,3 +46,47 @@ def test_many_parts_without_a_pause(heads, kv_heads, head_dim, prefix):
         torch.cuda.synchronize()
         assert context.status() == 0 and all(torch.equal(out, first) for out in outs)
     context.close()
+
+
+@pytest.mark.parametrize("counts", [None, [40, 33, 7]])
+def test_prefix_behind_its_producers_without_a_pause(counts):
+    """The second pass of a call starts before the first is over, yet behind everything that the call reads: queries, keys and lengths that the launch in
+    front of it has just written, in the same buffers step after step."""
+    lengths = [200, 150, 90]
+    batch = Batch(41, lengths, counts, heads=8, kv_heads=4, head_dim=128, page=64, prefix=600)
+    rows, steps = batch.q.shape[0], 60
+    g = torch.Generator().manual_seed(2)
+    queries = torch.randn(steps, *batch.q.shape, generator=g).bfloat16().cuda()
+    keys = torch.randn(steps, rows, 4 * 128, generator=g).bfloat16().cuda()
+    # Every step's rows go to the first slots of the prefix, which all queries read, and of the sequences.
+    places = torch.cat((batch.prefix_pages[:9].long()[:, None] * 64 + torch.arange(64), batch.pages[:, :1].long() * 64 + torch.arange(64))).flatten()
+    slots = torch.stack([places[torch.randperm(len(places), generator=g)[:rows]] for _ in range(steps)]).to(torch.int32).cuda()
+    positions, rotary = torch.arange(rows, dtype=torch.int32, device="cuda"), ops.Rotary.plan(128)
+    stored = [getattr(batch.cache, n).clone() for n in ("keys", "values", "key_scales", "value_scales")]
+    context = ops.Context("int8", workspace_bytes=64 << 20)
+    q, out, pages = torch.empty_like(queries[0]), batch.out.cuda(), batch.pages.cuda()
+    of = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    offsets = None if counts is None else torch.tensor(batch.offsets, dtype=torch.int32, device="cuda")
+    prefix_pages, prefix_length = batch.prefix_pages.cuda(), batch.prefix_length.cuda()
+
+    def run(pause):
+        for n, x in zip(("keys", "values", "key_scales", "value_scales"), stored):
+            getattr(batch.cache, n).copy_(x)
+        outs = torch.zeros(steps, *out.shape, dtype=out.dtype, device="cuda")
+        torch.cuda.synchronize()
+        for i in range(steps):
+            context.cache_write(batch.cache, keys[i], keys[i], slots[i], positions, rotary, queries[i], q)
+            if pause:
+                torch.cuda.synchronize()
+            context.cached_attention(q, batch.cache, pages, of, outs[i], query_offsets=offsets, prefix_pages=prefix_pages, prefix_length=prefix_length)
+            if pause:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        assert context.status() == 0
+        return outs
+
+    want = run(True)
+    assert torch.isfinite(want).all() and not torch.equal(want[0], want[1])
+    for _ in range(5):
+        assert torch.equal(run(False), want)
+    context.close()
