@@ -53,3 +53,18 @@ def test_groups_of_too_many_heads_are_refused():
         one = dict(queries=tensor(0, 1, heads * 64), output=tensor(1 << 36, 1, heads * 64), pages=tensor(1 << 37, 1, 5, I32), lengths=tensor(1 << 38, 1, 1, I32))
         got = attention(small(kv_heads=1, at=1 << 39), **one)
         assert got == "" if not refusal else refusal in got
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("heads,kv_heads,tokens", [(16, 8, 1), (32, 1, 1), (8, 1, 4), (64, 2, 1), (16, 8, 16)])
+def test_steps_that_a_default_context_is_enough_for(heads, kv_heads, tokens, head_dim):
+    """Without a prefix, and with up to 32 query rows to a cached head and sequence."""
+    from breeze_tts_cpp_b200 import ops
+    for sequences in (1, 64, 10000):
+        assert ops.attention_workspace(tokens * sequences, sequences, heads, kv_heads, head_dim) <= 8 << 20
+
+
+def test_steps_that_ask_for_more():
+    from breeze_tts_cpp_b200 import ops
+    assert ops.attention_workspace(1, 1, 64, 1, 128) > 8 << 20  # 64 heads to a cached one take partial sums of 64 rows
+    assert ops.attention_workspace(64, 64, 16, 8, 128, prefix=True) > 8 << 20
