@@ -2,10 +2,11 @@
 //
 // Mathematics. Keys and values are bytes with one fp32 scale per token, so s_j = (q . kq_j) ks_j times the softmax scale, and the output is
 // sum p_j vs_j vq_j / sum p_j. The products run on the tensor cores in fp16 with fp32 sums: an INT8 byte is exact in fp16, and so is an
-// e4m3 byte times 2^-8 (its bits shifted into place; the factor goes into the score's and the output's scale). Queries are exact too: each
-// row is divided by the power of two of its largest element. What is rounded is p_j vs_j, to fp16. To keep that product in fp16's
-// range whatever the scales are, the running maximum is taken over log2 p_j vs_j, so the product is at most one; the sum of p_j
-// alone uses the same reference and is fp32.
+// e4m3 byte times 2^-8 (its bits shifted into place; the factor goes into the score's and the output's scale). Two things are rounded.
+// BF16 queries (F16 ones enter as they are): a row is divided by the power of two of its largest element, which leaves elements down to 2^-17 of that
+// power exact and rounds those below to within 2^-25 of it; a product in bf16 would keep them, but four bytes take eight instructions to become that, not five. And
+// p_j vs_j, to fp16: to keep that product in fp16's range whatever the scales are, the running maximum is taken over log2 p_j vs_j, so it is at most
+// one; the sum of p_j alone uses the same reference and is fp32.
 //
 // Layout. S is computed transposed: 16 keys are the rows of an m16n8k16 product and 8 query rows its columns, so a decode step with two
 // query rows per cached head wastes 6 columns of 8, not 14 of 16. The order of the contraction over head_dim is free, so a thread's

@@ -1,8 +1,9 @@
 // Attention of many query rows over the quantized, paged cache: chunks of prompts, and a prefix that a whole batch shares.
 //
-// Mathematics: as for few query rows (cached_attention_sm100.cuh). Scores and outputs are fp16 products with fp32 sums on the tensor cores,
-// bytes enter them exactly, and what is rounded is p_j vs_j, to fp16, against a running reference that keeps it at most 256. The reference moves only
-// when a tile's maximum passes it by 2^8, so that the accumulated output is rescaled hardly ever.
+// Mathematics: as for few query rows (cached_attention_sm100.cuh). Scores and outputs are fp16 products with fp32 sums on the tensor cores, and
+// bytes enter them exactly. Rounded are BF16 queries more than 2^17 below their row's largest, to within 2^-25 of its power of two, and p_j vs_j, to
+// fp16, against a running reference that keeps it at most 256. The reference moves only when a tile's maximum passes it by 2^8, so that the
+// accumulated output is rescaled hardly ever.
 //
 // Layout. A segment is 128 query rows of one cached head (tokens times the group's heads; of a prefix: of all sequences), a tile 128 keys. Per tile
 // a CTA does S = Q K^T and O += P V as tcgen05.mma, with S, P and O in tensor memory; P overwrites S, two halves to a column. Two teams of eight

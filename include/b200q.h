@@ -221,7 +221,8 @@ int b200q_cache_read(b200q_context *, const b200q_cache *cache, const b200q_tens
  * sequence's; without it there is one row per sequence. Row i of n sees positions 0 .. length - n + i; a row that sees nothing is zero; rows behind the
  * last offset are left as they are. With prefix_pages ([1, columns]) and prefix_length ([1, 1]), all rows also see all of that prefix, which is read once for
  * the whole batch; positions in lengths and pages then count from behind it. scale 0 means 1 / sqrt(head_dim). A position on a page that the cache does
- * not have reads as NaN. The maximum, the sums and the output are kept in fp32; weights are rounded to fp16 for the second product.
+ * not have reads as NaN. The maximum, the sums and the output are kept in fp32; weights are rounded to fp16 for the second product,
+ * and BF16 queries for the first: elements more than 2^17 below the largest of their row of a head are taken to within 2^-25 of that one's power of two.
  * Scores are fp32: where a row's exceed about 2^20 in magnitude, their rounding alone decides it, and it may come out as zeros or NaN (no other row does).
  * e4m3's code for NaN in a cached value reads as 480: b200q_cache_write marks rows that are no numbers in their scales instead.
  * Uses the context's workspace behind its header (b200q_attention_workspace bytes in all), so graphs captured from one context must not run
