@@ -30,6 +30,9 @@ CUtensorMap cache_map(const void *base, const CacheView &cache, int box_rows) {
 // Query rows of a cached head up to which segments of at most sixteen are used, several to a sequence, each of which reads the cache again. From
 // 17 to 32 rows that takes 19.7 us against 21.6 with a segment of 128 (four sequences of up to 8000, up to six tokens, groups of eight), for a prefix's 24 rows
 // 27.3 against 28.2; with more it falls behind (16 sequences of up to 2000, 40 rows on the average: 55 against 36).
+// The offsets are on the device, so the batch's average decides for all of its sequences, and these figures are of batches whose sequences are alike. Decode rows
+// beside a chunk of a prompt are served badly either way: 64 sequences of one token (200 to 2000 long) and a chunk of 700 take 145 us in one call, 79 in
+// two; 60 and two chunks of 1024 145 and 110; 64 and a chunk of 200 82 and 68 (16 heads over 8, 128 wide, INT8). Callers are told to make two calls.
 constexpr int kFewRows = 32;
 constexpr size_t kPiece = 256; // parts of the workspace start on multiples of this
 size_t padded(size_t bytes) { return (bytes + kPiece - 1) / kPiece * kPiece; }

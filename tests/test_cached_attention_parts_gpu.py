@@ -90,3 +90,13 @@ def test_prefix_behind_its_producers_without_a_pause(counts):
     for _ in range(5):
         assert torch.equal(run(False), want)
     context.close()
+
+
+@pytest.mark.parametrize("counts", [[1] * 9 + [70] + [1] * 3, [1, 200, 0, 1, 90, 1], [300] + [1] * 30])
+@pytest.mark.parametrize("prefix", [None, 90])
+def test_decode_rows_beside_chunks_of_prompts(ctx_factory, counts, prefix):
+    """One call for both; the batch's average says which kernel takes it: the first and third the one for few rows, the second the other."""
+    g = torch.Generator().manual_seed(len(counts))
+    lengths = [n + int(torch.randint(0, 200, (1,), generator=g)) for n in counts]
+    batch = Batch(42, lengths, counts, heads=4, kv_heads=2, head_dim=64, page=16, prefix=prefix, spare_rows=2)
+    check(batch.run(ctx_factory("int8")), *batch.want())
