@@ -1,5 +1,6 @@
 // Host side of the attention over the quantized cache: workspace, tensor maps, choice of the instance.
 #include "kernels/cached_attention.h"
+#include "kernels/cache_dispatch.h"
 #include "kernels/cached_attention_tiles_sm100.cuh"
 #include "kernels/tensor_map.h"
 #include <algorithm>
@@ -9,11 +10,6 @@ namespace tts {
 namespace {
 using namespace b200;
 
-int shift_of(int power) {
-    int s = 0;
-    while ((1 << s) < power) ++s;
-    return s;
-}
 CUtensorMap cache_map(const void *base, const CacheView &cache, int box_rows) {
     CUtensorMap map;
     cuuint64_t dims[2] = {cuuint64_t(cache.head_dim), cuuint64_t(cache.rows())};
@@ -81,22 +77,6 @@ void launch_pass(bool narrow, int most_columns, const AttentionArgs &args, const
     if (narrow) launch_pass<T, F, HeadDim, 1>(args, most_columns, keys, values, ctas, stream);
     else launch_pass<T, F, HeadDim, 2>(args, most_columns, keys, values, ctas, stream);
 }
-// Calls f(element, format, head width) with the run-time types as compile-time ones.
-template <class Call> void by_type(Type element, Type format, int head_dim, Call &&call) {
-    auto width = [&](auto t, auto f) {
-        if (head_dim == 64) call(t, f, std::integral_constant<int, 64>{});
-        else call(t, f, std::integral_constant<int, 128>{});
-    };
-    auto storage = [&](auto t) {
-        if (format == Type::I8) width(t, std::integral_constant<Type, Type::I8>{});
-        else width(t, std::integral_constant<Type, Type::FP8>{});
-    };
-    if (element == Type::F16) storage(__half{});
-    else storage(__nv_bfloat16{});
-}
-bool aligned16(const TensorView &v) {
-    return reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && (v.rows <= 1 || v.ld() % 8 == 0);
-}
 template <class T, Type F, int HeadDim> void raise_limit() {
     auto raise = [](auto *kernel, size_t bytes) {
         const cudaError_t status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
@@ -135,8 +115,8 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     args.query_stride = p.queries.ld(), args.output_stride = p.output.ld();
     args.rows = rows, args.heads = heads, args.kv_heads = p.cache.kv_heads, args.group = heads / p.cache.kv_heads;
     args.group_inverse = 1.f / float(args.group);
-    args.aligned = aligned16(p.queries) && aligned16(p.output);
-    args.sectors = args.aligned && reinterpret_cast<uintptr_t>(p.output.data) % 32 == 0 && p.output.ld() % 16 == 0;
+    args.aligned = rows_start_on(16, p.queries) && rows_start_on(16, p.output);
+    args.sectors = args.aligned && rows_start_on(32, p.output);
     args.pages = p.pages, args.lengths = p.lengths, args.query_offsets = p.query_offsets;
     args.sequences = p.sequences, args.page_columns = p.page_columns, args.page_stride = p.page_stride;
     args.page_shift = shift_of(p.cache.page_size), args.total_pages = p.cache.pages, args.offset_count = p.sequences;
@@ -153,7 +133,11 @@ void launch_cached_attention(const AttentionProblem &p, void *workspace, size_t 
     combine.rows = rows, combine.heads = heads, combine.group = args.group, combine.output_stride = p.output.ld();
     combine.row_count = p.query_offsets ? p.query_offsets + p.sequences : nullptr;
     combine.output = p.output.data, combine.output_scale = format, combine.pass_word = args.pass_word;
-    const CUtensorMap keys = cache_map(p.cache.keys, p.cache, 1 << args.box_shift), values = cache_map(p.cache.values, p.cache, 1 << args.box_shift);
+    CUtensorMap keys{}, values{}; // of the kernel for few rows
+    if (!plan_pass(rows, p.sequences, args.group, false).many || (prefix && !plan_pass(rows, p.sequences, args.group, true).many)) {
+        keys = cache_map(p.cache.keys, p.cache, 1 << args.box_shift);
+        values = cache_map(p.cache.values, p.cache, 1 << args.box_shift);
+    }
     by_type(p.queries.type, p.cache.type, head_dim, [&](auto element, auto format, auto width) {
         using T = decltype(element);
         char *base = static_cast<char *>(workspace);

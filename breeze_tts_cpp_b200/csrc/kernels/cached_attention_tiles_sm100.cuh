@@ -72,13 +72,6 @@ __device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t 
 }
 // 16-byte chunk `chunk` of row `row` in a K-major operand panel (rows of 64 halves, 128-byte swizzle).
 __device__ __forceinline__ uint32_t panel_at(int row, int chunk) { return uint32_t(row * 128 + ((chunk ^ (row & 7)) << 4)); }
-// 32 bytes at once: a thread has a row, so narrower stores would write parts of sectors.
-__device__ __forceinline__ void store_sector(void *to, const float (&v)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])),
-                 "r"(__float_as_uint(v[2])), "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])), "r"(__float_as_uint(v[6])),
-                 "r"(__float_as_uint(v[7]))
-                 : "memory");
-}
 template <class T> __device__ __forceinline__ void store_row16(const AttentionArgs &a, T *to, const float (&v)[16], float factor) {
     union {
         float words[8];
@@ -88,7 +81,7 @@ template <class T> __device__ __forceinline__ void store_row16(const AttentionAr
 #pragma unroll
     for (int i = 0; i < 16; ++i) out.e[i] = T(v[i] * factor);
     if (a.sectors) {
-        store_sector(to, out.words);
+        ptx::store_sector(to, out.words);
     } else if (a.aligned) {
         reinterpret_cast<uint4 *>(to)[0] = out.fours[0];
         reinterpret_cast<uint4 *>(to)[1] = out.fours[1];
@@ -627,7 +620,7 @@ __global__ void __launch_bounds__(kManyThreads, 1) cached_attention_many(const A
                 for (int e = 0; e < 16; ++e) v[e] = factor[0] * __uint_as_float(o[0][e]) + factor[1] * __uint_as_float(o[1][e]);
                 if (kept) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 8) store_sector(kept + c + e, *reinterpret_cast<const float(*)[8]>(v + e));
+                    for (int e = 0; e < 16; e += 8) ptx::store_sector(kept + c + e, *reinterpret_cast<const float(*)[8]>(v + e));
                 } else {
                     store_row16(args, static_cast<T *>(args.output) + at_row * args.output_stride + size_t(head) * HeadDim + c, v, scale);
                 }

@@ -6,6 +6,7 @@
 #pragma once
 #include "core/tensor.h"
 #include "kernels/launch.cuh"
+#include "kernels/quant_codec.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <climits>
@@ -50,17 +51,12 @@ struct AttentionArgs {
     int *status;
 };
 
-__device__ __forceinline__ int load_index(const int *p) {
-    int v;
-    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
 // The start of a pass, by all threads of a CTA; a barrier of the CTA among it. Dependents may start once what this pass reads is there.
 __device__ __forceinline__ void begin_pass(const AttentionArgs &a) {
     if (a.follows) {
         // What came before the call was over (and its writes there for every proxy) when a thread of the first pass came out of its wait, released the word
         // and let this pass start. All CTAs of the first have to let it, so the word is there. A wait for all of the first pass instead takes 24 sequences
-        // behind 509 tokens from 14.8 to 20.9 us and 128 behind 16384 from 85.0 to 92.0; the word costs 0.1 and 0.6.
+        // behind 509 tokens from 14.8 to 20.9 us and 128 behind 16384 from 85.3 to 92.0; the word itself costs 0.1 us at most.
         int word = 0;
         if (threadIdx.x == blockDim.x - 32) // the others set the CTA up meanwhile
             asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(word) : "l"(a.pass_word) : "memory");

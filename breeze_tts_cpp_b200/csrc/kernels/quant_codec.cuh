@@ -56,7 +56,7 @@ __device__ __forceinline__ float rotation_sign(uint32_t column) {
     return ((h ^ (h >> 16)) & 1u) ? 1.f : -1.f;
 }
 
-// 16 bytes, or one 16-bit element, of what an upstream kernel wrote. The compiler may take a plain load through a pointer to const
+// 16 bytes, one 16-bit element, or one int, of what an upstream kernel wrote. The compiler may take a plain load through a pointer to const
 // __restrict__ out of a loop, wait on upstream or not; these stay behind the wait.
 __device__ __forceinline__ uint4 load_upstream16(const void *p) {
     uint4 r;
@@ -71,6 +71,11 @@ template <class T> __device__ __forceinline__ T load_upstream(const T *p) {
     } r{};
     asm volatile("ld.global.b16 %0, [%1];" : "=h"(r.bits) : "l"(p) : "memory");
     return r.value;
+}
+__device__ __forceinline__ int load_index(const int *p) {
+    int v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
 }
 // Eight consecutive 16-bit elements of an upstream kernel -> fp32. `aligned` selects one 128-bit load; otherwise (odd
 // pointers, ragged row ends) elements are fetched one by one and missing ones read as zero.

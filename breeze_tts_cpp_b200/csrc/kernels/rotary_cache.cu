@@ -10,19 +10,16 @@
 // row, while its loads are in flight. A thread takes 16 columns of a head, two blocks of eight that hold both partners of its pairs, so no pair
 // crosses lanes; a head's scale and norm reduce over the 4 or 8 lanes that share it.
 #include "kernels/rotary_cache.h"
+#include "kernels/cache_dispatch.h"
 #include "kernels/launch.cuh"
 #include "kernels/quant_codec.cuh"
+#include "kernels/sm100_ptx.cuh"
 #include <algorithm>
 
 namespace tts {
 namespace {
 using namespace b200;
 
-__device__ __forceinline__ int load_index(const int *p) {
-    int v;
-    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
 template <class T> __device__ __forceinline__ void store8(T *p, bool aligned, const float (&v)[8]) {
     union {
         uint4 word;
@@ -288,9 +285,7 @@ template <class T> __device__ __forceinline__ void store16(T *p, bool sectors, b
     } out;
 #pragma unroll
     for (int i = 0; i < 8; ++i) out.e[i] = T(a[i]), out.e[8 + i] = T(b[i]);
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(out.words[0]), "r"(out.words[1]), "r"(out.words[2]),
-                 "r"(out.words[3]), "r"(out.words[4]), "r"(out.words[5]), "r"(out.words[6]), "r"(out.words[7])
-                 : "memory");
+    ptx::store_sector(p, out.words);
 }
 // A thread takes 16 columns of a head, of keys and values: both 16-byte loads are in flight together. 1021 rows written and 8190 read back
 // (8 heads 128 wide, e4m3): 18.0 us for 66 MB in two launches, 3.6 TB/s; two rows a thread took 21.5, 16-byte stores 20.9.
@@ -329,23 +324,12 @@ template <class T, Type F, int HeadDim> __global__ void __launch_bounds__(256) r
     }
 }
 
-bool aligned16(const TensorView &v) {
-    return !v.data || (reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && (v.rows <= 1 || v.ld() % 8 == 0));
-}
-bool aligned32(const TensorView &v) {
-    return !v.data || (reinterpret_cast<uintptr_t>(v.data) % 32 == 0 && (v.rows <= 1 || v.ld() % 16 == 0));
-}
-int shift_of(int power) {
-    int s = 0;
-    while ((1 << s) < power) ++s;
-    return s;
-}
 Turning turning_of(const RotaryView &r) { return {r.turns, r.turns ? r.dims / 2 : 0, r.scale}; }
 
 template <class T>
 void rotate(TensorView input, TensorView output, const int *positions, RotaryView rotary, int head_dim, cudaStream_t stream) {
     RotaryArgs<T> args{input.ptr<T>(), output.ptr<T>(), input.rows, input.ld(), output.ld(), head_dim / 16, input.cols / 16,
-                       aligned16(input) && aligned16(output), positions, turning_of(rotary)};
+                       rows_start_on(16, input) && rows_start_on(16, output), positions, turning_of(rotary)};
     const int warps = std::clamp(input.rows / 128, 1, kRotaryWarps); // few rows spread over the multiprocessors
     launch_pdl("rotary", rotary.interleaved ? rotary_rows<T, true> : rotary_rows<T, false>, dim3(unsigned((input.rows + warps - 1) / warps)),
                dim3(unsigned(32 * warps)), 0, stream, args);
@@ -358,19 +342,6 @@ template <class T, Type F, int HeadDim> void write(const WriteArgs<T> &args, boo
 template <class T, Type F, int HeadDim> void read(const ReadArgs<T> &args, cudaStream_t stream) {
     const unsigned ctas = unsigned((args.rows + args.rows_per_cta - 1) / args.rows_per_cta);
     launch_pdl("cache read", read_rows<T, F, HeadDim>, dim3(ctas), dim3(256), 0, stream, args);
-}
-// Calls f(element, format, head width) with the run-time types as compile-time ones.
-template <class Call> void by_type(Type element, Type format, int head_dim, Call &&call) {
-    auto width = [&](auto t, auto f) {
-        if (head_dim == 64) call(t, f, std::integral_constant<int, 64>{});
-        else call(t, f, std::integral_constant<int, 128>{});
-    };
-    auto storage = [&](auto t) {
-        if (format == Type::I8) width(t, std::integral_constant<Type, Type::I8>{});
-        else width(t, std::integral_constant<Type, Type::FP8>{});
-    };
-    if (element == Type::F16) storage(__half{});
-    else storage(__nv_bfloat16{});
 }
 } // namespace
 
@@ -391,8 +362,8 @@ void launch_cache_write(CacheView cache, TensorView keys, TensorView values, con
         args.query_norm = query_norm.ptr<T>(), args.key_norm = key_norm.ptr<T>(), args.query_output = query_output.ptr<T>();
         args.query_stride = queries.ld(), args.key_stride = keys.ld(), args.value_stride = values.ld();
         args.output_stride = query_output.ld();
-        args.aligned = aligned16(queries) && aligned16(keys) && aligned16(values) && aligned16(query_norm) && aligned16(key_norm) &&
-                       aligned16(query_output);
+        args.aligned = rows_start_on(16, queries) && rows_start_on(16, keys) && rows_start_on(16, values) && rows_start_on(16, query_norm) && rows_start_on(16, key_norm) &&
+                       rows_start_on(16, query_output);
         args.query_heads = queries.data ? queries.cols / cache.head_dim : 0;
         args.kv_heads = cache.kv_heads, args.page_shift = shift_of(cache.page_size), args.slots = unsigned(cache.slots());
         args.cached_keys = static_cast<unsigned char *>(cache.keys), args.cached_values = static_cast<unsigned char *>(cache.values);
@@ -413,8 +384,8 @@ void launch_cache_read(CacheView cache, const int *slots, TensorView keys, Tenso
         args.keys = keys.ptr<T>(), args.values = values.ptr<T>(), args.key_stride = keys.ld(), args.value_stride = values.ld();
         args.rows = any.rows, args.kv_heads = cache.kv_heads, args.page_shift = shift_of(cache.page_size);
         args.per_row = std::min(256, cache.kv_heads * cache.head_dim / 16), args.rows_per_cta = 256 / args.per_row;
-        args.aligned = aligned16(keys) && aligned16(values);
-        args.sectors = aligned32(keys) && aligned32(values), args.slots = unsigned(cache.slots()), args.slot_of = slots;
+        args.aligned = rows_start_on(16, keys) && rows_start_on(16, values);
+        args.sectors = rows_start_on(32, keys) && rows_start_on(32, values), args.slots = unsigned(cache.slots()), args.slot_of = slots;
         read<T, decltype(format)::value, decltype(width)::value>(args, stream);
     });
 }

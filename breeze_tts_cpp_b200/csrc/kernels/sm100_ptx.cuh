@@ -17,6 +17,15 @@ __device__ __forceinline__ uint32_t smem_u32(const void *p) {
 __device__ __forceinline__ uint32_t warp_uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ int warp_index() { return int(warp_uniform(threadIdx.x >> 5)); }
 
+// 32 bytes at once to a multiple of 32: lanes that have a row, or a piece of one, each then write whole sectors.
+__device__ __forceinline__ uint32_t word_of(uint32_t v) { return v; }
+__device__ __forceinline__ uint32_t word_of(float v) { return __float_as_uint(v); }
+template <class T> __device__ __forceinline__ void store_sector(void *to, const T (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(word_of(v[0])), "r"(word_of(v[1])), "r"(word_of(v[2])),
+                 "r"(word_of(v[3])), "r"(word_of(v[4])), "r"(word_of(v[5])), "r"(word_of(v[6])), "r"(word_of(v[7]))
+                 : "memory");
+}
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
