@@ -1,5 +1,5 @@
-"""The few-rows attention with many parts to a multiprocessor, call after call without a pause: its merge buffers change hands all the time, while
-one of the two merging warps has less to do than the other, or nothing."""
+"""Cached attention as a server calls it: many parts to a multiprocessor, call after call without a pause, decode rows beside prompts, graphs in turn,
+pages that are shared, offsets that are none."""
 import pytest
 import torch
 
@@ -29,6 +29,7 @@ def some_of(batch, first, sequences):
     (8, 8, 64, None), (16, 8, 64, None), (8, 8, 128, None), (16, 8, 128, None), (24, 8, 64, None), (24, 8, 128, None), (32, 8, 64, None),
     (32, 8, 128, None), (8, 8, 64, 70), (16, 8, 64, 300), (16, 8, 128, 70)])
 def test_many_parts_without_a_pause(heads, kv_heads, head_dim, prefix):
+    """The few-rows kernel's merge buffers change hands all the time, while one of its two merging warps has less to do than the other, or nothing."""
     g = torch.Generator().manual_seed(heads + head_dim)
     lengths = torch.randint(1, 300, (1100,), generator=g).tolist()
     batch = Batch(40, lengths, None, heads=heads, kv_heads=kv_heads, head_dim=head_dim, page=64, prefix=prefix)
@@ -100,3 +101,79 @@ def test_decode_rows_beside_chunks_of_prompts(ctx_factory, counts, prefix):
     lengths = [n + int(torch.randint(0, 200, (1,), generator=g)) for n in counts]
     batch = Batch(42, lengths, counts, heads=4, kv_heads=2, head_dim=64, page=16, prefix=prefix, spare_rows=2)
     check(batch.run(ctx_factory("int8")), *batch.want())
+
+
+def test_two_graphs_of_one_context_in_turn():
+    """Both use the context's workspace, one behind the other: a prefix's two passes, chunks, and eager steps between their replays."""
+    side = torch.cuda.Stream()
+    context = ops.Context("int8", stream=side, workspace_bytes=64 << 20)
+    batches = [Batch(43, [90, 400, 33], None, heads=8, kv_heads=4, prefix=500), Batch(44, [150, 80], [60, 80], heads=4, kv_heads=2),
+               Batch(45, [700, 2, 90, 129], None, heads=4, kv_heads=4, head_dim=64)]
+    calls, want = [], []
+    for batch in batches:
+        q, pages, out = batch.q.cuda(), batch.pages.cuda(), batch.out.cuda()
+        lengths = torch.tensor(batch.lengths, dtype=torch.int32, device="cuda")
+        more = {} if batch.offsets is None else {"query_offsets": torch.tensor(batch.offsets, dtype=torch.int32, device="cuda")}
+        if batch.prefix_pages is not None:
+            more.update(prefix_pages=batch.prefix_pages.cuda(), prefix_length=batch.prefix_length.cuda())
+        calls.append((out, lambda a=(q, batch.cache, pages, lengths, out), more=more: context.cached_attention(*a, **more)))
+    torch.cuda.synchronize()
+    graphs = []
+    with torch.cuda.stream(side):
+        for (out, call), batch in zip(calls, batches):
+            call()
+            side.synchronize()
+            check(out, *batch.want())
+            want.append(out.clone())
+        for _, call in calls[:2]:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                call()
+        for out, _ in calls:
+            out.fill_(5.0)
+        for _ in range(100):
+            graphs[0].replay()
+            graphs[1].replay()
+            calls[2][1]()
+            graphs[0].replay()
+            calls[1][1]()
+    torch.cuda.synchronize()
+    assert context.status() == 0 and all(torch.equal(out, w) for (out, _), w in zip(calls, want))
+    graphs.clear()
+    context.close()
+
+
+def test_many_sequences_of_many_rows(ctx_factory):
+    """More sequences than a warp adds up by itself, for the kernel of many rows."""
+    g = torch.Generator().manual_seed(6)
+    counts = torch.randint(0, 45, (300,), generator=g).tolist()
+    batch = Batch(46, [n + b % 90 for b, n in enumerate(counts)], counts, heads=2, kv_heads=1, head_dim=64, page=16, spare_rows=1)
+    assert sum(counts) * 2 > 32 * len(counts)
+    check(batch.run(ctx_factory("int8")), *batch.want())
+
+
+@pytest.mark.parametrize("counts", [None, [40, 20, 33]])
+def test_pages_that_several_sequences_name(ctx_factory, counts):
+    """The same page in several tables, twice in one, and in the prefix."""
+    batch = Batch(47, [100, 80, 64], counts, heads=4, kv_heads=2, head_dim=64, page=16, prefix=64)
+    batch.pages[1, :5] = batch.pages[0, :5]
+    batch.pages[2, :4] = batch.pages[0, 2]
+    batch.prefix_pages[1] = batch.pages[0, 3]
+    batch.prefix_pages[3] = batch.pages[0, 3]
+    check(batch.run(ctx_factory("int8")), *batch.want())
+
+
+@pytest.mark.parametrize("counts,prefix", [([60, 50, 40], None), ([60, 50, 40], 100), ([2, 2, 2], 100)])
+def test_offsets_that_are_none(ctx_factory, counts, prefix):
+    """Whatever offsets name, nothing outside of the rows is written and nothing waits for good; calls with right ones are right again."""
+    batch = Batch(48, [n + 60 for n in counts], counts, heads=4, kv_heads=2, head_dim=64, page=16, prefix=prefix, spare_rows=4)
+    ctx, rows = ctx_factory("int8"), batch.q.shape[0]
+    lengths, held = torch.tensor(batch.lengths, dtype=torch.int32, device="cuda"), torch.full((rows + 4, 256), 5.0, dtype=batch.q.dtype, device="cuda")
+    more = {} if prefix is None else {"prefix_pages": batch.prefix_pages.cuda(), "prefix_length": batch.prefix_length.cuda()}
+    half = rows // 2
+    for offsets in ([0, rows, 2, half], [0, 2, half, 10**6], [-3, 2, half, rows], [rows, half, 2, 0], [2**31 - 1, -(2**31), 5, 5], [half, half + 1, rows, rows]):
+        ctx.cached_attention(batch.q.cuda(), batch.cache, batch.pages.cuda(), lengths, held[2: 2 + rows],
+                             query_offsets=torch.tensor(offsets, dtype=torch.int32, device="cuda"), **more)
+        torch.cuda.synchronize()
+        assert ctx.status() == 0 and (held[:2] == 5).all() and (held[2 + rows:] == 5).all()
+    check(batch.run(ctx), *batch.want())
